@@ -331,6 +331,57 @@ int unit_conv_chain_u8_ws(const unit_chain_layer *layers, int32_t count, const v
 int unit_conv_chain_u8_status(const unit_chain_layer *layers, int32_t count, const void *x, void *ws, size_t ws_bytes,
                               int32_t *status, unit_stream_t stream);
 
+/* ------------------------------------------------------------------ MXFP4
+ * Rows of 4-bit floats (sign, two exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6); 32 consecutive elements of a
+ * row share a scale 2^(s - 127), s one byte, 255 for a block that is NaN throughout (the OCP microscaling formats' MXFP4).  No
+ * counterpart in the reference, whose 8-bit products these stand beside.
+ *
+ * In the buffers of these calls (unit_mxfp4_bytes says their sizes; 16-byte aligned) a row's codes fill kb * 128 bytes,
+ * kb = K / 256 rounded up, the even element of a pair in the low half of its byte, zeros behind K; the scale of block b of a row
+ * lies at [b / 8][b % 2][row][(b % 8) / 2] of [kb][2][rows][4]: a lane's four scales of a 128-byte stage are one dword. */
+enum { UNIT_F32 = 0, UNIT_F16 = 1, UNIT_BF16 = 2, UNIT_MXFP4 = 3 };
+
+int unit_mxfp4_bytes(int64_t rows, int32_t K, size_t *codes, size_t *scales);
+
+/* x (rows, K), contiguous, aligned to its elements.  A block's scale is the power of two below its largest magnitude, divided by
+ * 4 (at least 2^-127); elements are x / scale, rounded to the nearest element, ties to the even mantissa, magnitudes above 6 to
+ * 6.  A block with an infinity or a NaN takes scale 255. */
+int unit_quantize_mxfp4(const void *x, int32_t dtype, int64_t rows, int32_t K, void *codes, void *scales, unit_stream_t stream);
+/* The values that codes and scales stand for, (rows, K), rounded once where dtype does not hold them. */
+int unit_dequantize_mxfp4(const void *codes, const void *scales, int64_t rows, int32_t K, void *out, int32_t dtype,
+                          unit_stream_t stream);
+/* A checkpoint's storage into these buffers: codes_in (rows, 16 * b) and scales_in (rows, b), b = K / 32 rounded up, row-major,
+ * aligned to nothing; codes behind K are dropped. */
+int unit_prepare_mxfp4(const void *codes_in, const void *scales_in, int64_t rows, int32_t K, void *codes, void *scales,
+                       unit_stream_t stream);
+
+/* out (M, N) = q(x) . W^T, products and sums in fp32 on v_mfma_scale_f32_32x32x64_f8f6f4, rounded once to out_dtype.  x either
+ * (M, K) floats (x_dtype UNIT_F32, UNIT_F16, UNIT_BF16; xscales ignored), quantised on the way as unit_quantize_mxfp4 does, with
+ * a workspace of unit_mxfp4_workspace_bytes (16-byte aligned, of any contents), or codes and scales (UNIT_MXFP4, no workspace). */
+int unit_mxfp4_workspace_bytes(int32_t rows, int32_t K, size_t *bytes);
+int unit_dense_mxfp4(const void *x, const void *xscales, int32_t x_dtype, const void *wcodes, const void *wscales, void *out,
+                     int32_t out_dtype, int32_t M, int32_t N, int32_t K, void *ws, size_t ws_bytes, unit_stream_t stream);
+
+/* ------------------------------------------------------------------ products grouped by expert
+ * Rows sorted by group: sizes[0] rows of group 0, then sizes[1] of group 1, ...; sizes are `groups` int32 or int64 (size_bytes
+ * 4 or 8) in device memory, read when the work runs.  A size counts as min(max(size, 0), rows left); rows behind the last
+ * group's belong to none and give zeros.  Row operands may pass 2^31 bytes, a group's weight may not.  rows may be 0.
+ * 16-bit operands: N and K multiples of 8, pointers 16-byte aligned; sums in fp32, rounded once to out_dtype.
+ *
+ * forward: out (rows, N), out[r] = w[g(r)] x[r], w (groups, N, K) */
+int unit_grouped_dense(const void *x, const void *w, const void *sizes, int32_t size_bytes, void *out, int32_t dtype,
+                       int32_t out_dtype, int32_t rows, int32_t groups, int32_t N, int32_t K, unit_stream_t stream);
+/* its gradients for dy (rows, N): dx (rows, K), dx[r] = w[g(r)]^T dy[r]; dw (groups, N, K), dw[g] = the sum of dy[r] x[r]^T over
+ * the rows of g, zeros for a group without rows */
+int unit_grouped_dense_grad_data(const void *dy, const void *w, const void *sizes, int32_t size_bytes, void *dx, int32_t dtype,
+                                 int32_t out_dtype, int32_t rows, int32_t groups, int32_t N, int32_t K, unit_stream_t stream);
+int unit_grouped_dense_grad_weight(const void *x, const void *dy, const void *sizes, int32_t size_bytes, void *dw, int32_t dtype,
+                                   int32_t out_dtype, int32_t rows, int32_t groups, int32_t N, int32_t K, unit_stream_t stream);
+/* the forward product on MXFP4 operands, x and workspace as in unit_dense_mxfp4; wcodes, wscales of groups * N rows */
+int unit_grouped_dense_mxfp4(const void *x, const void *xscales, int32_t x_dtype, const void *wcodes, const void *wscales,
+                             const void *sizes, int32_t size_bytes, void *out, int32_t out_dtype, int32_t rows, int32_t groups,
+                             int32_t N, int32_t K, void *ws, size_t ws_bytes, unit_stream_t stream);
+
 /* ------------------------------------------------------------------ diagnostics */
 
 /* One v_mfma_i32_32x32x32_i8 / v_mfma_f32_32x32x16_f16 on a single wavefront, operands and

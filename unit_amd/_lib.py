@@ -51,6 +51,16 @@ SYMBOLS = (
     "unit_conv_chain_u8_ws_bytes",
     "unit_conv_chain_u8_ws",
     "unit_conv_chain_u8_status",
+    "unit_mxfp4_bytes",
+    "unit_quantize_mxfp4",
+    "unit_dequantize_mxfp4",
+    "unit_prepare_mxfp4",
+    "unit_mxfp4_workspace_bytes",
+    "unit_dense_mxfp4",
+    "unit_grouped_dense",
+    "unit_grouped_dense_grad_data",
+    "unit_grouped_dense_grad_weight",
+    "unit_grouped_dense_mxfp4",
     "unit_mfma_tile_i8",
     "unit_mfma_tile_f16",
     "unit_mfma_peak",
@@ -132,6 +142,16 @@ def load():
     L.unit_conv_chain_u8_ws_bytes.argtypes = [ctypes.POINTER(ChainLayerDesc), i32, ctypes.POINTER(ctypes.c_size_t)]
     L.unit_conv_chain_u8_ws.argtypes = [ctypes.POINTER(ChainLayerDesc), i32, vp, vp, ctypes.c_size_t, vp]
     L.unit_conv_chain_u8_status.argtypes = [ctypes.POINTER(ChainLayerDesc), i32, vp, vp, ctypes.c_size_t, vp, vp]
+    i64, size, sizep = ctypes.c_int64, ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)
+    L.unit_mxfp4_bytes.argtypes = [i64, i32, sizep, sizep]
+    L.unit_quantize_mxfp4.argtypes = [vp, i32, i64, i32, vp, vp, vp]
+    L.unit_dequantize_mxfp4.argtypes = [vp, vp, i64, i32, vp, i32, vp]
+    L.unit_prepare_mxfp4.argtypes = [vp, vp, i64, i32, vp, vp, vp]
+    L.unit_mxfp4_workspace_bytes.argtypes = [i32, i32, sizep]
+    L.unit_dense_mxfp4.argtypes = [vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, vp, size, vp]
+    for name in ("unit_grouped_dense", "unit_grouped_dense_grad_data", "unit_grouped_dense_grad_weight"):
+        getattr(L, name).argtypes = [vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp]
+    L.unit_grouped_dense_mxfp4.argtypes = [vp, vp, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, vp, size, vp]
     L.unit_mfma_tile_i8.argtypes = [vp, vp, vp, vp]
     L.unit_mfma_tile_f16.argtypes = [vp, vp, vp, vp]
     L.unit_mfma_peak.argtypes = [i32, i32, i32, vp, vp]
