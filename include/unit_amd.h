@@ -338,7 +338,8 @@ int unit_conv_chain_u8_status(const unit_chain_layer *layers, int32_t count, con
  *
  * In the buffers of these calls (unit_mxfp4_bytes says their sizes; 16-byte aligned) a row's codes fill kb * 128 bytes,
  * kb = K / 256 rounded up, the even element of a pair in the low half of its byte, zeros behind K; the scale of block b of a row
- * lies at [b / 8][b % 2][row][(b % 8) / 2] of [kb][2][rows][4]: a lane's four scales of a 128-byte stage are one dword. */
+ * lies at [b / 8][b % 2][row][(b % 8) / 2] of [kb][2][rows][4]: a lane's four scales of a 128-byte stage are one dword.
+ * 1 KiB more follows, which the products read (and use nothing of) at the end of the last tile. */
 enum { UNIT_F32 = 0, UNIT_F16 = 1, UNIT_BF16 = 2, UNIT_MXFP4 = 3 };
 
 int unit_mxfp4_bytes(int64_t rows, int32_t K, size_t *codes, size_t *scales);

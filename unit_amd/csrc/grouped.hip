@@ -4,137 +4,13 @@
 namespace unit {
 namespace {
 
-enum { FORWARD, GRAD_DATA, GRAD_WEIGHT };
-
-struct OpHalf : OpF16 {
-  using elem = _Float16;
-};
-struct OpMx {
-  using elem = void;
-};
-
-// The plain kernel: one wave per 32 x 32 block of the result, operands straight from memory into the fragments (lane l:
-// row or column l % 32, eight consecutive reduction elements at 8 * (l / 32)).
-template <class Op, int DIR, class Out>
-__global__ __launch_bounds__(64) void grouped_plain(GroupedParams p) {
-  constexpr bool MX = std::is_same_v<Op, OpMx>;
-  const int lane = threadIdx.x, l32 = lane & 31, half = lane >> 5;
-  int g = 0, first = 0, count = 0, x0 = 0;
-  if constexpr (DIR == GRAD_WEIGHT) {
-    g = blockIdx.z;
-    for (int i = 0; i <= g; ++i) {
-      first += count;
-      const int s = group_size(p, i);
-      count = s < p.rows - first ? s : p.rows - first;
-    }
-    x0 = blockIdx.x * 32;
-  } else {
-    int tile = blockIdx.x;
-    for (;; ++g) {
-      first += count;
-      const int s = g < p.groups ? group_size(p, g) : p.rows;
-      count = s < p.rows - first ? s : p.rows - first;
-      const int tiles = (count + 31) / 32;
-      if (tile < tiles) break;
-      tile -= tiles;
-      if (g == p.groups) return;
-    }
-    x0 = tile * 32;
-  }
-  const int y0 = blockIdx.y * 32;
-  v16f acc;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) acc[r] = 0;
-  // extents of the result block: rows (columns) of this tile's group
-  const int xs = DIR == GRAD_WEIGHT ? p.n : count, ys = DIR == FORWARD ? p.n : p.k;
-  const int xr = x0 + l32 < xs ? x0 + l32 : xs - 1, yr = y0 + l32 < ys ? y0 + l32 : ys - 1;  // in bounds; surplus ones are not stored
-  if (DIR == GRAD_WEIGHT || g < p.groups) {
-    if constexpr (MX) {
-      const int stages = mx_stages(p.k);
-      const size_t ld = (size_t)stages * 128;
-      const size_t row = (size_t)first + xr, col = (size_t)g * p.n + yr;
-      for (int s = 0; s < stages; ++s) {
-        const u32 sx = p.xs[(size_t)(2 * s + half) * p.rows + row], sy = p.ys[(size_t)(2 * s + half) * p.groups * p.n + col];
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const v4i x = *reinterpret_cast<const v4i *>(p.x + row * ld + s * 128 + (2 * kk + half) * 16);
-          const v4i y = *reinterpret_cast<const v4i *>(p.y + col * ld + s * 128 + (2 * kk + half) * 16);
-          const v8i x8 = {x[0], x[1], x[2], x[3]}, y8 = {y[0], y[1], y[2], y[3]};
-          acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, y8, acc, 4, 4, 0, (int)(sx >> 8 * kk), 0, (int)(sy >> 8 * kk));
-        }
-      }
-    } else {
-      using E = typename Op::elem;
-      typedef E v8e __attribute__((ext_vector_type(8)));
-      const E *X = reinterpret_cast<const E *>(p.x), *Y = reinterpret_cast<const E *>(p.y);
-      const size_t wrow = (size_t)g * p.n;
-      const int K = DIR == FORWARD ? p.k : DIR == GRAD_DATA ? p.n : count;
-      for (int k0 = 8 * half; k0 - 8 * half < K; k0 += 16) {
-        v8e x, y;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int k = k0 + i;
-          x[i] = y[i] = (E)0.0f;
-          if (k < K) {
-            if constexpr (DIR == FORWARD) {
-              x[i] = X[((size_t)first + xr) * p.k + k];
-              y[i] = Y[(wrow + yr) * p.k + k];
-            } else if constexpr (DIR == GRAD_DATA) {
-              x[i] = X[((size_t)first + xr) * p.n + k];
-              y[i] = Y[(wrow + k) * p.k + yr];
-            } else {
-              x[i] = X[((size_t)first + k) * p.n + xr];
-              y[i] = Y[((size_t)first + k) * p.k + yr];
-            }
-          }
-        }
-        acc = Op::mma(__builtin_bit_cast(v4i, x), __builtin_bit_cast(v4i, y), acc);
-      }
-    }
-  }
-  Out *out = reinterpret_cast<Out *>(p.out);
-  if (y0 + l32 < ys) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int x = x0 + 8 * (r >> 2) + 4 * half + (r & 3);
-      if (x < xs) out[((DIR == GRAD_WEIGHT ? (size_t)g * p.n : (size_t)first) + x) * ys + y0 + l32] = (Out)acc[r];  // the one rounding
-    }
-  }
-}
-
-template <class Op, int DIR, class Out>
-int run_grouped(const char *what, const GroupedParams &p, hipStream_t s) {
-  const int ys = DIR == FORWARD ? p.n : p.k;
-  dim3 grid;
-  if constexpr (DIR == GRAD_WEIGHT) {
-    grid = dim3(ceil_div(p.n, 32), ceil_div(ys, 32), p.groups);
-  } else {
-    // at most: every group (and the rows of none) ends inside a tile
-    const long parts = p.sizes ? (p.groups + 1 < p.rows ? p.groups + 1 : p.rows) : 1;
-    grid = dim3((unsigned)((p.rows + parts * 31) / 32), ceil_div(ys, 32));
-  }
-  hipLaunchKernelGGL((grouped_plain<Op, DIR, Out>), grid, dim3(64), 0, s, p);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: launch: %s", what, hipGetErrorString(e));
-  return UNIT_OK;
-}
-
-template <class Op, int DIR>
-int run_out(const char *what, const GroupedParams &p, int out_dtype, hipStream_t s) {
-  if (out_dtype == UNIT_F32) return run_grouped<Op, DIR, float>(what, p, s);
-  if (out_dtype == UNIT_F16) return run_grouped<Op, DIR, _Float16>(what, p, s);
-  return run_grouped<Op, DIR, __bf16>(what, p, s);
-}
-
-template <int DIR>
-int run_typed(const char *what, const GroupedParams &p, int dtype, int out_dtype, hipStream_t s) {
-  return dtype == UNIT_F16 ? run_out<OpHalf, DIR>(what, p, out_dtype, s) : run_out<OpBF16, DIR>(what, p, out_dtype, s);
+int run_typed(const char *what, int dir, const GroupedParams &p, int dtype, int out_dtype, hipStream_t s) {
+  return (dtype == UNIT_F16 ? run_grouped_f16 : run_grouped_bf16)(what, dir, p, out_dtype, s);
 }
 
 int check_types(const char *what, int dtype, int out_dtype) {
   if (dtype != UNIT_F16 && dtype != UNIT_BF16) return fail(UNIT_E_ARG, "%s: dtype must be UNIT_F16 or UNIT_BF16, got %d", what, dtype);
-  if (out_dtype != UNIT_F32 && out_dtype != UNIT_F16 && out_dtype != UNIT_BF16)
-    return fail(UNIT_E_ARG, "%s: out_dtype must be UNIT_F32, UNIT_F16 or UNIT_BF16, got %d", what, out_dtype);
+  if (out_dtype != UNIT_F32 && out_dtype != dtype) return fail(UNIT_E_ARG, "%s: out_dtype must be UNIT_F32 or the operands' type, got %d", what, out_dtype);
   return UNIT_OK;
 }
 
@@ -176,7 +52,7 @@ extern "C" int unit_grouped_dense(const void *x, const void *w, const void *size
   if (int rc = check_device()) return rc;
   if (!rows) return UNIT_OK;
   GroupedParams p{static_cast<const char *>(x), static_cast<const char *>(w), nullptr, nullptr, static_cast<char *>(out), sizes, size_bytes, groups, rows, N, K};
-  return run_typed<FORWARD>(what, p, dtype, out_dtype, static_cast<hipStream_t>(stream));
+  return run_typed(what, FORWARD, p, dtype, out_dtype, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int unit_grouped_dense_grad_data(const void *dy, const void *w, const void *sizes, int32_t size_bytes, void *dx, int32_t dtype, int32_t out_dtype,
@@ -189,7 +65,7 @@ extern "C" int unit_grouped_dense_grad_data(const void *dy, const void *w, const
   if (int rc = check_device()) return rc;
   if (!rows) return UNIT_OK;
   GroupedParams p{static_cast<const char *>(dy), static_cast<const char *>(w), nullptr, nullptr, static_cast<char *>(dx), sizes, size_bytes, groups, rows, N, K};
-  return run_typed<GRAD_DATA>(what, p, dtype, out_dtype, static_cast<hipStream_t>(stream));
+  return run_typed(what, GRAD_DATA, p, dtype, out_dtype, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int unit_grouped_dense_grad_weight(const void *x, const void *dy, const void *sizes, int32_t size_bytes, void *dw, int32_t dtype, int32_t out_dtype,
@@ -202,7 +78,7 @@ extern "C" int unit_grouped_dense_grad_weight(const void *x, const void *dy, con
   if (int rc = check_ptrs(what, true, {dw})) return rc;
   if (int rc = check_device()) return rc;
   GroupedParams p{static_cast<const char *>(dy), static_cast<const char *>(x), nullptr, nullptr, static_cast<char *>(dw), sizes, size_bytes, groups, rows, N, K};
-  return run_typed<GRAD_WEIGHT>(what, p, dtype, out_dtype, static_cast<hipStream_t>(stream));
+  return run_typed(what, GRAD_WEIGHT, p, dtype, out_dtype, static_cast<hipStream_t>(stream));
 }
 
 namespace {
@@ -234,7 +110,7 @@ int run_mxfp4(const char *what, const void *x, const void *xscales, int x_dtype,
   }
   GroupedParams p{static_cast<const char *>(x), static_cast<const char *>(wcodes), static_cast<const u32 *>(xscales), static_cast<const u32 *>(wscales),
                   static_cast<char *>(out), sizes, size_bytes, groups, rows, N, K};
-  return run_out<OpMx, FORWARD>(what, p, out_dtype, s);
+  return run_grouped_mx(what, p, out_dtype, s);
 }
 
 }  // namespace

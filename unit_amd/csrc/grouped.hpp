@@ -14,14 +14,6 @@ namespace unit {
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 
-struct OpBF16 {
-  using acc_t = v16f;
-  using elem = __bf16;
-  static __device__ __forceinline__ acc_t mma(v4i x, v4i y, acc_t c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0, 0);
-  }
-};
-
 struct GroupedParams {
   const char *x, *y;       // first operand (rows), second operand (weights; x for the weight gradient)
   const u32 *xs, *ys;      // MXFP4: scales of the two
@@ -32,16 +24,17 @@ struct GroupedParams {
   int n, k;                // weight (groups, n, k)
 };
 
-// rows of group g as the sizes give them, clamped to what is left; g == groups: what no group has
-struct RowRange {
-  int group, first, count;
-};
-
 __device__ __forceinline__ int group_size(const GroupedParams &p, int g) {
   if (!p.sizes) return p.rows;
   long s = p.size_bytes == 8 ? static_cast<const long *>(p.sizes)[g] : (long)static_cast<const int *>(p.sizes)[g];
   s = s < 0 ? 0 : s;
   return (int)(s < p.rows ? s : p.rows);
 }
+
+// the products by operand type (dir: FORWARD, GRAD_DATA, GRAD_WEIGHT); out_dtype UNIT_F32 or the operands' type, MXFP4: any
+enum { FORWARD, GRAD_DATA, GRAD_WEIGHT };
+int run_grouped_f16(const char *what, int dir, const GroupedParams &p, int out_dtype, hipStream_t s);
+int run_grouped_bf16(const char *what, int dir, const GroupedParams &p, int out_dtype, hipStream_t s);
+int run_grouped_mx(const char *what, const GroupedParams &p, int out_dtype, hipStream_t s);
 
 }  // namespace unit

@@ -1,0 +1,475 @@
+// Tiled kernel of the grouped products: tiles of both operands go global -> LDS by direct loads into a ring of NSTAGE stages, every
+// MFMA is followed by one slice of the step's other work, as in mma_dma_kernel (mma_dma.hpp); here a workgroup first finds the
+// group its tile belongs to, operands may both be reduction-major, and all loads are bounded by buffer descriptors.
+//
+// Operand forms.  "rows": reduction-contiguous rows, in LDS as rows of BKB bytes with their 16-byte chunks XORed (swz), fragments
+// read 16 bytes a lane.  "cols": reduction-major, (reduction, width) with the width contiguous; the tile lies in LDS as in memory,
+// [reduction][width], and fragments come out of it with the LDS transposing read, two per fragment.
+//   forward        X = x rows,  Y = w rows       out[row][n]
+//   data gradient  X = dy rows, Y = w cols       dx[row][k]
+//   weight gradient X = dy cols, Y = x cols      dw[n][k], the reduction runs over a group's rows
+// X is the first MFMA operand: the result's rows lie along the accumulator registers, its columns along the lanes.
+//
+// Bounds.  A stage's descriptor begins at the stage's first byte and ends where the operand's valid rows end, so rows past a group's
+// last (weight gradient) read as zeros, and rows past a tile's last valid one read as zeros or stay in the tensor.  A reduction that ends
+// inside a stage of rows: lanes whose chunk lies past its end are sent out of the descriptor, on both sides, so that what
+// lies behind (NaN, say) meets nothing.
+#pragma once
+#include "grouped.hpp"
+#include "mma_dma.hpp"
+
+namespace unit {
+
+struct OpHalf {
+  using acc_t = v16f;
+  static constexpr bool kMx = false;
+  static __device__ __forceinline__ acc_t mma(v4i x, v4i y, acc_t c) { return OpF16::mma(x, y, c); }
+};
+struct OpBF16 {
+  using acc_t = v16f;
+  static constexpr bool kMx = false;
+  static __device__ __forceinline__ acc_t mma(v4i x, v4i y, acc_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0, 0);
+  }
+};
+// 64 elements of 4 bits are 32 bytes like 16 of 16 bits: the tiling in bytes is the same.  S: which byte of the scale dwords
+struct OpMx {
+  using acc_t = v16f;
+  static constexpr bool kMx = true;
+  template <int S>
+  static __device__ __forceinline__ acc_t mma(v4i x, v4i y, acc_t c, int sx, int sy) {
+    const v8i x8 = {x[0], x[1], x[2], x[3]}, y8 = {y[0], y[1], y[2], y[3]};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x8, y8, c, 4, 4, S, sx, S, sy);
+  }
+};
+
+// ------------------------------------------------------------------------------------------- rows -> groups -> tiles
+__device__ __forceinline__ u32 scalar(u32 v) { return (u32)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ u32 lane_value(u32 v, int l) { return (u32)__builtin_amdgcn_readlane((int)v, l); }
+
+// inclusive sums over the 64 lanes, no larger than `top` (v <= top <= 2^30, so no addition wraps)
+__device__ __forceinline__ u32 scan_upto(u32 v, u32 top) {
+  auto add = [&](u32 o) { v = min(v + o, top); };
+  add((u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8: inside 16 lanes
+  add((u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+  add((u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+  add((u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+  add((u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));  // row_bcast 15: lane 15 to rows 1, 47 to 3
+  add((u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));  // row_bcast 31
+  return v;
+}
+
+struct GroupTileOf {
+  int group;         // p.groups: rows of no group
+  int first, count;  // the group's rows
+  int mt, nt;        // tile of the group's rows, tile of the columns
+  bool any;          // the workgroup has a tile
+};
+
+// The tile of workgroup `bid`.  Every wave does this by itself, lanes over groups: sums of sizes give the rows, sums of tile counts the
+// tiles; the number of tiles is known here only, so the host launches what any sizes can need and the rest ends at once.
+// Workgroups are dealt round-robin to the eight XCDs: those of one XCD take consecutive tiles, which walk a group in panels of PH
+// row tiles, column tile after column tile, so that the XCD's L2 holds the panel's rows and sees each weight tile once a panel.
+template <int BM, int PH>
+__device__ __forceinline__ GroupTileOf find_tile(const GroupedParams &p, int nts, int bid, int lane) {
+  GroupTileOf t;
+  u32 rows0 = 0, tiles0 = 0;  // of the chunks of 64 groups before
+  u32 start = 0, end = 0, tend = 0;
+  auto chunk = [&](int c) __attribute__((always_inline)) {
+    const int g = c * 64 + lane;
+    const u32 size = g < p.groups ? (u32)group_size(p, g) : 0;
+    end = min(rows0 + scan_upto(size, (u32)p.rows), (u32)p.rows);
+    start = (u32)__shfl_up((int)end, 1);
+    start = lane ? start : rows0;
+    tend = tiles0 + scan_upto((end - start + BM - 1) / BM, 1u << 30);
+  };
+  const int chunks = (p.groups + 63) / 64;
+  for (int c = 0; c < chunks; ++c) {
+    if (c) rows0 = lane_value(end, 63), tiles0 = lane_value(tend, 63);
+    chunk(c);
+  }
+  const u32 rows_in = lane_value(end, 63), tiles_in = lane_value(tend, 63);
+  const u32 total = (tiles_in + ((u32)p.rows - rows_in + BM - 1) / BM) * (u32)nts;
+  const u32 per = total / 8, rem = total % 8, xcd = (u32)bid % 8, idx = (u32)bid / 8;
+  const u32 logical = xcd * per + min(xcd, rem) + idx;
+  t.any = idx < per + (xcd < rem ? 1u : 0u);
+  if (!t.any) return t;
+  const u32 m = scalar(logical / (u32)nts);  // in whole row tiles of all groups: a group is nts * (its row tiles)
+  u32 before;
+  if (m >= tiles_in) {
+    t.group = p.groups;
+    t.first = (int)rows_in;
+    t.count = p.rows - (int)rows_in;
+    before = tiles_in;
+  } else {
+    if (chunks > 1) {
+      rows0 = tiles0 = 0;
+      for (int c = 0;; ++c) {
+        chunk(c);
+        if (lane_value(tend, 63) > m) {
+          t.group = c * 64;
+          break;
+        }
+        rows0 = lane_value(end, 63), tiles0 = lane_value(tend, 63);
+      }
+    } else {
+      t.group = 0;
+    }
+    const int l = __builtin_ctzll(__ballot(tend > m));  // ends never decrease: the first group that ends behind m
+    t.group += l;
+    t.first = (int)lane_value(start, l);
+    t.count = (int)lane_value(end, l) - t.first;
+    before = l ? lane_value(tend, l - 1) : tiles0;
+  }
+  const u32 mts = ((u32)t.count + BM - 1) / BM, within = scalar(logical) - before * (u32)nts;
+  const u32 panel = within / ((u32)nts * PH), in_panel = within - panel * ((u32)nts * PH);
+  const u32 high = min(mts - panel * PH, (u32)PH);
+  t.nt = (int)scalar(in_panel / high);
+  t.mt = (int)scalar(panel * PH + in_panel - (u32)t.nt * high);
+  t.group = (int)scalar((u32)t.group);
+  return t;
+}
+
+// rows of group g alone
+__device__ __forceinline__ void find_rows(const GroupedParams &p, int g, int lane, int &first, int &count) {
+  u32 rows0 = 0, end = 0, start = 0;
+  for (int c = 0; c <= g / 64; ++c) {
+    if (c) rows0 = lane_value(end, 63);
+    const int i = c * 64 + lane;
+    end = min(rows0 + scan_upto(i < p.groups ? (u32)group_size(p, i) : 0, (u32)p.rows), (u32)p.rows);
+    start = (u32)__shfl_up((int)end, 1);
+    start = lane ? start : rows0;
+  }
+  first = (int)lane_value(start, g % 64);
+  count = (int)lane_value(end, g % 64) - first;
+}
+
+// ------------------------------------------------------------------------------------------- the kernel
+__device__ __forceinline__ v4i bounded(const char *base, u32 bytes) {
+  const unsigned long long b = (unsigned long long)base;
+  v4i r;
+  r[0] = (int)scalar((u32)b);
+  r[1] = (int)scalar((u32)(b >> 32) & 0xffffu);
+  r[2] = (int)scalar(bytes);
+  r[3] = 0x00020000;
+  return r;
+}
+constexpr u32 kOutside = 0xfffffff0u;  // past every descriptor
+
+template <class Op, int DIR, class T, int NSTAGE, class Out>
+__global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nts, int xts) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr bool MX = Op::kMx, XT = DIR == GRAD_WEIGHT, YT = DIR != FORWARD;
+  constexpr int ES = MX ? 0 : 2;                     // bytes per element of the 16-bit forms
+  constexpr int KK = T::BKB / 32, CPR = T::CPR, NW = T::NT / 64, RPL = 64 / CPR;
+  constexpr int KS = T::BKB / 2;                     // cols: reduction elements of a stage
+  constexpr int XL = T::XBYTES / 1024 / NW, YL = T::YBYTES / 1024 / NW;
+  constexpr int SCALES = MX ? (T::BX + T::BY) * 8 : 0, PIECES = MX ? (SCALES + 1023) / 1024 : 0, PIECE = PIECES ? PIECES : 1;
+  constexpr int LPS = XL + YL + (MX ? 1 : 0);        // direct loads per wave and stage
+  constexpr int STAGE = T::STAGE + PIECES * 1024;
+  static_assert(XL * 1024 * NW == T::XBYTES && YL * 1024 * NW == T::YBYTES && KK % 2 == 0, "loads split evenly over the waves");
+  static_assert(!MX || (T::BKB == 128 && PIECES <= NW && DIR == FORWARD), "a stage of MXFP4 is one dword of scales per row and half");
+  constexpr int NM = T::TX * T::TY, NF = T::TX + T::TY;
+
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wx = wave % T::WX, wy = wave / T::WX, l32 = lane & 31, half = lane >> 5;
+  const u32 ring = (u32)(uintptr_t)(lptr_t)lds;
+
+  int group, first, count, x0, y0;
+  if constexpr (DIR == GRAD_WEIGHT) {
+    const int b = (int)blockIdx.x, per = (int)gridDim.x / 8, rem = (int)gridDim.x % 8, xcd = b % 8;
+    const int logical = xcd * per + min(xcd, rem) + b / 8;
+    group = logical / (nts * xts);
+    const int in = logical - group * (nts * xts);
+    y0 = in / xts * T::BY;
+    x0 = in % xts * T::BX;
+    find_rows(p, group, lane, first, count);
+  } else {
+    const GroupTileOf g = find_tile<T::BX, 4>(p, nts, (int)blockIdx.x, lane);
+    if (!g.any) return;
+    group = g.group, first = g.first, count = g.count;
+    x0 = g.mt * T::BX;
+    y0 = g.nt * T::BY;
+  }
+  const int xs = DIR == GRAD_WEIGHT ? p.n : count, ys = DIR == FORWARD ? p.n : p.k;  // extents of this group's result
+  const bool live = group < p.groups;
+
+  // operand bases (of this tile's first row or column), bytes per row, and how many bytes lie behind the base
+  const int K = DIR == FORWARD ? p.k : DIR == GRAD_DATA ? p.n : count;  // reduction elements
+  const long xld = MX ? (long)mx_stages(p.k) * 128 : DIR == FORWARD ? 2l * p.k : 2l * p.n;
+  const long yld = MX ? xld : 2l * p.k;
+  const int kbytes = MX ? (int)xld : K * 2;
+  const int nk = !live ? 0 : XT ? (count + KS - 1) / KS : YT ? (K + KS - 1) / KS : (kbytes + T::BKB - 1) / T::BKB;
+  const char *xb, *yb;
+  long xleft, yleft;
+  if constexpr (XT) {
+    xb = p.x + (long)first * xld + 2l * x0, xleft = (long)count * xld - 2l * x0;
+    yb = p.y + (long)first * yld + 2l * y0, yleft = (long)count * yld - 2l * y0;
+  } else {
+    xb = p.x + (long)(first + x0) * xld, xleft = (long)min(xs - x0, T::BX) * xld;
+    if constexpr (YT)
+      yb = p.y + (long)group * p.n * yld + 2l * y0, yleft = (long)p.n * yld - 2l * y0;
+    else
+      yb = p.y + ((long)group * p.n + y0) * yld, yleft = (long)min(ys - y0, T::BY) * yld;
+  }
+  const long xstep = XT ? (long)KS * xld : T::BKB, ystep = YT ? (long)KS * yld : T::BKB;  // bytes from stage to stage
+
+  // this lane's chunk of each load; rows: the byte of the stage's row it holds, to compare with the reduction's end
+  u32 xoff[XL], yoff[YL];
+  auto offsets = [&](u32(&off)[XL > YL ? XL : YL], int n, bool cols, int width, long ld) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      if (cols) {
+        const int cpr = width / 8, row = (wave * n + i) * (64 / cpr) + lane / cpr;
+        off[i] = (u32)row * (u32)ld + (u32)(((lane % cpr) ^ (4 * (row & 3))) << 4);
+      } else {
+        const int row = (wave * n + i) * RPL + lane / CPR;
+        off[i] = (u32)row * (u32)ld + (u32)(((lane % CPR) ^ swz<T::BKB>(row)) << 4);
+      }
+    }
+  };
+  {
+    u32 tmp[XL > YL ? XL : YL];
+    offsets(tmp, XL, XT, T::BX, xld);
+#pragma unroll
+    for (int i = 0; i < XL; ++i) xoff[i] = tmp[i];
+    offsets(tmp, YL, YT, T::BY, yld);
+#pragma unroll
+    for (int i = 0; i < YL; ++i) yoff[i] = tmp[i];
+  }
+  // MXFP4: the scales of a stage, X rows then Y rows, each [half][row] dwords, 64 pieces of four rows per load
+  const char *sptr = nullptr;
+  long sstep = 0;
+  if constexpr (MX) {
+    const int c = min((wave % PIECE) * 64 + lane, (T::BX + T::BY) / 2 - 1), cy = c - T::BX / 2;
+    const long xrows = p.rows, yrows = (long)p.groups * p.n;
+    if (c < T::BX / 2)
+      sptr = reinterpret_cast<const char *>(p.xs + c / (T::BX / 4) * xrows + first + x0 + c % (T::BX / 4) * 4), sstep = xrows * 8;
+    else
+      sptr = reinterpret_cast<const char *>(p.ys + cy / (T::BY / 4) * yrows + (long)group * p.n + y0 + cy % (T::BY / 4) * 4), sstep = yrows * 8;
+  }
+
+  struct Source {
+    v4i x, y;
+  };
+  // descriptors of stage kt
+  auto source = [&](int kt) __attribute__((always_inline)) {
+    const long xa = kt * xstep, ya = kt * ystep;
+    auto clip = [](long v) { return (u32)min(v, 0xffffff00l); };
+    return Source{bounded(xb + xa, clip(xleft - xa)), bounded(yb + ya, clip(yleft - ya))};
+  };
+  // load i of stage kt into ring buffer `slot`; last: the reduction may end inside the stage
+  auto issue_one = [&](const Source &src, int kt, int slot, int i, auto last) __attribute__((always_inline)) {
+    const u32 buf = ring + (u32)(slot * STAGE);
+    auto inside = [&](u32 off, int j, bool cols, int n) {
+      if (!decltype(last)::value || cols || MX) return off;
+      const int row = (wave * n + j) * RPL + lane / CPR;
+      const int at = kt * T::BKB + (((lane % CPR) ^ swz<T::BKB>(row)) << 4);
+      return at < kbytes ? off : kOutside;
+    };
+    if (i < XL)
+      dma_buffer_16(buf + (wave * XL + i) * 1024, inside(xoff[i], i, XT, XL), src.x, 0);
+    else if (i < XL + YL)
+      dma_buffer_16(buf + T::XBYTES + (wave * YL + (i - XL)) * 1024, inside(yoff[i - XL], i - XL, YT, YL), src.y, 0);
+    else
+      direct_load_16(sptr + kt * sstep, buf + T::STAGE + (wave % PIECE) * 1024);
+  };
+
+  typename Op::acc_t acc[T::TX][T::TY];
+#pragma unroll
+  for (int i = 0; i < T::TX; ++i)
+#pragma unroll
+    for (int j = 0; j < T::TY; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+
+  // fragment addresses inside a stage, k-step 0
+  const int xrow = wx * (T::TX * 32) + l32, yrow = wy * (T::TY * 32) + l32;
+  const int xsw = swz<T::BKB>(xrow), ysw = swz<T::BKB>(yrow);
+  int xtr[T::TX], ytr[T::TY];
+  {
+    const int jrow = (lane & 15) >> 2, q = lane & 3, g16 = (lane >> 4) & 1;
+    auto at = [&](int c, int width) { return (8 * half + jrow) * (width * 2) + (((c + 2 * g16 + (q >> 1)) ^ (4 * jrow)) << 4) + (q & 1) * 8; };
+    if constexpr (XT) {
+#pragma unroll
+      for (int i = 0; i < T::TX; ++i) xtr[i] = at(wx * (T::TX * 4) + i * 4, T::BX);
+    }
+    if constexpr (YT) {
+#pragma unroll
+      for (int j = 0; j < T::TY; ++j) ytr[j] = T::XBYTES + at(wy * (T::TY * 4) + j * 4, T::BY);
+    }
+  }
+  auto transposed = [&](const char *src, int pitch) __attribute__((always_inline)) {
+    typedef __attribute__((address_space(3))) v4s *trptr_t;
+    typedef short v8s __attribute__((ext_vector_type(8)));
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((trptr_t)(src));
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((trptr_t)(src + 4 * pitch));
+    return __builtin_bit_cast(v4i, (v8s)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  v4i xf[2][T::TX], yf[2][T::TY];
+  int sx[2][T::TX], sy[2][T::TY];  // MXFP4: scale dwords of this stage and of the next
+  // fragment idx of a step's list: X0, Y0 .. Y(TY-1), X1 .. X(TX-1)
+  auto load_one = [&](const char *stage, int kk, int s, int idx) __attribute__((always_inline)) {
+    if (idx >= 1 && idx <= T::TY) {
+      const int j = idx - 1;
+      if constexpr (YT)
+        yf[s][j] = transposed(stage + ytr[j] + kk * 16 * (T::BY * 2), T::BY * 2);
+      else
+        yf[s][j] = *reinterpret_cast<const v4i *>(stage + T::XBYTES + (yrow + j * 32) * T::BKB + (((2 * kk + half) ^ ysw) << 4));
+      if (MX && kk == 0) sy[1][j] = *reinterpret_cast<const int *>(stage + T::STAGE + T::BX * 8 + half * (T::BY * 4) + (yrow + j * 32) * 4);
+    } else {
+      const int i = idx == 0 ? 0 : idx - T::TY;
+      if constexpr (XT)
+        xf[s][i] = transposed(stage + xtr[i] + kk * 16 * (T::BX * 2), T::BX * 2);
+      else
+        xf[s][i] = *reinterpret_cast<const v4i *>(stage + (xrow + i * 32) * T::BKB + (((2 * kk + half) ^ xsw) << 4));
+      if (MX && kk == 0) sx[1][i] = *reinterpret_cast<const int *>(stage + T::STAGE + half * (T::BX * 4) + (xrow + i * 32) * 4);
+    }
+  };
+  auto next_scales = [&]() __attribute__((always_inline)) {
+    if constexpr (MX) {
+#pragma unroll
+      for (int i = 0; i < T::TX; ++i) sx[0][i] = sx[1][i];
+#pragma unroll
+      for (int j = 0; j < T::TY; ++j) sy[0][j] = sy[1][j];
+    }
+  };
+  using yes = std::integral_constant<bool, true>;
+  using no = std::integral_constant<bool, false>;
+  // One k-step: MFMAs, each followed by its share of the next step's fragment reads and of the loads of a later stage.
+  auto step = [&](auto kkc, const char *rd_stage, int rd_kk, const Source &src, int issue_kt, int slot, auto has_read, auto has_issue, auto last)
+                  __attribute__((always_inline)) {
+    constexpr int s = decltype(kkc)::value & 1;
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      const int i = m / T::TY, j = m % T::TY;
+      if constexpr (MX)
+        acc[i][j] = Op::template mma<decltype(kkc)::value>(xf[s][i], yf[s][j], acc[i][j], sx[0][i], sy[0][j]);
+      else
+        acc[i][j] = Op::mma(xf[s][i], yf[s][j], acc[i][j]);
+      if constexpr (decltype(has_read)::value) {
+#pragma unroll
+        for (int f = m * NF / NM; f < (m + 1) * NF / NM; ++f) load_one(rd_stage, rd_kk, s ^ 1, f);
+      }
+      if constexpr (decltype(has_issue)::value) {
+#pragma unroll
+        for (int f = m * LPS / NM; f < (m + 1) * LPS / NM; ++f) issue_one(src, issue_kt, slot, f, last);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // One stage.  ISSUE: stage kt + NSTAGE exists and goes into the buffer that this stage frees; STEADY: NSTAGE - 1 younger stages are in
+  // flight at the barrier; NEXT: stage kt + 1 exists; LAST: the stage that is fetched may hold the reduction's end.
+  auto stage = [&](int kt, int slot, auto issue_next, auto steady, auto next, auto last) __attribute__((always_inline)) {
+    const char *cur = lds + slot * STAGE;
+    const char *nxt = lds + (slot + 1 == NSTAGE ? 0 : slot + 1) * STAGE;
+    const Source none{};
+    auto early = [&](auto kkc) __attribute__((always_inline)) { step(kkc, cur, decltype(kkc)::value + 1, none, 0, 0, yes{}, no{}, no{}); };
+    early(std::integral_constant<int, 0>{});
+    if constexpr (KK > 2) {
+      early(std::integral_constant<int, 1>{});
+      early(std::integral_constant<int, 2>{});
+    }
+    if constexpr (decltype(steady)::value)
+      UNIT_WAIT_VMCNT((NSTAGE - 2) * LPS);
+    else
+      UNIT_WAIT_VMCNT(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): this wave's reads of `cur` are done
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    Source src{};
+    if constexpr (decltype(issue_next)::value) src = source(kt + NSTAGE);
+    step(std::integral_constant<int, KK - 1>{}, nxt, 0, src, kt + NSTAGE, slot, next, issue_next, last);
+    if constexpr (decltype(next)::value) next_scales();
+  };
+
+  if (nk > 0) {
+#pragma unroll
+    for (int s = 0; s < NSTAGE; ++s)
+      if (s < nk) {
+        const Source src = source(s);
+#pragma unroll
+        for (int i = 0; i < LPS; ++i) issue_one(src, s, s, i, yes{});
+      }
+    if (nk >= NSTAGE)
+      UNIT_WAIT_VMCNT((NSTAGE - 1) * LPS);
+    else
+      UNIT_WAIT_VMCNT(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) load_one(lds, 0, 0, f);
+    next_scales();
+    int kt = 0;
+    for (; kt + 2 * NSTAGE < nk; kt += NSTAGE) {  // fetches up to stage kt + 2 * NSTAGE - 1: never the last one
+#pragma unroll
+      for (int s = 0; s < NSTAGE; ++s) stage(kt + s, s, yes{}, yes{}, yes{}, no{});
+    }
+    for (; kt + NSTAGE < nk; ++kt) stage(kt, kt % NSTAGE, yes{}, yes{}, yes{}, yes{});
+    for (; kt + 1 < nk; ++kt) stage(kt, kt % NSTAGE, no{}, no{}, yes{}, no{});
+    stage(kt, kt % NSTAGE, no{}, no{}, no{}, no{});
+  }
+
+  // results: rounded once, here
+  const long out_row = (DIR == GRAD_WEIGHT ? (long)group * p.n : (long)first) + x0;
+  const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(p.out + out_row * ys * (long)sizeof(Out), 0, -1, 0x00020000);
+#pragma unroll
+  for (int j = 0; j < T::TY; ++j) {
+    const int y = y0 + wy * (T::TY * 32) + j * 32 + l32;
+    if (y >= ys) continue;
+#pragma unroll
+    for (int i = 0; i < T::TX; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int x = wx * (T::TX * 32) + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+        if (x0 + x < xs) store_result<kRowPolicy>(out, ((u32)x * (u32)ys + (u32)y) * (u32)sizeof(Out), (Out)acc[i][j][r]);
+      }
+  }
+}
+
+template <class Op, int DIR, class T, int NSTAGE, class Out>
+int run_grouped_tile(const char *what, const char *tag, const GroupedParams &p, hipStream_t s) {
+  constexpr int lds = NSTAGE * (T::STAGE + (Op::kMx ? ((T::BX + T::BY) * 8 + 1023) / 1024 * 1024 : 0));
+  static_assert(lds <= kMaxLds, "ring does not fit the LDS");
+  auto kern = grouped_tile<Op, DIR, T, NSTAGE, Out>;
+  static thread_local bool allowed = false;
+  if (!allowed && lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds);
+    if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: hipFuncSetAttribute: %s", what, hipGetErrorString(e));
+    allowed = true;
+  }
+  const int ys = DIR == FORWARD ? p.n : p.k, nts = ceil_div(ys, T::BY), xts = ceil_div(p.n, T::BX);
+  long wgs;
+  if (DIR == GRAD_WEIGHT) {
+    wgs = (long)p.groups * nts * xts;
+  } else {
+    // at most: every group, and the rows of none, ends inside a tile
+    const long parts = p.sizes ? (p.groups + 1 < p.rows ? p.groups + 1 : p.rows) : 1;
+    wgs = (p.rows + parts * (T::BX - 1)) / T::BX * nts + 7;  // + 7: an XCD's share is rounded up
+  }
+  if (wgs * T::NT >= 1l << 32) return fail(UNIT_E_ARG, "%s: %ld tiles exceed one launch", what, wgs);
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(T::NT), lds, s, p, nts, xts);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: launch: %s", what, hipGetErrorString(e));
+  set_variant("%s_x%d_y%d_k%d_r%d", tag, T::BX, T::BY, T::BKB, NSTAGE);
+  return UNIT_OK;
+}
+
+// Large tiles (256 x 256) where the groups' rows fill them on average, else 128 x 128.  us, experts of 512 rows on average, 16384 x
+// 1024 -> 2048: 103 against 124; MXFP4 333 x 2088 -> 1516: 22.5 against 13.8.
+inline bool grouped_large(const GroupedParams &p, int dir) {
+  const int pinned = tuning_override("UNIT_AMD_GROUPED_TILE");
+  if (pinned) return pinned == 2;
+  const int xs = dir == GRAD_WEIGHT ? p.n : p.rows / p.groups, ys = dir == FORWARD ? p.n : p.k;
+  const long tiles = (long)ceil_div(xs, 256) * ceil_div(ys, 256) * p.groups;
+  return xs >= 192 && ys >= 192 && tiles >= 128;
+}
+
+template <class Op, int DIR, class Out>
+int run_grouped_sizes(const char *what, const char *tag, const GroupedParams &p, hipStream_t s) {
+  if (grouped_large(p, DIR)) return run_grouped_tile<Op, DIR, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
+  return run_grouped_tile<Op, DIR, Tile<128, 128, 64, 2, 2>, 4, Out>(what, tag, p, s);
+}
+
+}  // namespace unit

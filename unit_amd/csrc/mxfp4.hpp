@@ -18,7 +18,8 @@ constexpr int kMxStage = 256;  // elements per 128 bytes of codes, the padding o
 
 inline __host__ __device__ int mx_stages(int K) { return (K + kMxStage - 1) / kMxStage; }
 inline size_t mx_code_bytes(long rows, int K) { return (size_t)rows * mx_stages(K) * 128; }
-inline size_t mx_scale_bytes(long rows, int K) { return (size_t)rows * mx_stages(K) * 8; }
+// 1 KiB behind the last plane: the products fetch the scales of whole tiles of up to 256 rows
+inline size_t mx_scale_bytes(long rows, int K) { return (size_t)rows * mx_stages(K) * 8 + 1024; }
 
 // The block's scale: the exponent of its largest magnitude less 2 (the largest element, 6, is 1.5 * 2^2), biased by 127.
 // amax_bits: the bits of that magnitude as a float.  Subnormal magnitudes lie below the smallest scale times the smallest
