@@ -5,63 +5,139 @@
 namespace unit {
 namespace {
 
-template <class T>
-__device__ __forceinline__ float as_float(T v) {
-  return (float)v;
-}
+// A workgroup takes 8 * ROUNDS rows of one 256-element stage, half a wave a row: a lane eight elements, four lanes a block.
+// All of a lane's loads are issued before the first is used; the scales of a stage, one dword per row and half, are gathered in
+// LDS so that they leave in runs of consecutive rows.
+template <class T, int ROUNDS>
+struct StageRows {
+  static constexpr int kRows = 8 * ROUNDS;
+  typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));  // rows begin on any element
+  using bits = std::conditional_t<sizeof(T) == 4, u32, unsigned short>;
+  typedef bits b8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
 
-// One lane takes eight elements, four lanes a block.  Scaling by a power of two and rounding to the nearest element (ties to
-// the even mantissa, magnitudes above 6 to 6) are v_cvt_scalef32_pk_fp4_f32.
+// Scaling by a power of two and rounding to the nearest element (ties to the even mantissa, magnitudes above 6 to 6) are what
+// v_cvt_scalef32_pk_fp4 does.
 template <class T>
-__global__ __launch_bounds__(256) void quantize_kernel(const T *x, long rows, int K, u32 *codes, unsigned char *scales) {
-  const int per_row = mx_stages(K) * 32;  // lanes per row
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  const long row = id / per_row;
-  const int lane = (int)(id % per_row), k0 = lane * 8;
-  const bool live = row < rows;
-  float v[8];
-  u32 top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = live && k0 + i < K ? as_float(x[row * K + k0 + i]) : 0.0f;
-    const u32 a = __builtin_bit_cast(u32, v[i]) & 0x7fffffffu;
-    top = a > top ? a : top;
-  }
-  u32 other = __shfl_xor(top, 1);
-  top = other > top ? other : top;
-  other = __shfl_xor(top, 2);
-  top = other > top ? other : top;
-  if (!live) return;
-  const u32 s = mx_scale(top);
-  const float p = mx_power(s == 255 ? 127 : s);
+__device__ __forceinline__ u32 eight_codes(typename StageRows<T, 1>::b8 v, float p) {
   u32 c = 0;
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], p, 0);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], p, 1);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], p, 2);
-  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], p, 3);
-  codes[row * per_row + lane] = c;
-  const int b = lane / 4;
-  if (lane % 4 == 0) scales[((long)(b / 8 * 2 + b % 2) * rows + row) * 4 + b % 8 / 2] = (unsigned char)s;
+  auto two = [&](auto n) __attribute__((always_inline)) {
+    constexpr int N = decltype(n)::value;
+    if constexpr (std::is_same_v<T, float>) {
+      typedef float v8f __attribute__((ext_vector_type(8)));
+      const v8f f = __builtin_bit_cast(v8f, v);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2 * N], f[2 * N + 1], p, N);
+    } else {
+      typedef T v2 __attribute__((ext_vector_type(2)));
+      const u32 pair = __builtin_bit_cast(v4u, v)[N];
+      if constexpr (std::is_same_v<T, _Float16>)
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(v2, pair), p, N);
+      else
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(v2, pair), p, N);
+    }
+  };
+  two(std::integral_constant<int, 0>{});
+  two(std::integral_constant<int, 1>{});
+  two(std::integral_constant<int, 2>{});
+  two(std::integral_constant<int, 3>{});
+  return c;
 }
 
+// the bits of the largest magnitude of eight elements, as a float; infinities and NaN are the largest
 template <class T>
-__global__ __launch_bounds__(256) void dequantize_kernel(const u32 *codes, const unsigned char *scales, long rows, int K, T *out) {
-  const int per_row = mx_stages(K) * 32;
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  const long row = id / per_row;
-  const int lane = (int)(id % per_row), k0 = lane * 8;
-  if (row >= rows || k0 >= K) return;
-  const int b = lane / 4;
-  const u32 s = scales[((long)(b / 8 * 2 + b % 2) * rows + row) * 4 + b % 8 / 2];
-  const u32 c = codes[row * per_row + lane];
-  // 255 is NaN; 2^127 and the other powers are multiplied in single precision, once
-  const float p = s == 255 ? __builtin_nanf("") : mx_power(s);
+__device__ __forceinline__ u32 eight_top(typename StageRows<T, 1>::b8 v) {
+  u32 top = 0;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const u32 h = c >> (4 * i) & 15, m = h & 7;
-    // 0, 0.5, then 2^(m / 2 - 1) * (1 + m % 2 / 2)
-    const float a = m < 2 ? 0.5f * (float)m : __builtin_bit_cast(float, (126u + (m >> 1)) << 23 | (m & 1) << 22);
-    if (k0 + i < K) out[row * K + k0 + i] = (T)((h & 8 ? -a : a) * p);
+    for (int i = 0; i < 8; ++i) top = max(top, v[i] & 0x7fffffffu);
+    return top;
+  } else {
+    // sign-less 16-bit patterns are ordered like the values: two at a time
+    const v4u w = __builtin_bit_cast(v4u, v);
+    typedef unsigned short v2s __attribute__((ext_vector_type(2)));
+    v2s m = __builtin_bit_cast(v2s, w[0] & 0x7fff7fffu);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(v2s, w[i] & 0x7fff7fffu));
+    top = max((u32)m[0], (u32)m[1]);
+    if constexpr (std::is_same_v<T, __bf16>) return top << 16;
+    return __builtin_bit_cast(u32, (float)__builtin_bit_cast(_Float16, (unsigned short)top)) & 0x7fffffffu;  // NaN stays NaN
+  }
+}
+
+template <class T, int ROUNDS>
+__global__ __launch_bounds__(256) void quantize_kernel(const T *x, int rows, int K, u32 *codes, u32 *scales, FastDiv by_stages) {
+  using R = StageRows<T, ROUNDS>;
+  __shared__ unsigned char gather[2 * R::kRows * 4];
+  const int t = threadIdx.x, l32 = t & 31, stages = by_stages.d;
+  int s, row0;
+  by_stages.divmod((int)blockIdx.x, row0, s);
+  row0 *= R::kRows;
+  const int k0 = s * kMxStage + l32 * 8;
+  typename R::b8 v[ROUNDS];
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int row = min(row0 + i * 8 + (t >> 5), rows - 1);
+    const typename R::bits *src = reinterpret_cast<const typename R::bits *>(x) + (size_t)row * K + k0;
+    if (k0 + 8 <= K) {
+      v[i] = *reinterpret_cast<const typename R::b8 *>(src);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = k0 + j < K ? src[j] : 0;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int r = i * 8 + (t >> 5), row = row0 + r;
+    u32 top = eight_top<T>(v[i]);
+    top = max(top, (u32)__builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true));  // lanes 1, 0, 3, 2
+    top = max(top, (u32)__builtin_amdgcn_mov_dpp((int)top, 0x4e, 0xf, 0xf, true));  // lanes 2, 3, 0, 1
+    const u32 e = mx_scale(top);
+    const u32 c = eight_codes<T>(v[i], mx_power(e == 255 ? 127 : e));
+    if (row < rows) codes[(size_t)row * (stages * 32) + s * 32 + l32] = c;
+    const int b = l32 >> 2;
+    if ((l32 & 3) == 0) gather[((b & 1) * R::kRows + r) * 4 + (b >> 1)] = (unsigned char)e;
+  }
+  __syncthreads();
+  const int h = t / R::kRows, r = t % R::kRows;
+  if (h < 2 && row0 + r < rows) scales[(size_t)(2 * s + h) * rows + row0 + r] = reinterpret_cast<const u32 *>(gather)[t];
+}
+
+template <class T, int ROUNDS>
+__global__ __launch_bounds__(256) void dequantize_kernel(const u32 *codes, const u32 *scales, int rows, int K, T *out, FastDiv by_stages) {
+  using R = StageRows<T, ROUNDS>;
+  const int t = threadIdx.x, l32 = t & 31, stages = by_stages.d;
+  int s, row0;
+  by_stages.divmod((int)blockIdx.x, row0, s);
+  row0 = row0 * R::kRows + (t >> 5);
+  const int k0 = s * kMxStage + l32 * 8, b = l32 >> 2;
+  u32 c[ROUNDS], e[ROUNDS];
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int row = min(row0 + i * 8, rows - 1);
+    c[i] = codes[(size_t)row * (stages * 32) + s * 32 + l32];
+    e[i] = scales[(size_t)(2 * s + (b & 1)) * rows + row] >> (8 * (b >> 1)) & 255;
+  }
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int row = row0 + i * 8;
+    if (row >= rows || k0 >= K) continue;
+    const float p = e[i] == 255 ? __builtin_nanf("") : mx_power(e[i]);
+    typename R::v8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const u32 h = c[i] >> (4 * j) & 15, m = h & 7;
+      // 0, 0.5, then 2^(m / 2 - 1) * (1 + m % 2 / 2); one rounding, to T
+      const u32 a = m < 2 ? m * 0x3f000000u : (126u + (m >> 1)) << 23 | (m & 1) << 22;
+      v[j] = (T)(__builtin_bit_cast(float, a | (h & 8) << 28) * p);
+    }
+    T *dst = out + (size_t)row * K + k0;
+    if (k0 + 8 <= K) {
+      *reinterpret_cast<typename R::v8 *>(dst) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k0 + j < K) dst[j] = v[j];
+    }
   }
 }
 
@@ -93,6 +169,17 @@ int check_mx(const char *what, int64_t rows, int32_t K, std::initializer_list<co
 
 unsigned mx_grid(int64_t rows, int32_t K) { return (unsigned)((rows * mx_stages(K) * 32 + 255) / 256); }
 
+// run(rounds, workgroups, divider): 64 rows a workgroup while that makes two workgroups per CU, else 8
+template <class F>
+void by_stage(int64_t rows, int32_t K, F run) {
+  const int stages = mx_stages(K);
+  const int64_t tall = (rows + 63) / 64 * stages;
+  if (tall >= 512)
+    run(std::integral_constant<int, 8>{}, dim3((unsigned)tall), FastDiv::make(stages));
+  else
+    run(std::integral_constant<int, 1>{}, dim3((unsigned)((rows + 7) / 8 * stages)), FastDiv::make(stages));
+}
+
 int launched(const char *what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? UNIT_OK : fail(UNIT_E_LAUNCH, "%s: launch: %s", what, hipGetErrorString(e));
@@ -121,7 +208,11 @@ extern "C" int unit_quantize_mxfp4(const void *x, int32_t dtype, int64_t rows, i
   if (!rows) return UNIT_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto run = [&](auto *p) {
-    hipLaunchKernelGGL(quantize_kernel, dim3(mx_grid(rows, K)), dim3(256), 0, s, p, (long)rows, K, static_cast<u32 *>(codes), static_cast<unsigned char *>(scales));
+    by_stage(rows, K, [&](auto rounds, dim3 grid, FastDiv by_stages) {
+      using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+      hipLaunchKernelGGL((quantize_kernel<T, decltype(rounds)::value>), grid, dim3(256), 0, s, p, (int)rows, K, static_cast<u32 *>(codes), static_cast<u32 *>(scales),
+                         by_stages);
+    });
   };
   if (dtype == UNIT_F32) run(static_cast<const float *>(x));
   if (dtype == UNIT_F16) run(static_cast<const _Float16 *>(x));
@@ -139,7 +230,11 @@ extern "C" int unit_dequantize_mxfp4(const void *codes, const void *scales, int6
   if (!rows) return UNIT_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto run = [&](auto *p) {
-    hipLaunchKernelGGL(dequantize_kernel, dim3(mx_grid(rows, K)), dim3(256), 0, s, static_cast<const u32 *>(codes), static_cast<const unsigned char *>(scales), (long)rows, K, p);
+    by_stage(rows, K, [&](auto rounds, dim3 grid, FastDiv by_stages) {
+      using T = std::remove_pointer_t<decltype(p)>;
+      hipLaunchKernelGGL((dequantize_kernel<T, decltype(rounds)::value>), grid, dim3(256), 0, s, static_cast<const u32 *>(codes), static_cast<const u32 *>(scales),
+                         (int)rows, K, p, by_stages);
+    });
   };
   if (dtype == UNIT_F32) run(static_cast<float *>(out));
   if (dtype == UNIT_F16) run(static_cast<_Float16 *>(out));
