@@ -223,8 +223,7 @@ def test_other_streams_and_graph_replays(dev):
     """On a stream of its own, and captured: sizes are read when the work runs, so a replay follows what they hold by then."""
     x, w, dy, s = operands([70, 0, 200, 30], 4, 264, 136, "bfloat16", dev)
     wq = U.quantize_mxfp4(w)
-    run = lambda: (U.grouped_dense(x, w, s), *U.grouped_dense_grad(x, w, dy, s), U.grouped_dense_mxfp4(x, wq, s), U.dense_mxfp4(x, U.Mxfp4Tensor(
-        *(lambda q: (q.codes, q.scales))(U.quantize_mxfp4(w[1])), (264, 136))))
+    run = lambda: (U.grouped_dense(x, w, s), *U.grouped_dense_grad(x, w, dy, s), U.grouped_dense_mxfp4(x, wq, s), U.dense_mxfp4(x, U.quantize_mxfp4(w[1])))
     eager = run()
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())

@@ -174,7 +174,7 @@ def test_refusals(dev):
         U.quantize_mxfp4(torch.zeros((4, 64)))
     with pytest.raises(TypeError, match="dtype"):
         U.quantize_mxfp4(torch.zeros((4, 64), dtype=torch.float64, device=dev))
-    with pytest.raises(ValueError, match="two axes"):
+    with pytest.raises(ValueError, match="two axes or three"):
         U.quantize_mxfp4(torch.zeros((64,), device=dev))
     with pytest.raises(ValueError, match="K must be positive"):
         U.quantize_mxfp4(torch.zeros((4, 0), device=dev))

@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
+#include <new>
 
 #include "../../include/unit_amd.h"
 
@@ -40,6 +41,22 @@ struct Library {
 };
 Library lib;
 constexpr int kFunctions = sizeof(Library) / sizeof(void *);
+
+// those of the expert and MXFP4 products (bind_grouped)
+struct GroupedLibrary {
+  decltype(&unit_mxfp4_bytes) mx_bytes;
+  decltype(&unit_quantize_mxfp4) quantize;
+  decltype(&unit_dequantize_mxfp4) dequantize;
+  decltype(&unit_mxfp4_workspace_bytes) mx_workspace;
+  decltype(&unit_dense_mxfp4) dense_mx;
+  decltype(&unit_grouped_dense) grouped;
+  decltype(&unit_grouped_dense_grad_data) grad_data;
+  decltype(&unit_grouped_dense_grad_weight) grad_weight;
+  decltype(&unit_grouped_dense_mxfp4) grouped_mx;
+};
+GroupedLibrary glib;
+constexpr int kGroupedFunctions = sizeof(GroupedLibrary) / sizeof(void *);
+PyObject *mx_type, *n_shape;  // grouped.Mxfp4Tensor
 
 // ops.PreparedConvWeight, PreparedDenseWeight, PreparedGemmB; torch.int8, torch.float16
 PyObject *conv_weight_type, *dense_weight_type, *gemm_b_type, *dtype_s8, *dtype_f16;
@@ -354,20 +371,240 @@ PyObject *gemm(PyObject *const *a, Py_ssize_t n) {
   return finish(std::move(out), [&](void *s, void *xp, void *bp, void *o) { return lib.gemm(xp, bp, o, m, nn, k, half, s); }, *x, *b);
 }
 
-// (addresses in Library's order, the three prepared classes, torch.int8, torch.float16)
-PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  if (n != 6 || !PyTuple_CheckExact(a[0]) || PyTuple_GET_SIZE(a[0]) != kFunctions) {
+// ------------------------------------------------------------------------------- expert and MXFP4 products
+// a floating type's code in the library, -1 for others
+int float_code(at::ScalarType t) {
+  return t == at::kFloat ? UNIT_F32 : t == at::kHalf ? UNIT_F16 : t == at::kBFloat16 ? UNIT_BF16 : -1;
+}
+
+bool out_type(PyObject *o, at::ScalarType *t) {
+  if (!PyUnicode_CheckExact(o)) return false;
+  if (PyUnicode_CompareWithASCIIString(o, "bfloat16") == 0) return *t = at::kBFloat16, true;
+  if (PyUnicode_CompareWithASCIIString(o, "float16") == 0) return *t = at::kHalf, true;
+  if (PyUnicode_CompareWithASCIIString(o, "float32") == 0) return *t = at::kFloat, true;
+  return false;
+}
+
+// floats the library can be handed as they are, or null
+const at::Tensor *floats(PyObject *o, int *code) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor &t = THPVariable_Unpack(o);
+  *code = float_code(t.scalar_type());
+  return *code >= 0 ? operand(o, t.scalar_type(), (int)t.dim()) : nullptr;
+}
+
+// an Mxfp4Tensor: its buffer, sizes of its shape (dims of them) and its rows
+struct Mx {
+  at::Tensor buf;
+  int64_t size[3], rows;
+  int dims;
+  size_t codes;  // bytes before the scales
+  char *data() const { return static_cast<char *>(buf.data_ptr()); }
+};
+bool mx_operand(PyObject *o, Mx *q) {
+  if ((PyObject *)Py_TYPE(o) != mx_type) return false;
+  PyObject *shape = PyObject_GetAttr(o, n_shape);
+  if (!shape) return PyErr_Clear(), false;
+  bool ok = PyTuple_CheckExact(shape) && PyTuple_GET_SIZE(shape) >= 2 && PyTuple_GET_SIZE(shape) <= 3;
+  q->rows = 1;
+  q->dims = ok ? (int)PyTuple_GET_SIZE(shape) : 0;
+  for (int i = 0; ok && i < q->dims; ++i) {
+    int32_t v;
+    ok = number(PyTuple_GET_ITEM(shape, i), &v);
+    q->size[i] = v;
+    if (i + 1 < q->dims) q->rows *= v;
+  }
+  Py_DECREF(shape);
+  PyObject *buf = ok ? PyObject_GetAttr(o, n_buf) : nullptr;
+  if (!buf) return PyErr_Clear(), false;
+  const at::Tensor *t = operand(buf, at::kByte, 1);
+  size_t scales;
+  ok = t && glib.mx_bytes(q->rows, (int32_t)q->size[q->dims - 1], &q->codes, &scales) == UNIT_OK && (size_t)t->numel() >= q->codes + scales;
+  if (ok) q->buf = *t;
+  Py_DECREF(buf);
+  return ok;
+}
+
+template <class F>
+int without_gil(F &&call) {
+  WithoutGil others;
+  return call();
+}
+
+// (x)
+PyObject *quantize(PyObject *const *a, Py_ssize_t n) {
+  int code;
+  const at::Tensor *x = n == 1 ? floats(a[0], &code) : nullptr;
+  if (!x || x->dim() < 2 || x->dim() > 3 || !small(*x)) Py_RETURN_NONE;
+  const int32_t k = (int32_t)x->size(-1);
+  int64_t rows = 1;
+  for (int i = 0; i + 1 < x->dim(); ++i) rows *= x->size(i);
+  size_t codes, scales;
+  if (glib.mx_bytes(rows, k, &codes, &scales) != UNIT_OK) Py_RETURN_NONE;
+  at::Tensor buf = result(*x, {(int64_t)(codes + scales)}, at::kByte);
+  void *s = stream(), *src = x->data_ptr();
+  char *dst = static_cast<char *>(buf.data_ptr());
+  if (without_gil([&] { return glib.quantize(src, code, rows, k, dst, dst + codes, s); }) != UNIT_OK) Py_RETURN_NONE;
+  PyObject *shape = PyTuple_New(x->dim());
+  for (int i = 0; shape && i < x->dim(); ++i) PyTuple_SET_ITEM(shape, i, PyLong_FromLongLong(x->size(i)));
+  PyObject *b = THPVariable_Wrap(std::move(buf));
+  PyObject *q = shape && b ? PyObject_CallFunctionObjArgs(mx_type, b, shape, nullptr) : nullptr;
+  Py_XDECREF(shape);
+  Py_XDECREF(b);
+  if (!q) throw std::bad_alloc();
+  return q;
+}
+
+// (q, out_dtype)
+PyObject *dequantize(PyObject *const *a, Py_ssize_t n) {
+  Mx q;
+  at::ScalarType type;
+  if (n != 2 || !mx_operand(a[0], &q) || !out_type(a[1], &type)) Py_RETURN_NONE;
+  at::Tensor out = result(q.buf, at::IntArrayRef(q.size, q.dims), type);
+  void *s = stream(), *dst = out.data_ptr();
+  char *src = q.data();
+  if (without_gil([&] { return glib.dequantize(src, src + q.codes, q.rows, (int32_t)q.size[q.dims - 1], dst, float_code(type), s); }) != UNIT_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+const at::Tensor *group_sizes(PyObject *o, int64_t groups, const at::Tensor &like) {
+  const at::Tensor *t = operand(o, at::kInt, 1);
+  if (!t) t = operand(o, at::kLong, 1);
+  return t && t->size(0) == groups && t->device() == like.device() ? t : nullptr;
+}
+
+// (data, weight, group sizes or None, out_dtype)
+PyObject *product_mx(PyObject *const *a, Py_ssize_t n) {
+  Mx w, q;
+  at::ScalarType type;
+  if (n != 4 || !mx_operand(a[1], &w) || !out_type(a[3], &type)) Py_RETURN_NONE;
+  const bool grouped = a[2] != Py_None;
+  if (w.dims != (grouped ? 3 : 2)) Py_RETURN_NONE;
+  const int32_t k = (int32_t)w.size[w.dims - 1], cols = (int32_t)w.size[w.dims - 2], groups = grouped ? (int32_t)w.size[0] : 1;
+  int code = UNIT_MXFP4;
+  const at::Tensor *x = floats(a[0], &code);
+  at::Tensor ws;
+  size_t need = 0;
+  void *xp, *xsp = nullptr;
+  int64_t rows;
+  if (x) {
+    if (x->dim() != 2 || !small(*x) || x->size(1) != k) Py_RETURN_NONE;
+    rows = x->size(0);
+    if (glib.mx_workspace((int32_t)rows, k, &need) != UNIT_OK) Py_RETURN_NONE;
+    if (need) ws = result(*x, {(int64_t)need}, at::kByte);
+    xp = x->data_ptr();
+  } else {
+    code = UNIT_MXFP4;
+    if (!mx_operand(a[0], &q) || q.dims != 2 || q.size[1] != k) Py_RETURN_NONE;
+    x = &q.buf;
+    rows = q.rows;
+    xp = q.data();
+    xsp = q.data() + q.codes;
+  }
+  if (x->device() != w.buf.device()) Py_RETURN_NONE;
+  const at::Tensor *sizes = grouped ? group_sizes(a[2], groups, *x) : nullptr;
+  if (grouped && !sizes) Py_RETURN_NONE;
+  at::Tensor out = result(*x, {rows, cols}, type);
+  void *s = stream(), *o = out.data_ptr(), *wsp = need ? ws.data_ptr() : nullptr, *gp = sizes ? sizes->data_ptr() : nullptr;
+  char *wp = w.data();
+  const int width = sizes ? (int)sizes->element_size() : 4, out_code = float_code(type);
+  const int rc = without_gil([&] {
+    return grouped ? glib.grouped_mx(xp, xsp, code, wp, wp + w.codes, gp, width, o, out_code, (int32_t)rows, groups, cols, k, wsp, need, s)
+                   : glib.dense_mx(xp, xsp, code, wp, wp + w.codes, o, out_code, (int32_t)rows, cols, k, wsp, need, s);
+  });
+  if (rc != UNIT_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// data (rows, K), weight (E, N, K), group sizes of a 16-bit product
+struct Experts {
+  const at::Tensor *x, *w, *sizes;
+  int32_t rows, groups, cols, k;
+  int code, width;
+};
+bool experts(PyObject *x, PyObject *w, PyObject *sizes, Experts *e) {
+  e->x = floats(x, &e->code);
+  if (!e->x || e->code == UNIT_F32 || e->x->dim() != 2 || !small(*e->x)) return false;
+  e->w = operand(w, e->x->scalar_type(), 3);
+  if (!e->w || !small(*e->w) || e->w->size(2) != e->x->size(1) || e->w->device() != e->x->device()) return false;
+  e->rows = (int32_t)e->x->size(0), e->groups = (int32_t)e->w->size(0), e->cols = (int32_t)e->w->size(1), e->k = (int32_t)e->w->size(2);
+  e->sizes = group_sizes(sizes, e->groups, *e->x);
+  if (!e->sizes) return false;
+  e->width = (int)e->sizes->element_size();
+  return true;
+}
+
+// (data, weight, group sizes, out_dtype)
+PyObject *grouped(PyObject *const *a, Py_ssize_t n) {
+  Experts e;
+  at::ScalarType type;
+  if (n != 4 || !experts(a[0], a[1], a[2], &e) || !out_type(a[3], &type)) Py_RETURN_NONE;
+  at::Tensor out = result(*e.x, {e.rows, e.cols}, type);
+  return finish(std::move(out), [&](void *s, void *xp, void *wp, void *gp, void *o) {
+    return glib.grouped(xp, wp, gp, e.width, o, e.code, float_code(type), e.rows, e.groups, e.cols, e.k, s);
+  }, *e.x, *e.w, *e.sizes);
+}
+
+// (data, weight, grad, group sizes, out_dtype, weight_out_dtype)
+PyObject *grouped_grad(PyObject *const *a, Py_ssize_t n) {
+  Experts e;
+  at::ScalarType type, wtype;
+  if (n != 6 || !experts(a[0], a[1], a[3], &e) || !out_type(a[4], &type) || !out_type(a[5], &wtype)) Py_RETURN_NONE;
+  const at::Tensor *dy = operand(a[2], e.x->scalar_type(), 2);
+  if (!dy || dy->size(0) != e.rows || dy->size(1) != e.cols || dy->device() != e.x->device()) Py_RETURN_NONE;
+  at::Tensor dx = result(*e.x, {e.rows, e.k}, type), dw = result(*e.x, {e.groups, e.cols, e.k}, wtype);
+  void *s = stream(), *xp = e.x->data_ptr(), *wp = e.w->data_ptr(), *yp = dy->data_ptr(), *gp = e.sizes->data_ptr(), *dxp = dx.data_ptr(), *dwp = dw.data_ptr();
+  const int rc = without_gil([&] {
+    const int first = glib.grad_data(yp, wp, gp, e.width, dxp, e.code, float_code(type), e.rows, e.groups, e.cols, e.k, s);
+    return first ? first : glib.grad_weight(xp, yp, gp, e.width, dwp, e.code, float_code(wtype), e.rows, e.groups, e.cols, e.k, s);
+  });
+  if (rc != UNIT_OK) Py_RETURN_NONE;
+  PyObject *both = PyTuple_New(2);
+  if (!both) throw std::bad_alloc();
+  PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(dx)));
+  PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(dw)));
+  return both;
+}
+
+// `addresses`, a tuple of `count` of them
+bool take_addresses(PyObject *addresses, int count, void **f) {
+  if (!PyTuple_CheckExact(addresses) || PyTuple_GET_SIZE(addresses) != count) {
+    PyErr_SetString(PyExc_ValueError, "bind: unexpected arguments");
+    return false;
+  }
+  for (int i = 0; i < count; ++i) {
+    f[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(addresses, i));
+    if (!f[i]) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
+      return false;
+    }
+  }
+  return true;
+}
+
+// (addresses in GroupedLibrary's order, Mxfp4Tensor)
+PyObject *bind_grouped(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  void *f[kGroupedFunctions];
+  if (n != 2) {
     PyErr_SetString(PyExc_ValueError, "bind: unexpected arguments");
     return nullptr;
   }
+  if (!take_addresses(a[0], kGroupedFunctions, f)) return nullptr;
+  memcpy(&glib, f, sizeof glib);
+  Py_INCREF(a[1]);
+  Py_XDECREF(mx_type);
+  mx_type = a[1];
+  Py_RETURN_NONE;
+}
+
+// (addresses in Library's order, the three prepared classes, torch.int8, torch.float16)
+PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   void *f[kFunctions];
-  for (int i = 0; i < kFunctions; ++i) {
-    f[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(a[0], i));
-    if (!f[i]) {
-      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
-      return nullptr;
-    }
+  if (n != 6) {
+    PyErr_SetString(PyExc_ValueError, "bind: unexpected arguments");
+    return nullptr;
   }
+  if (!take_addresses(a[0], kFunctions, f)) return nullptr;
   memcpy(&lib, f, sizeof lib);
   PyObject **const kept[] = {&conv_weight_type, &dense_weight_type, &gemm_b_type, &dtype_s8, &dtype_f16};
   for (int i = 0; i < 5; ++i) {
@@ -386,6 +623,9 @@ constexpr PyMethodDef method(const char *name) {
 PyMethodDef methods[] = {
     method<conv_u8>("conv_u8"),   method<conv_fused>("conv_fused"), method<conv_requant>("conv_requant"), method<conv3d>("conv3d"),
     method<conv_f16>("conv_f16"), method<dense>("dense"),           method<gemm>("gemm"),
+    method<quantize>("quantize"), method<dequantize>("dequantize"), method<product_mx>("product_mx"),     method<grouped>("grouped"),
+    method<grouped_grad>("grouped_grad"),
+    {"bind_grouped", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind_grouped)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
@@ -398,7 +638,7 @@ extern "C" __attribute__((visibility("default"))) PyObject *PyInit__calls() {
     PyObject **name;
     const char *text;
   } const names[] = {{&n_buf, "buf"}, {&n_K, "K"},         {&n_C, "C"}, {&n_KH, "KH"},     {&n_KW, "KW"}, {&n_cb, "cb"},
-                     {&n_N, "N"},     {&n_dtype, "dtype"}, {&n_w, "w"}, {&n_wsum, "wsum"}, {&n_bt, "bt"}};
+                     {&n_N, "N"},     {&n_dtype, "dtype"}, {&n_w, "w"}, {&n_wsum, "wsum"}, {&n_bt, "bt"}, {&n_shape, "shape"}};
   for (const auto &x : names)
     if (!(*x.name = PyUnicode_InternFromString(x.text))) return nullptr;
   return PyModule_Create(&module);

@@ -177,6 +177,9 @@ class _Calls:
                 "unit_conv2d_nchw_f16f32_ws_bytes", "unit_dense_dotprod_u8s8s32", "unit_dense_u8s8s32", "unit_dense_u8s8s32_prepared",
                 "unit_gemm_f16", "unit_gemm_f16_prepared", "unit_gemm_f16_ws")
 
+    def _bind(self, calls, addresses):
+        calls.bind(addresses, PreparedConvWeight, PreparedDenseWeight, PreparedGemmB, torch.int8, torch.float16)
+
     def __getattr__(self, name):  # the first use of each function
         if name not in self._NAMES:
             raise AttributeError(name)
@@ -186,8 +189,7 @@ class _Calls:
             return _declined
         try:
             from . import _calls
-            _calls.bind(tuple(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in self._LIBRARY), PreparedConvWeight,
-                        PreparedDenseWeight, PreparedGemmB, torch.int8, torch.float16)
+            self._bind(_calls, tuple(ctypes.cast(getattr(L, f), ctypes.c_void_p).value for f in self._LIBRARY))
             fn = getattr(_calls, name)
         except (ImportError, AttributeError, ValueError) as e:
             fn = _declined
