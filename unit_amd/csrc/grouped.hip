@@ -102,14 +102,16 @@ int run_mxfp4(const char *what, const void *x, const void *xscales, int x_dtype,
   }
   if (int rc = check_device()) return rc;
   if (!rows) return UNIT_OK;
+  GroupedParams p{static_cast<const char *>(x), static_cast<const char *>(wcodes), static_cast<const u32 *>(xscales), static_cast<const u32 *>(wscales),
+                  static_cast<char *>(out), sizes, size_bytes, groups, rows, N, K, x_dtype};
+  if (floats && grouped_mx_takes_floats(p)) return run_grouped_mx(what, p, out_dtype, s);
   if (floats) {
     char *buf = static_cast<char *>(ws);
     if (int rc = unit_quantize_mxfp4(x, x_dtype, rows, K, buf, buf + codes, s)) return rc;
-    x = buf;
-    xscales = buf + codes;
+    p.x = buf;
+    p.xs = reinterpret_cast<const u32 *>(buf + codes);
+    p.x_dtype = UNIT_MXFP4;
   }
-  GroupedParams p{static_cast<const char *>(x), static_cast<const char *>(wcodes), static_cast<const u32 *>(xscales), static_cast<const u32 *>(wscales),
-                  static_cast<char *>(out), sizes, size_bytes, groups, rows, N, K};
   return run_grouped_mx(what, p, out_dtype, s);
 }
 

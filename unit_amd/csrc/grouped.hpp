@@ -22,6 +22,7 @@ struct GroupedParams {
   int size_bytes;          // 4 or 8
   int groups, rows;        // groups, rows of the row operands
   int n, k;                // weight (groups, n, k)
+  int x_dtype;             // MXFP4 products: UNIT_MXFP4, or UNIT_F16 / UNIT_BF16 for x still in floats
 };
 
 __device__ __forceinline__ int group_size(const GroupedParams &p, int g) {
@@ -35,6 +36,7 @@ __device__ __forceinline__ int group_size(const GroupedParams &p, int g) {
 enum { FORWARD, GRAD_DATA, GRAD_WEIGHT };
 int run_grouped_f16(const char *what, int dir, const GroupedParams &p, int out_dtype, hipStream_t s);
 int run_grouped_bf16(const char *what, int dir, const GroupedParams &p, int out_dtype, hipStream_t s);
+bool grouped_mx_takes_floats(const GroupedParams &p);
 int run_grouped_mx(const char *what, const GroupedParams &p, int out_dtype, hipStream_t s);
 
 }  // namespace unit

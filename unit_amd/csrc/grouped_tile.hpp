@@ -59,6 +59,56 @@ __device__ __forceinline__ u32 scan_upto(u32 v, u32 top) {
   return v;
 }
 
+// Where the groups begin and end, in rows and in tiles of BM rows: sums of sizes over the lanes, lane l for group l of the chunk of 64
+// at hand.  Every wave does this by itself.
+template <int BM>
+struct GroupScan {
+  u32 rows0, tiles0;      // rows and tiles of the chunks before
+  u32 start, end, tend;   // this lane's group: first row, end of rows, end of tiles
+  u32 rows_in, tiles_in;  // rows and tiles of all groups
+  int chunks;
+
+  __device__ __forceinline__ void chunk(const GroupedParams &p, int c, int lane) {
+    const int g = c * 64 + lane;
+    const u32 size = g < p.groups ? (u32)group_size(p, g) : 0;
+    end = min(rows0 + scan_upto(size, (u32)p.rows), (u32)p.rows);
+    start = (u32)__builtin_amdgcn_update_dpp((int)rows0, (int)end, 0x138, 0xf, 0xf, false);  // the lane before's; lane 0: rows0
+    tend = tiles0 + scan_upto((end - start + BM - 1) / BM, 1u << 30);
+  }
+  __device__ __forceinline__ void run(const GroupedParams &p, int lane) {
+    rows0 = tiles0 = 0;
+    chunks = (p.groups + 63) / 64;
+    for (int c = 0; c < chunks; ++c) {
+      if (c) rows0 = lane_value(end, 63), tiles0 = lane_value(tend, 63);
+      chunk(p, c, lane);
+    }
+    rows_in = lane_value(end, 63), tiles_in = lane_value(tend, 63);
+  }
+  // tiles of all rows, those of no group included
+  __device__ __forceinline__ u32 total(const GroupedParams &p) const { return tiles_in + ((u32)p.rows - rows_in + BM - 1) / BM; }
+  // the group of row tile m < total(): itself (p.groups: none), its rows, and how many tiles lie before them
+  __device__ __forceinline__ void find(const GroupedParams &p, u32 m, int lane, int &group, int &first, int &count, u32 &before) {
+    if (m >= tiles_in) {
+      group = p.groups, first = (int)rows_in, count = p.rows - (int)rows_in, before = tiles_in;
+      return;
+    }
+    int c = 0;
+    if (chunks > 1) {
+      rows0 = tiles0 = 0;
+      for (;; ++c) {
+        chunk(p, c, lane);
+        if (lane_value(tend, 63) > m) break;
+        rows0 = lane_value(end, 63), tiles0 = lane_value(tend, 63);
+      }
+    }
+    const int l = __builtin_ctzll(__ballot(tend > m));  // ends never decrease: the first group that ends behind m
+    group = c * 64 + l;
+    first = (int)lane_value(start, l);
+    count = (int)lane_value(end, l) - first;
+    before = l ? lane_value(tend, l - 1) : tiles0;
+  }
+};
+
 struct GroupTileOf {
   int group;         // p.groups: rows of no group
   int first, count;  // the group's rows
@@ -66,67 +116,27 @@ struct GroupTileOf {
   bool any;          // the workgroup has a tile
 };
 
-// The tile of workgroup `bid`.  Every wave does this by itself, lanes over groups: sums of sizes give the rows, sums of tile counts the
-// tiles; the number of tiles is known here only, so the host launches what any sizes can need and the rest ends at once.
-// Workgroups are dealt round-robin to the eight XCDs: those of one XCD take consecutive tiles, which walk a group in panels of PH
-// row tiles, column tile after column tile, so that the XCD's L2 holds the panel's rows and sees each weight tile once a panel.
+// The tile of workgroup `bid`.  The number of tiles is known here only, so the host launches what any sizes can need and the rest
+// ends at once.  Workgroups are dealt round-robin to the eight XCDs: those of one XCD take consecutive tiles, which walk a group in
+// panels of PH row tiles, column tile after column tile, so that the XCD's L2 holds the panel's rows and sees each weight tile once
+// a panel.
 template <int BM, int PH>
 __device__ __forceinline__ GroupTileOf find_tile(const GroupedParams &p, int nts, int bid, int lane) {
   GroupTileOf t;
-  u32 rows0 = 0, tiles0 = 0;  // of the chunks of 64 groups before
-  u32 start = 0, end = 0, tend = 0;
-  auto chunk = [&](int c) __attribute__((always_inline)) {
-    const int g = c * 64 + lane;
-    const u32 size = g < p.groups ? (u32)group_size(p, g) : 0;
-    end = min(rows0 + scan_upto(size, (u32)p.rows), (u32)p.rows);
-    start = (u32)__shfl_up((int)end, 1);
-    start = lane ? start : rows0;
-    tend = tiles0 + scan_upto((end - start + BM - 1) / BM, 1u << 30);
-  };
-  const int chunks = (p.groups + 63) / 64;
-  for (int c = 0; c < chunks; ++c) {
-    if (c) rows0 = lane_value(end, 63), tiles0 = lane_value(tend, 63);
-    chunk(c);
-  }
-  const u32 rows_in = lane_value(end, 63), tiles_in = lane_value(tend, 63);
-  const u32 total = (tiles_in + ((u32)p.rows - rows_in + BM - 1) / BM) * (u32)nts;
+  GroupScan<BM> scan;
+  scan.run(p, lane);
+  const u32 total = scan.total(p) * (u32)nts;
   const u32 per = total / 8, rem = total % 8, xcd = (u32)bid % 8, idx = (u32)bid / 8;
   const u32 logical = xcd * per + min(xcd, rem) + idx;
   t.any = idx < per + (xcd < rem ? 1u : 0u);
   if (!t.any) return t;
-  const u32 m = scalar(logical / (u32)nts);  // in whole row tiles of all groups: a group is nts * (its row tiles)
   u32 before;
-  if (m >= tiles_in) {
-    t.group = p.groups;
-    t.first = (int)rows_in;
-    t.count = p.rows - (int)rows_in;
-    before = tiles_in;
-  } else {
-    if (chunks > 1) {
-      rows0 = tiles0 = 0;
-      for (int c = 0;; ++c) {
-        chunk(c);
-        if (lane_value(tend, 63) > m) {
-          t.group = c * 64;
-          break;
-        }
-        rows0 = lane_value(end, 63), tiles0 = lane_value(tend, 63);
-      }
-    } else {
-      t.group = 0;
-    }
-    const int l = __builtin_ctzll(__ballot(tend > m));  // ends never decrease: the first group that ends behind m
-    t.group += l;
-    t.first = (int)lane_value(start, l);
-    t.count = (int)lane_value(end, l) - t.first;
-    before = l ? lane_value(tend, l - 1) : tiles0;
-  }
+  scan.find(p, scalar(logical / (u32)nts), lane, t.group, t.first, t.count, before);  // a group is nts * (its row tiles)
   const u32 mts = ((u32)t.count + BM - 1) / BM, within = scalar(logical) - before * (u32)nts;
   const u32 panel = within / ((u32)nts * PH), in_panel = within - panel * ((u32)nts * PH);
   const u32 high = min(mts - panel * PH, (u32)PH);
   t.nt = (int)scalar(in_panel / high);
   t.mt = (int)scalar(panel * PH + in_panel - (u32)t.nt * high);
-  t.group = (int)scalar((u32)t.group);
   return t;
 }
 
@@ -137,8 +147,7 @@ __device__ __forceinline__ void find_rows(const GroupedParams &p, int g, int lan
     if (c) rows0 = lane_value(end, 63);
     const int i = c * 64 + lane;
     end = min(rows0 + scan_upto(i < p.groups ? (u32)group_size(p, i) : 0, (u32)p.rows), (u32)p.rows);
-    start = (u32)__shfl_up((int)end, 1);
-    start = lane ? start : rows0;
+    start = (u32)__builtin_amdgcn_update_dpp((int)rows0, (int)end, 0x138, 0xf, 0xf, false);
   }
   first = (int)lane_value(start, g % 64);
   count = (int)lane_value(end, g % 64) - first;
@@ -155,6 +164,14 @@ __device__ __forceinline__ v4i bounded(const char *base, u32 bytes) {
   return r;
 }
 constexpr u32 kOutside = 0xfffffff0u;  // past every descriptor
+
+// XOR of the 16-byte chunk position inside a row of a "cols" tile, so that the four rows of a transposing read fall into
+// different bank groups (rows of 128, 256 or 512 bytes)
+template <int WIDTH>
+__device__ __forceinline__ int cols_swz(int row) {
+  static_assert(WIDTH == 64 || WIDTH == 128 || WIDTH == 256, "tile widths");
+  return WIDTH == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3);
+}
 
 template <class Op, int DIR, class T, int NSTAGE, class Out>
 __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nts, int xts) {
@@ -215,29 +232,23 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
   }
   const long xstep = XT ? (long)KS * xld : T::BKB, ystep = YT ? (long)KS * yld : T::BKB;  // bytes from stage to stage
 
-  // this lane's chunk of each load; rows: the byte of the stage's row it holds, to compare with the reduction's end
+  // this lane's chunk of each load
   u32 xoff[XL], yoff[YL];
-  auto offsets = [&](u32(&off)[XL > YL ? XL : YL], int n, bool cols, int width, long ld) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      if (cols) {
-        const int cpr = width / 8, row = (wave * n + i) * (64 / cpr) + lane / cpr;
-        off[i] = (u32)row * (u32)ld + (u32)(((lane % cpr) ^ (4 * (row & 3))) << 4);
-      } else {
-        const int row = (wave * n + i) * RPL + lane / CPR;
-        off[i] = (u32)row * (u32)ld + (u32)(((lane % CPR) ^ swz<T::BKB>(row)) << 4);
-      }
+  auto offset = [&](auto cols, auto width, int load, long ld) __attribute__((always_inline)) {
+    constexpr int W = decltype(width)::value;
+    if constexpr (decltype(cols)::value) {
+      constexpr int CPW = W / 8;
+      const int row = load * (64 / CPW) + lane / CPW;
+      return (u32)row * (u32)ld + (u32)(((lane % CPW) ^ cols_swz<W>(row)) << 4);
+    } else {
+      const int row = load * RPL + lane / CPR;
+      return (u32)row * (u32)ld + (u32)(((lane % CPR) ^ swz<T::BKB>(row)) << 4);
     }
   };
-  {
-    u32 tmp[XL > YL ? XL : YL];
-    offsets(tmp, XL, XT, T::BX, xld);
 #pragma unroll
-    for (int i = 0; i < XL; ++i) xoff[i] = tmp[i];
-    offsets(tmp, YL, YT, T::BY, yld);
+  for (int i = 0; i < XL; ++i) xoff[i] = offset(std::integral_constant<bool, XT>{}, std::integral_constant<int, T::BX>{}, wave * XL + i, xld);
 #pragma unroll
-    for (int i = 0; i < YL; ++i) yoff[i] = tmp[i];
-  }
+  for (int i = 0; i < YL; ++i) yoff[i] = offset(std::integral_constant<bool, YT>{}, std::integral_constant<int, T::BY>{}, wave * YL + i, yld);
   // MXFP4: the scales of a stage, X rows then Y rows, each [half][row] dwords, 64 pieces of four rows per load
   const char *sptr = nullptr;
   long sstep = 0;
@@ -290,14 +301,17 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
   int xtr[T::TX], ytr[T::TY];
   {
     const int jrow = (lane & 15) >> 2, q = lane & 3, g16 = (lane >> 4) & 1;
-    auto at = [&](int c, int width) { return (8 * half + jrow) * (width * 2) + (((c + 2 * g16 + (q >> 1)) ^ (4 * jrow)) << 4) + (q & 1) * 8; };
+    auto at = [&](int c, auto width) {
+      constexpr int W = decltype(width)::value;
+      return (8 * half + jrow) * (W * 2) + (((c + 2 * g16 + (q >> 1)) ^ cols_swz<W>(jrow)) << 4) + (q & 1) * 8;
+    };
     if constexpr (XT) {
 #pragma unroll
-      for (int i = 0; i < T::TX; ++i) xtr[i] = at(wx * (T::TX * 4) + i * 4, T::BX);
+      for (int i = 0; i < T::TX; ++i) xtr[i] = at(wx * (T::TX * 4) + i * 4, std::integral_constant<int, T::BX>{});
     }
     if constexpr (YT) {
 #pragma unroll
-      for (int j = 0; j < T::TY; ++j) ytr[j] = T::XBYTES + at(wy * (T::TY * 4) + j * 4, T::BY);
+      for (int j = 0; j < T::TY; ++j) ytr[j] = T::XBYTES + at(wy * (T::TY * 4) + j * 4, std::integral_constant<int, T::BY>{});
     }
   }
   auto transposed = [&](const char *src, int pitch) __attribute__((always_inline)) {
@@ -456,20 +470,29 @@ int run_grouped_tile(const char *what, const char *tag, const GroupedParams &p, 
   return UNIT_OK;
 }
 
-// Large tiles (256 x 256) where the groups' rows fill them on average, else 128 x 128.  us, experts of 512 rows on average, 16384 x
-// 1024 -> 2048: 103 against 124; MXFP4 333 x 2088 -> 1516: 22.5 against 13.8.
-inline bool grouped_large(const GroupedParams &p, int dir) {
-  const int pinned = tuning_override("UNIT_AMD_GROUPED_TILE");
-  if (pinned) return pinned == 2;
-  const int xs = dir == GRAD_WEIGHT ? p.n : p.rows / p.groups, ys = dir == FORWARD ? p.n : p.k;
-  const long tiles = (long)ceil_div(xs, 256) * ceil_div(ys, 256) * p.groups;
-  return xs >= 192 && ys >= 192 && tiles >= 128;
+// Which tile.  xs, ys: rows of the first and second operand in a group, on average over the groups that can have any.
+enum { TILE_FEW, TILE_SMALL, TILE_MIDDLE, TILE_LARGE };
+inline int grouped_tile_size(const GroupedParams &p, int dir) {
+  if (const int pinned = tuning_override("UNIT_AMD_GROUPED_TILE")) return pinned - 1;
+  const long busy = p.groups < p.rows ? p.groups : (p.rows ? p.rows : 1);
+  const long xs = dir == GRAD_WEIGHT ? p.n : (p.rows + busy - 1) / busy, ys = dir == FORWARD ? p.n : p.k, groups = dir == GRAD_WEIGHT ? p.groups : busy;
+  const auto tiles = [&](int x, int y) { return (xs + x - 1) / x * ((ys + y - 1) / y) * groups; };
+  if (dir == FORWARD && xs <= 32) return TILE_FEW;
+  const long k = dir == FORWARD ? p.k : dir == GRAD_DATA ? p.n : p.rows / p.groups;
+  if (xs >= 192 && ys >= 192 && tiles(256, 256) >= 128 && xs * ys * groups >= (1l << 32) / (k + 1)) return TILE_LARGE;
+  return tiles(128, 128) >= 512 ? TILE_MIDDLE : TILE_SMALL;
 }
 
 template <class Op, int DIR, class Out>
 int run_grouped_sizes(const char *what, const char *tag, const GroupedParams &p, hipStream_t s) {
-  if (grouped_large(p, DIR)) return run_grouped_tile<Op, DIR, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
-  return run_grouped_tile<Op, DIR, Tile<128, 128, 64, 2, 2>, 4, Out>(what, tag, p, s);
+  switch (grouped_tile_size(p, DIR)) {
+    case TILE_FEW:
+      if constexpr (DIR == FORWARD) return run_grouped_tile<Op, DIR, Tile<32, 128, 128, 1, 4>, 3, Out>(what, tag, p, s);
+      [[fallthrough]];
+    case TILE_SMALL: return run_grouped_tile<Op, DIR, Tile<64, 64, 128, 2, 2>, 3, Out>(what, tag, p, s);
+    case TILE_MIDDLE: return run_grouped_tile<Op, DIR, Tile<128, 128, 64, 2, 2>, 4, Out>(what, tag, p, s);
+    default: return run_grouped_tile<Op, DIR, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
+  }
 }
 
 }  // namespace unit

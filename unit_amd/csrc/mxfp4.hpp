@@ -31,4 +31,59 @@ __device__ __forceinline__ u32 mx_scale(u32 amax_bits) {
 // 2^(s - 127); s = 0 is a subnormal float
 __device__ __forceinline__ float mx_power(u32 s) { return __builtin_bit_cast(float, s ? s << 23 : 1u << 22); }
 
+// eight elements of a row as their bits
+template <class T>
+struct Eight {
+  using bits = std::conditional_t<sizeof(T) == 4, u32, unsigned short>;
+  typedef bits b8 __attribute__((ext_vector_type(8)));
+};
+
+// Scaling by a power of two and rounding to the nearest element (ties to the even mantissa, magnitudes above 6 to 6) are what
+// v_cvt_scalef32_pk_fp4 does.
+template <class T>
+__device__ __forceinline__ u32 eight_codes(typename Eight<T>::b8 v, float p) {
+  u32 c = 0;
+  auto two = [&](auto n) __attribute__((always_inline)) {
+    constexpr int N = decltype(n)::value;
+    if constexpr (std::is_same_v<T, float>) {
+      typedef float v8f __attribute__((ext_vector_type(8)));
+      const v8f f = __builtin_bit_cast(v8f, v);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2 * N], f[2 * N + 1], p, N);
+    } else {
+      typedef T v2 __attribute__((ext_vector_type(2)));
+      const u32 pair = __builtin_bit_cast(v4u, v)[N];
+      if constexpr (std::is_same_v<T, _Float16>)
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(v2, pair), p, N);
+      else
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(v2, pair), p, N);
+    }
+  };
+  two(std::integral_constant<int, 0>{});
+  two(std::integral_constant<int, 1>{});
+  two(std::integral_constant<int, 2>{});
+  two(std::integral_constant<int, 3>{});
+  return c;
+}
+
+// the bits of the largest magnitude of eight elements, as a float; infinities and NaN are the largest
+template <class T>
+__device__ __forceinline__ u32 eight_top(typename Eight<T>::b8 v) {
+  u32 top = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, v[i] & 0x7fffffffu);
+    return top;
+  } else {
+    // sign-less 16-bit patterns are ordered like the values: two at a time
+    const v4u w = __builtin_bit_cast(v4u, v);
+    typedef unsigned short v2s __attribute__((ext_vector_type(2)));
+    v2s m = __builtin_bit_cast(v2s, w[0] & 0x7fff7fffu);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(v2s, w[i] & 0x7fff7fffu));
+    top = max((u32)m[0], (u32)m[1]);
+    if constexpr (std::is_same_v<T, __bf16>) return top << 16;
+    return __builtin_bit_cast(u32, (float)__builtin_bit_cast(_Float16, (unsigned short)top)) & 0x7fffffffu;  // NaN stays NaN
+  }
+}
+
 }  // namespace unit
