@@ -8,7 +8,8 @@
 //   forward        X = x rows,  Y = w rows       out[row][n]
 //   data gradient  X = dy rows, Y = w cols       dx[row][k]
 //   weight gradient X = dy cols, Y = x cols      dw[n][k], the reduction runs over a group's rows
-// X is the first MFMA operand: the result's rows lie along the accumulator registers, its columns along the lanes.
+// Y is the first MFMA operand: the result's rows lie along the lanes, its columns along the accumulator registers, four consecutive ones
+// in four registers, so that results leave 16 bytes at a time (through LDS, where they are put in order).
 //
 // Bounds.  A stage's descriptor begins at the stage's first byte and ends where the operand's valid rows end, so rows past a group's
 // last (weight gradient) read as zeros, and rows past a tile's last valid one read as zeros or stay in the tensor.  A reduction that ends
@@ -359,9 +360,9 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
     for (int m = 0; m < NM; ++m) {
       const int i = m / T::TY, j = m % T::TY;
       if constexpr (MX)
-        acc[i][j] = Op::template mma<decltype(kkc)::value>(xf[s][i], yf[s][j], acc[i][j], sx[0][i], sy[0][j]);
+        acc[i][j] = Op::template mma<decltype(kkc)::value>(yf[s][j], xf[s][i], acc[i][j], sy[0][j], sx[0][i]);
       else
-        acc[i][j] = Op::mma(xf[s][i], yf[s][j], acc[i][j]);
+        acc[i][j] = Op::mma(yf[s][j], xf[s][i], acc[i][j]);
       if constexpr (decltype(has_read)::value) {
 #pragma unroll
         for (int f = m * NF / NM; f < (m + 1) * NF / NM; ++f) load_one(rd_stage, rd_kk, s ^ 1, f);
@@ -425,20 +426,48 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
     stage(kt, kt % NSTAGE, no{}, no{}, no{}, no{});
   }
 
-  // results: rounded once, here
+  // Results, rounded once, here: each wave puts 32 rows of its columns in order in LDS of its own and writes them in runs of 16 bytes a lane.
+  // (Straight from the registers, 2 bytes a lane, the stores of a 256 x 256 tile of 16-bit results took 4 us.)
+  constexpr int ES_OUT = (int)sizeof(Out), PITCH = T::TY * 32 * ES_OUT + 16, PER = 16 / ES_OUT, RUNS = T::TY * 32 / PER;  // elements per run, runs per row
+  static_assert(NW * 32 * PITCH <= NSTAGE * STAGE, "the waves' rows fit the ring");
+  __syncthreads();  // the ring is read out
+  char *const rows = lds + wave * (32 * PITCH);
   const long out_row = (DIR == GRAD_WEIGHT ? (long)group * p.n : (long)first) + x0;
   const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(p.out + out_row * ys * (long)sizeof(Out), 0, -1, 0x00020000);
+  const bool whole = ys % PER == 0;
+  typedef Out v4o __attribute__((ext_vector_type(4)));
 #pragma unroll
-  for (int j = 0; j < T::TY; ++j) {
-    const int y = y0 + wy * (T::TY * 32) + j * 32 + l32;
-    if (y >= ys) continue;
+  for (int i = 0; i < T::TX; ++i) {
+    const int xi = wx * (T::TX * 32) + i * 32;
+    if (x0 + xi >= xs) break;
 #pragma unroll
-    for (int i = 0; i < T::TX; ++i)
+    for (int j = 0; j < T::TY; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int x = wx * (T::TX * 32) + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (x0 + x < xs) store_result<kRowPolicy>(out, ((u32)x * (u32)ys + (u32)y) * (u32)sizeof(Out), (Out)acc[i][j][r]);
+      for (int r = 0; r < 4; ++r) {
+        v4o v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (Out)acc[i][j][4 * r + e];
+        *reinterpret_cast<v4o *>(rows + l32 * PITCH + (j * 32 + 8 * r + 4 * half) * ES_OUT) = v;
       }
+#pragma unroll
+    for (int k = 0; k < 32 * RUNS / 64; ++k) {
+      const int row = (k * 64 + lane) / RUNS, c = (k * 64 + lane) % RUNS * PER, x = xi + row, y = y0 + wy * (T::TY * 32) + c;
+      const v4u v = *reinterpret_cast<const v4u *>(rows + row * PITCH + c * ES_OUT);
+      if (x0 + x >= xs || y >= ys) continue;
+      const u32 at = ((u32)x * (u32)ys + (u32)y) * (u32)ES_OUT;
+      if (whole) {
+        store_result<kRowPolicy>(out, at, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (y + e < ys) {
+            if constexpr (ES_OUT == 4)
+              store_result<kRowPolicy>(out, at + e * 4, v[e]);
+            else
+              store_result<kRowPolicy>(out, at + e * 2, (unsigned short)(v[e / 2] >> (e % 2 * 16)));
+          }
+      }
+    }
   }
 }
 
