@@ -187,11 +187,10 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
   constexpr int STAGE = T::STAGE + PIECES * 1024;
   static_assert(XL * 1024 * NW == T::XBYTES && YL * 1024 * NW == T::YBYTES && KK % 2 == 0, "loads split evenly over the waves");
   static_assert(!MX || (T::BKB == 128 && PIECES <= NW && DIR == FORWARD), "a stage of MXFP4 is one dword of scales per row and half");
-  constexpr int NM = T::TX * T::TY, NF = T::TX + T::TY;
 
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int wx = wave % T::WX, wy = wave / T::WX, l32 = lane & 31, half = lane >> 5;
+  const int wx = wave / T::WY, wy = wave % T::WY, l32 = lane & 31, half = lane >> 5;  // waves of different rows share a SIMD
   const u32 ring = (u32)(uintptr_t)(lptr_t)lds;
 
   int group, first, count, x0, y0;
@@ -353,9 +352,14 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
   using yes = std::integral_constant<bool, true>;
   using no = std::integral_constant<bool, false>;
   // One k-step: MFMAs, each followed by its share of the next step's fragment reads and of the loads of a later stage.
-  auto step = [&](auto kkc, const char *rd_stage, int rd_kk, const Source &src, int issue_kt, int slot, auto has_read, auto has_issue, auto last)
+  // NX: how many of its row blocks this wave has rows for; the others are left out.
+  auto step = [&](auto nxc, auto kkc, const char *rd_stage, int rd_kk, const Source &src, int issue_kt, int slot, auto has_read, auto has_issue, auto last)
                   __attribute__((always_inline)) {
-    constexpr int s = decltype(kkc)::value & 1;
+    constexpr int s = decltype(kkc)::value & 1, NX = decltype(nxc)::value, NM = NX * T::TY, NF = NX ? NX + T::TY : 0;
+    if constexpr (NX == 0 && decltype(has_issue)::value) {
+#pragma unroll
+      for (int f = 0; f < LPS; ++f) issue_one(src, issue_kt, slot, f, last);
+    }
 #pragma unroll
     for (int m = 0; m < NM; ++m) {
       const int i = m / T::TY, j = m % T::TY;
@@ -376,11 +380,11 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
   };
   // One stage.  ISSUE: stage kt + NSTAGE exists and goes into the buffer that this stage frees; STEADY: NSTAGE - 1 younger stages are in
   // flight at the barrier; NEXT: stage kt + 1 exists; LAST: the stage that is fetched may hold the reduction's end.
-  auto stage = [&](int kt, int slot, auto issue_next, auto steady, auto next, auto last) __attribute__((always_inline)) {
+  auto stage = [&](auto nxc, int kt, int slot, auto issue_next, auto steady, auto next, auto last) __attribute__((always_inline)) {
     const char *cur = lds + slot * STAGE;
     const char *nxt = lds + (slot + 1 == NSTAGE ? 0 : slot + 1) * STAGE;
     const Source none{};
-    auto early = [&](auto kkc) __attribute__((always_inline)) { step(kkc, cur, decltype(kkc)::value + 1, none, 0, 0, yes{}, no{}, no{}); };
+    auto early = [&](auto kkc) __attribute__((always_inline)) { step(nxc, kkc, cur, decltype(kkc)::value + 1, none, 0, 0, yes{}, no{}, no{}); };
     early(std::integral_constant<int, 0>{});
     if constexpr (KK > 2) {
       early(std::integral_constant<int, 1>{});
@@ -395,7 +399,7 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
     __builtin_amdgcn_sched_barrier(0);
     Source src{};
     if constexpr (decltype(issue_next)::value) src = source(kt + NSTAGE);
-    step(std::integral_constant<int, KK - 1>{}, nxt, 0, src, kt + NSTAGE, slot, next, issue_next, last);
+    step(nxc, std::integral_constant<int, KK - 1>{}, nxt, 0, src, kt + NSTAGE, slot, next, issue_next, last);
     if constexpr (decltype(next)::value) next_scales();
   };
 
@@ -413,17 +417,32 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
       UNIT_WAIT_VMCNT(0);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
+    auto loop = [&](auto nxc) __attribute__((always_inline)) {
+      constexpr int NX = decltype(nxc)::value;
 #pragma unroll
-    for (int f = 0; f < NF; ++f) load_one(lds, 0, 0, f);
-    next_scales();
-    int kt = 0;
-    for (; kt + 2 * NSTAGE < nk; kt += NSTAGE) {  // fetches up to stage kt + 2 * NSTAGE - 1: never the last one
+      for (int f = 0; f < (NX ? NX + T::TY : 0); ++f) load_one(lds, 0, 0, f);
+      next_scales();
+      int kt = 0;
+      for (; kt + 2 * NSTAGE < nk; kt += NSTAGE) {  // fetches up to stage kt + 2 * NSTAGE - 1: never the last one
 #pragma unroll
-      for (int s = 0; s < NSTAGE; ++s) stage(kt + s, s, yes{}, yes{}, yes{}, no{});
-    }
-    for (; kt + NSTAGE < nk; ++kt) stage(kt, kt % NSTAGE, yes{}, yes{}, yes{}, yes{});
-    for (; kt + 1 < nk; ++kt) stage(kt, kt % NSTAGE, no{}, no{}, yes{}, no{});
-    stage(kt, kt % NSTAGE, no{}, no{}, no{}, no{});
+        for (int s = 0; s < NSTAGE; ++s) stage(nxc, kt + s, s, yes{}, yes{}, yes{}, no{});
+      }
+      for (; kt + NSTAGE < nk; ++kt) stage(nxc, kt, kt % NSTAGE, yes{}, yes{}, yes{}, yes{});
+      for (; kt + 1 < nk; ++kt) stage(nxc, kt, kt % NSTAGE, no{}, no{}, yes{}, no{});
+      stage(nxc, kt, kt % NSTAGE, no{}, no{}, no{}, no{});
+    };
+    // a wave without columns has no rows either
+    const int blocks = y0 + wy * (T::TY * 32) < ys ? min(max((xs - x0 - wx * (T::TX * 32) + 31) / 32, 0), T::TX) : 0;
+    if (blocks == T::TX)
+      loop(std::integral_constant<int, T::TX>{});
+    else if (blocks == 0)
+      loop(std::integral_constant<int, 0>{});
+    else if (T::TX > 2 && blocks == 3)
+      loop(std::integral_constant<int, T::TX < 3 ? T::TX : 3>{});
+    else if (T::TX > 2 && blocks == 2)
+      loop(std::integral_constant<int, T::TX < 2 ? T::TX : 2>{});
+    else
+      loop(std::integral_constant<int, 1>{});
   }
 
   // Results, rounded once, here: each wave puts 32 rows of its columns in order in LDS of its own and writes them in runs of 16 bytes a lane.
