@@ -30,10 +30,10 @@ __global__ __launch_bounds__(KW * 64, 2) void grouped_split(GroupedParams p, int
     t = find_tile<BM, 4>(p, nts, (int)blockIdx.x, lane);
     if (!t.any) return;
   } else {
-    t.group = 0, t.first = 0, t.count = p.rows, t.mt = 0, t.nt = (int)blockIdx.x;
+    t.group = 0, t.first = 0, t.count = p.rows, t.x0 = 0, t.nt = (int)blockIdx.x;
     if (t.nt >= nts) return;
   }
-  const int x0 = t.mt * BM, y0 = t.nt * BN, rows = min(t.count - x0, BM), cols = min(p.n - y0, BN);  // both positive
+  const int x0 = t.x0, y0 = t.nt * BN, rows = min(t.count - x0, BM), cols = min(p.n - y0, BN);  // both positive
   const int stages = mx_stages(p.k), ld = stages * 128, units = t.group < p.groups ? stages : 0;
   const long wrows = (long)p.groups * p.n, wrow = (long)t.group * p.n + y0;
 

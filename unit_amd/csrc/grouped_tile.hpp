@@ -113,7 +113,8 @@ struct GroupScan {
 struct GroupTileOf {
   int group;         // p.groups: rows of no group
   int first, count;  // the group's rows
-  int mt, nt;        // tile of the group's rows, tile of the columns
+  int x0, high;      // the tile's rows: first (of the group's), how many
+  int nt;            // tile of the columns
   bool any;          // the workgroup has a tile
 };
 
@@ -137,7 +138,11 @@ __device__ __forceinline__ GroupTileOf find_tile(const GroupedParams &p, int nts
   const u32 panel = within / ((u32)nts * PH), in_panel = within - panel * ((u32)nts * PH);
   const u32 high = min(mts - panel * PH, (u32)PH);
   t.nt = (int)scalar(in_panel / high);
-  t.mt = (int)scalar(panel * PH + in_panel - (u32)t.nt * high);
+  const u32 mt = panel * PH + in_panel - (u32)t.nt * high;
+  // as many tiles as BM asks for, of even heights in blocks of 32 rows; never beyond the end: (mts - 1) * BM < count
+  const u32 even = scalar(((u32)t.count + 32 * mts - 1) / (32 * mts)) * 32;
+  t.x0 = (int)scalar(mt * even);
+  t.high = min(t.count - t.x0, (int)even);
   return t;
 }
 
@@ -174,9 +179,9 @@ __device__ __forceinline__ int cols_swz(int row) {
   return WIDTH == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3);
 }
 
+// One tile: rows x0 .. x0 + high - 1 of the group's (weight gradient: rows of dw), columns y0 .. y0 + BY - 1.
 template <class Op, int DIR, class T, int NSTAGE, class Out>
-__global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nts, int xts) {
-  extern __shared__ __attribute__((aligned(16))) char lds[];
+__device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, int group, int first, int count, int x0, int high, int y0) {
   constexpr bool MX = Op::kMx, XT = DIR == GRAD_WEIGHT, YT = DIR != FORWARD;
   constexpr int ES = MX ? 0 : 2;                     // bytes per element of the 16-bit forms
   constexpr int KK = T::BKB / 32, CPR = T::CPR, NW = T::NT / 64, RPL = 64 / CPR;
@@ -191,25 +196,11 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wx = wave / T::WY, wy = wave % T::WY, l32 = lane & 31, half = lane >> 5;  // waves of different rows share a SIMD
+  // the row blocks there are, shared out evenly: this wave's first and how many
+  const int high32 = (high + 31) / 32, block0 = (high32 * wx + T::WX - 1) / T::WX, blocks_x = (high32 * (wx + 1) + T::WX - 1) / T::WX - block0;
   const u32 ring = (u32)(uintptr_t)(lptr_t)lds;
 
-  int group, first, count, x0, y0;
-  if constexpr (DIR == GRAD_WEIGHT) {
-    const int b = (int)blockIdx.x, per = (int)gridDim.x / 8, rem = (int)gridDim.x % 8, xcd = b % 8;
-    const int logical = xcd * per + min(xcd, rem) + b / 8;
-    group = logical / (nts * xts);
-    const int in = logical - group * (nts * xts);
-    y0 = in / xts * T::BY;
-    x0 = in % xts * T::BX;
-    find_rows(p, group, lane, first, count);
-  } else {
-    const GroupTileOf g = find_tile<T::BX, 4>(p, nts, (int)blockIdx.x, lane);
-    if (!g.any) return;
-    group = g.group, first = g.first, count = g.count;
-    x0 = g.mt * T::BX;
-    y0 = g.nt * T::BY;
-  }
-  const int xs = DIR == GRAD_WEIGHT ? p.n : count, ys = DIR == FORWARD ? p.n : p.k;  // extents of this group's result
+  const int ys = DIR == FORWARD ? p.n : p.k;  // columns of the result
   const bool live = group < p.groups;
 
   // operand bases (of this tile's first row or column), bytes per row, and how many bytes lie behind the base
@@ -224,7 +215,7 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
     xb = p.x + (long)first * xld + 2l * x0, xleft = (long)count * xld - 2l * x0;
     yb = p.y + (long)first * yld + 2l * y0, yleft = (long)count * yld - 2l * y0;
   } else {
-    xb = p.x + (long)(first + x0) * xld, xleft = (long)min(xs - x0, T::BX) * xld;
+    xb = p.x + (long)(first + x0) * xld, xleft = (long)high * xld;
     if constexpr (YT)
       yb = p.y + (long)group * p.n * yld + 2l * y0, yleft = (long)p.n * yld - 2l * y0;
     else
@@ -296,7 +287,7 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
   // fragment addresses inside a stage, k-step 0
-  const int xrow = wx * (T::TX * 32) + l32, yrow = wy * (T::TY * 32) + l32;
+  const int xrow = block0 * 32 + l32, yrow = wy * (T::TY * 32) + l32;
   const int xsw = swz<T::BKB>(xrow), ysw = swz<T::BKB>(yrow);
   int xtr[T::TX], ytr[T::TY];
   {
@@ -307,7 +298,7 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
     };
     if constexpr (XT) {
 #pragma unroll
-      for (int i = 0; i < T::TX; ++i) xtr[i] = at(wx * (T::TX * 4) + i * 4, std::integral_constant<int, T::BX>{});
+      for (int i = 0; i < T::TX; ++i) xtr[i] = at(block0 * 4 + i * 4, std::integral_constant<int, T::BX>{});
     }
     if constexpr (YT) {
 #pragma unroll
@@ -432,7 +423,7 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
       stage(nxc, kt, kt % NSTAGE, no{}, no{}, no{}, no{});
     };
     // a wave without columns has no rows either
-    const int blocks = y0 + wy * (T::TY * 32) < ys ? min(max((xs - x0 - wx * (T::TX * 32) + 31) / 32, 0), T::TX) : 0;
+    const int blocks = y0 + wy * (T::TY * 32) < ys ? blocks_x : 0;
     if (blocks == T::TX)
       loop(std::integral_constant<int, T::TX>{});
     else if (blocks == 0)
@@ -457,8 +448,8 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
   typedef Out v4o __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int i = 0; i < T::TX; ++i) {
-    const int xi = wx * (T::TX * 32) + i * 32;
-    if (x0 + xi >= xs) break;
+    if (i >= blocks_x) break;
+    const int xi = (block0 + i) * 32;
 #pragma unroll
     for (int j = 0; j < T::TY; ++j)
 #pragma unroll
@@ -472,7 +463,7 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
     for (int k = 0; k < 32 * RUNS / 64; ++k) {
       const int row = (k * 64 + lane) / RUNS, c = (k * 64 + lane) % RUNS * PER, x = xi + row, y = y0 + wy * (T::TY * 32) + c;
       const v4u v = *reinterpret_cast<const v4u *>(rows + row * PITCH + c * ES_OUT);
-      if (x0 + x >= xs || y >= ys) continue;
+      if (x >= high || y >= ys) continue;
       const u32 at = ((u32)x * (u32)ys + (u32)y) * (u32)ES_OUT;
       if (whole) {
         store_result<kRowPolicy>(out, at, v);
@@ -487,6 +478,24 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
           }
       }
     }
+  }
+}
+
+template <class Op, int DIR, class T, int NSTAGE, class Out>
+__global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nts, int xts) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63;
+  if constexpr (DIR == GRAD_WEIGHT) {
+    const int b = (int)blockIdx.x, per = (int)gridDim.x / 8, rem = (int)gridDim.x % 8, xcd = b % 8;
+    const int logical = xcd * per + min(xcd, rem) + b / 8;
+    const int group = logical / (nts * xts), in = logical - group * (nts * xts), x0 = in % xts * T::BX;
+    int first, count;
+    find_rows(p, group, lane, first, count);
+    compute_tile<Op, DIR, T, NSTAGE, Out>(p, lds, group, first, count, x0, min(p.n - x0, T::BX), in / xts * T::BY);
+  } else {
+    const GroupTileOf g = find_tile<T::BX, 4>(p, nts, (int)blockIdx.x, lane);
+    if (!g.any) return;
+    compute_tile<Op, DIR, T, NSTAGE, Out>(p, lds, g.group, g.first, g.count, g.x0, g.high, g.nt * T::BY);
   }
 }
 
@@ -533,13 +542,18 @@ inline int grouped_tile_size(const GroupedParams &p, int dir) {
 
 template <class Op, int DIR, class Out>
 int run_grouped_sizes(const char *what, const char *tag, const GroupedParams &p, hipStream_t s) {
+  switch (tuning_override("UNIT_AMD_GROUPED_TRY")) {
+    case 2: return run_grouped_tile<Op, DIR, Tile<256, 256, 64, 2, 4>, 4, Out>(what, tag, p, s);
+    case 4: return run_grouped_tile<Op, DIR, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
+  }
   switch (grouped_tile_size(p, DIR)) {
     case TILE_FEW:
       if constexpr (DIR == FORWARD) return run_grouped_tile<Op, DIR, Tile<32, 128, 128, 1, 4>, 3, Out>(what, tag, p, s);
       [[fallthrough]];
     case TILE_SMALL: return run_grouped_tile<Op, DIR, Tile<64, 64, 128, 2, 2>, 3, Out>(what, tag, p, s);
     case TILE_MIDDLE: return run_grouped_tile<Op, DIR, Tile<128, 128, 64, 2, 2>, 4, Out>(what, tag, p, s);
-    default: return run_grouped_tile<Op, DIR, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
+    default:
+      return run_grouped_tile<Op, DIR, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
   }
 }
 
