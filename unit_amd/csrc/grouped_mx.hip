@@ -9,10 +9,7 @@ int run(const char *what, const GroupedParams &p, hipStream_t s) {
   if (p.x_dtype == UNIT_F16) return run_grouped_split<_Float16, Out>(what, p, s);
   if (p.x_dtype == UNIT_BF16) return run_grouped_split<__bf16, Out>(what, p, s);
   const char *tag = "mxdense";
-  switch (tuning_override("UNIT_AMD_GROUPED_TRY")) {
-    case 4: return run_grouped_tile<OpMx, FORWARD, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
-  }
-  switch (grouped_tile_size(p, FORWARD)) {
+  switch (grouped_tile_size(p, FORWARD, true)) {
     case TILE_FEW: return run_grouped_tile<OpMx, FORWARD, Tile<32, 64, 128, 1, 2>, 2, Out>(what, tag, p, s);
     case TILE_SMALL: return run_grouped_tile<OpMx, FORWARD, Tile<64, 64, 128, 2, 2>, 3, Out>(what, tag, p, s);
     case TILE_MIDDLE: return run_grouped_tile<OpMx, FORWARD, Tile<128, 128, 128, 2, 2>, 2, Out>(what, tag, p, s);

@@ -437,7 +437,7 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
   }
 
   // Results, rounded once, here: each wave puts 32 rows of its columns in order in LDS of its own and writes them in runs of 16 bytes a lane.
-  // (Straight from the registers, 2 bytes a lane, the stores of a 256 x 256 tile of 16-bit results took 4 us.)
+  // (Straight from the registers, 2 bytes a lane: experts of 16384 x 1024 -> 2048 102.7 us, 96.2 like this.)
   constexpr int ES_OUT = (int)sizeof(Out), PITCH = T::TY * 32 * ES_OUT + 16, PER = 16 / ES_OUT, RUNS = T::TY * 32 / PER;  // elements per run, runs per row
   static_assert(NW * 32 * PITCH <= NSTAGE * STAGE, "the waves' rows fit the ring");
   __syncthreads();  // the ring is read out
@@ -467,6 +467,9 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
       const u32 at = ((u32)x * (u32)ys + (u32)y) * (u32)ES_OUT;
       if (whole) {
         store_result<kRowPolicy>(out, at, v);
+      } else if (y + PER <= ys) {  // rows begin on any element: the same 16 bytes, unaligned
+        typedef u32 v4un __attribute__((ext_vector_type(4), aligned(2)));
+        *reinterpret_cast<v4un *>(p.out + (out_row + x) * (long)ys * ES_OUT + (long)y * ES_OUT) = v;
       } else {
 #pragma unroll
         for (int e = 0; e < PER; ++e)
@@ -527,26 +530,32 @@ int run_grouped_tile(const char *what, const char *tag, const GroupedParams &p, 
   return UNIT_OK;
 }
 
-// Which tile.  xs, ys: rows of the first and second operand in a group, on average over the groups that can have any.
+// Which tile.  xs, ys: rows of the two operands of a group, the first one's on average over the groups that can have any; only the
+// device knows how many each has.  us, measured on both sides of each line (rows x K -> N over groups; * the one taken):
+//   FEW     32 rows, two to six workgroups a CU: up to 32 rows a group, and 64 tiles of 32 x 128
+//             fp16 16 x 1024 -> 2048 over 16:   FEW *8.2, SMALL 8.9     46 x 3592 -> 264 over 11:  FEW 21.4, SMALL *16.2
+//   SMALL   64 x 64, three workgroups a CU: fewer than 192 tiles of 128 x 128
+//             MXFP4 1911 x 3280 -> 600:         SMALL *15.2, MIDDLE 18.1  1277 x 1376 -> 2704 over 2: SMALL 14.5, MIDDLE *11.6
+//   MIDDLE  128 x 128, two a CU
+//   LARGE   256 x 256, one a CU: at least half of the CUs get one, 512 bytes of reduction and 2^32 products in all
+//             bf16 16384 x 1024 -> 2048 over 32: MIDDLE 103, LARGE *90    MXFP4 14826 x 384 -> 2176: MIDDLE *32.6, LARGE 39.5
+//             fp16 gradients 1000 x 520 -> 776 over 12: SMALL *17.6, MIDDLE 20.6, LARGE 36.4
+// Environment: UNIT_AMD_GROUPED_TILE=1..4 pins one.
 enum { TILE_FEW, TILE_SMALL, TILE_MIDDLE, TILE_LARGE };
-inline int grouped_tile_size(const GroupedParams &p, int dir) {
+inline int grouped_tile_size(const GroupedParams &p, int dir, bool mx) {
   if (const int pinned = tuning_override("UNIT_AMD_GROUPED_TILE")) return pinned - 1;
-  const long busy = p.groups < p.rows ? p.groups : (p.rows ? p.rows : 1);
-  const long xs = dir == GRAD_WEIGHT ? p.n : (p.rows + busy - 1) / busy, ys = dir == FORWARD ? p.n : p.k, groups = dir == GRAD_WEIGHT ? p.groups : busy;
+  const long rows = p.rows ? p.rows : 1, busy = p.groups < rows ? p.groups : rows, mean = (rows + busy - 1) / busy;
+  const long xs = dir == GRAD_WEIGHT ? p.n : mean, ys = dir == FORWARD ? p.n : p.k, groups = dir == GRAD_WEIGHT ? p.groups : busy;
+  const long k = dir == FORWARD ? p.k : dir == GRAD_DATA ? p.n : mean, kbytes = mx ? k / 2 : k * 2;
   const auto tiles = [&](int x, int y) { return (xs + x - 1) / x * ((ys + y - 1) / y) * groups; };
-  if (dir == FORWARD && xs <= 32) return TILE_FEW;
-  const long k = dir == FORWARD ? p.k : dir == GRAD_DATA ? p.n : p.rows / p.groups;
-  if (xs >= 192 && ys >= 192 && tiles(256, 256) >= 128 && xs * ys * groups >= (1l << 32) / (k + 1)) return TILE_LARGE;
-  return tiles(128, 128) >= 512 ? TILE_MIDDLE : TILE_SMALL;
+  if (dir == FORWARD && xs <= 32 && tiles(32, 128) >= 64) return TILE_FEW;
+  if (xs >= 192 && ys >= 192 && kbytes >= 512 && tiles(256, 256) >= 128 && xs * ys * groups >= (1l << 32) / k) return TILE_LARGE;
+  return tiles(128, 128) >= 192 ? TILE_MIDDLE : TILE_SMALL;
 }
 
 template <class Op, int DIR, class Out>
 int run_grouped_sizes(const char *what, const char *tag, const GroupedParams &p, hipStream_t s) {
-  switch (tuning_override("UNIT_AMD_GROUPED_TRY")) {
-    case 2: return run_grouped_tile<Op, DIR, Tile<256, 256, 64, 2, 4>, 4, Out>(what, tag, p, s);
-    case 4: return run_grouped_tile<Op, DIR, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
-  }
-  switch (grouped_tile_size(p, DIR)) {
+  switch (grouped_tile_size(p, DIR, Op::kMx)) {
     case TILE_FEW:
       if constexpr (DIR == FORWARD) return run_grouped_tile<Op, DIR, Tile<32, 128, 128, 1, 4>, 3, Out>(what, tag, p, s);
       [[fallthrough]];
