@@ -146,17 +146,30 @@ __device__ __forceinline__ GroupTileOf find_tile(const GroupedParams &p, int nts
   return t;
 }
 
-// rows of group g alone
-__device__ __forceinline__ void find_rows(const GroupedParams &p, int g, int lane, int &first, int &count) {
+// The rows of the group whose turn it is: the longest first where a wave holds them all, so that the last workgroups have little to do,
+// else as they come.
+__device__ __forceinline__ void find_rows(const GroupedParams &p, int turn, int lane, int &group, int &first, int &count) {
   u32 rows0 = 0, end = 0, start = 0;
-  for (int c = 0; c <= g / 64; ++c) {
+  const int last = p.groups <= 64 ? 0 : turn / 64;
+  for (int c = 0; c <= last; ++c) {
     if (c) rows0 = lane_value(end, 63);
     const int i = c * 64 + lane;
     end = min(rows0 + scan_upto(i < p.groups ? (u32)group_size(p, i) : 0, (u32)p.rows), (u32)p.rows);
     start = (u32)__builtin_amdgcn_update_dpp((int)rows0, (int)end, 0x138, 0xf, 0xf, false);
   }
-  first = (int)lane_value(start, g % 64);
-  count = (int)lane_value(end, g % 64) - first;
+  int l = turn % 64;
+  group = turn;
+  if (p.groups <= 64) {
+    const u32 size = end - start;
+    int before = 0;  // how many have their turn before this lane's group
+    for (int g = 0; g < p.groups; ++g) {
+      const u32 other = lane_value(size, g);
+      before += other > size || (other == size && g < lane);
+    }
+    group = l = __builtin_ctzll(__ballot(lane < p.groups && before == turn));
+  }
+  first = (int)lane_value(start, l);
+  count = (int)lane_value(end, l) - first;
 }
 
 // ------------------------------------------------------------------------------------------- the kernel
@@ -444,7 +457,9 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
   char *const rows = lds + wave * (32 * PITCH);
   const long out_row = (DIR == GRAD_WEIGHT ? (long)group * p.n : (long)first) + x0;
   const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(p.out + out_row * ys * (long)sizeof(Out), 0, -1, 0x00020000);
-  const bool whole = ys % PER == 0;
+  // Weight gradients in fp32 whose rows are whole lines go out with nt: as large as all operands together, they would push those out
+  // of the memory-side cache (119 -> 115 us for both gradients of 8192 rows; results of 16 bits lose, forward 90 -> 97).
+  const bool whole = ys % PER == 0, lines = ys % 32 == 0;
   typedef Out v4o __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int i = 0; i < T::TX; ++i) {
@@ -465,7 +480,9 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
       const v4u v = *reinterpret_cast<const v4u *>(rows + row * PITCH + c * ES_OUT);
       if (x >= high || y >= ys) continue;
       const u32 at = ((u32)x * (u32)ys + (u32)y) * (u32)ES_OUT;
-      if (whole) {
+      if (DIR == GRAD_WEIGHT && ES_OUT == 4 && lines) {
+        store_result<kResultPolicy>(out, at, v);
+      } else if (whole) {
         store_result<kRowPolicy>(out, at, v);
       } else if (y + PER <= ys) {  // rows begin on any element: the same 16 bytes, unaligned
         typedef u32 v4un __attribute__((ext_vector_type(4), aligned(2)));
@@ -489,11 +506,11 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63;
   if constexpr (DIR == GRAD_WEIGHT) {
-    const int b = (int)blockIdx.x, per = (int)gridDim.x / 8, rem = (int)gridDim.x % 8, xcd = b % 8;
-    const int logical = xcd * per + min(xcd, rem) + b / 8;
-    const int group = logical / (nts * xts), in = logical - group * (nts * xts), x0 = in % xts * T::BX;
-    int first, count;
-    find_rows(p, group, lane, first, count);
+    // Consecutive workgroups, which go to the eight XCDs in turn, share a group: each XCD has its part of the long ones and of the
+    // short ones (8192 rows over 16, 288 to 1220 each: 71 us with two groups an XCD, 64.5 like this).
+    const int turn = (int)blockIdx.x / (nts * xts), in = (int)blockIdx.x - turn * (nts * xts), x0 = in % xts * T::BX;
+    int group, first, count;
+    find_rows(p, turn, lane, group, first, count);
     compute_tile<Op, DIR, T, NSTAGE, Out>(p, lds, group, first, count, x0, min(p.n - x0, T::BX), in / xts * T::BY);
   } else {
     const GroupTileOf g = find_tile<T::BX, 4>(p, nts, (int)blockIdx.x, lane);
