@@ -197,6 +197,57 @@ def test_mxfp4_large_groups_and_nan(dev):
     near(got[keep], forward(xd, wd, sizes)[keep], forward(xd.abs(), wd.abs(), sizes)[keep], k, "float32")
 
 
+@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_every_tile_on_every_case(dev, case, tile, monkeypatch):
+    """The tile is a matter of speed: each of the four gives the right result whatever the sizes."""
+    monkeypatch.setenv("UNIT_AMD_GROUPED_TILE", str(tile))
+    sizes, spare, n, k = CASES[case]
+    x, w, dy, s = operands(sizes, spare, n, k, "bfloat16", dev)
+    xd, wd, dyd = x.double(), w.double(), dy.double()
+    near(U.grouped_dense(x, w, s), forward(xd, wd, sizes), forward(xd.abs(), wd.abs(), sizes), k, "float32")
+    got, want, size = U.grouped_dense_grad(x, w, dy, s), backward(xd, wd, dyd, sizes), backward(xd.abs(), wd.abs(), dyd.abs(), sizes)
+    near(got[0], want[0], size[0], n, "float32")
+    near(got[1], want[1], size[1], max(sizes), "float32")
+    q, wq = U.quantize_mxfp4(x), U.quantize_mxfp4(w)
+    xd, wd = U.dequantize_mxfp4(q).double(), U.dequantize_mxfp4(wq).double()
+    near(U.grouped_dense_mxfp4(q, wq, s), forward(xd, wd, sizes), forward(xd.abs(), wd.abs(), sizes), k, "float32")
+
+
+def test_rows_of_more_than_2_31_bytes(dev):
+    """2.2 GB of rows: the groups on either side of the 2^31-byte line, and the last rows; forward, both gradients."""
+    n, k, rows = 64, 4096, 270_000
+    g = torch.Generator(device=dev).manual_seed(2)
+    x = torch.randint(-2, 3, (rows, k), generator=g, device=dev, dtype=torch.int8).to(torch.bfloat16)
+    w = torch.randint(-2, 3, (3, n, k), generator=g, device=dev).to(torch.bfloat16)
+    dy = torch.randint(-2, 3, (rows, n), generator=g, device=dev).to(torch.bfloat16)
+    sizes = [262_100, 60, 7_800]  # the line is row 262144
+    s = torch.tensor(sizes, device=dev)
+    y, (dx, dw) = U.grouped_dense(x, w, s), U.grouped_dense_grad(x, w, dy, s, "bfloat16")
+    for e, r in ((0, slice(0, 64)), (0, slice(262_000, 262_100)), (1, slice(262_100, 262_160)), (2, slice(262_160, 262_400)), (2, slice(269_900, 269_960))):
+        assert torch.equal(y[r].double(), x[r].double() @ w[e].double().T)
+        assert torch.equal(dx[r].double(), (dy[r].double() @ w[e].double()).to(torch.bfloat16).double())
+    assert bool((y[269_960:] == 0).all()) and bool((dx[269_960:] == 0).all())
+    for e, r in ((1, slice(262_100, 262_160)), (2, slice(262_160, 269_960))):
+        assert torch.equal(dw[e].double(), dy[r].double().T @ x[r].double())
+
+
+def test_quantised_weights_of_more_than_2_31_bytes(dev):
+    """A stack of 2.3 GB of codes: the first and the last experts, as prepared and as multiplied."""
+    e, n, k = 70, 8192, 8192
+    g = torch.Generator(device=dev).manual_seed(3)
+    codes = torch.randint(0, 256, (e, n, k // 2), generator=g, device=dev, dtype=torch.uint8)
+    scales = torch.randint(120, 124, (e, n, k // 32), generator=g, device=dev, dtype=torch.uint8)
+    w = U.prepare_mxfp4_weight(codes, scales)
+    sizes = [2] + [0] * (e - 3) + [3, 40]
+    x = torch.randn((45, k), generator=g, device=dev).to(torch.bfloat16)
+    got = U.grouped_dense_mxfp4(x, w, torch.tensor(sizes, device=dev))
+    xd = U.dequantize_mxfp4(U.quantize_mxfp4(x)).double()
+    for i, r in ((0, slice(0, 2)), (e - 2, slice(2, 5)), (e - 1, slice(5, 45))):
+        wd = U.dequantize_mxfp4(U.prepare_mxfp4_weight(codes[i], scales[i])).double()
+        near(got[r], xd[r] @ wd.T, xd[r].abs() @ wd.abs().T, k, "float32")
+
+
 def test_no_rows(dev):
     w, s = randn((3, 16, 32), "float16", 1, dev), torch.zeros(3, dtype=torch.int32, device=dev)
     x, dy = torch.empty((0, 32), dtype=torch.float16, device=dev), torch.empty((0, 16), dtype=torch.float16, device=dev)
