@@ -94,21 +94,39 @@ __global__ __launch_bounds__(256) void dequantize_kernel(const u32 *codes, const
 }
 
 // codes (rows, 16 * blocks), scales (rows, blocks), blocks = K / 32 rounded up; whatever the last block holds behind K is dropped
-__global__ __launch_bounds__(256) void prepare_kernel(const unsigned char *codes_in, const unsigned char *scales_in, long rows, int K,
-                                                      u32 *codes, unsigned char *scales) {
-  const int per_row = mx_stages(K) * 32, blocks = (K + 31) / 32;
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  const long row = id / per_row;
-  const int lane = (int)(id % per_row), k0 = lane * 8, b = lane / 4;
-  if (row >= rows) return;
-  u32 c = 0;
-  if (k0 < K) {
-    const unsigned char *src = codes_in + row * (16l * blocks) + lane * 4;
-    c = src[0] | (u32)src[1] << 8 | (u32)src[2] << 16 | (u32)src[3] << 24;
-    if (K - k0 < 8) c &= (1u << 4 * (K - k0)) - 1;
+template <int ROUNDS>
+__global__ __launch_bounds__(256) void prepare_kernel(const unsigned char *codes_in, const unsigned char *scales_in, int rows, int K, u32 *codes, u32 *scales,
+                                                      FastDiv by_stages) {
+  constexpr int ROWS = 8 * ROUNDS;
+  typedef u32 u32_any __attribute__((aligned(1)));
+  const int t = threadIdx.x, l32 = t & 31, stages = by_stages.d, blocks = (K + 31) / 32;
+  int s, row0;
+  by_stages.divmod((int)blockIdx.x, row0, s);
+  row0 *= ROWS;
+  const int k0 = s * kMxStage + l32 * 8;
+  u32 c[ROUNDS];
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int row = min(row0 + i * 8 + (t >> 5), rows - 1);
+    c[i] = 0;
+    if (k0 < K) c[i] = *reinterpret_cast<const u32_any *>(codes_in + (size_t)row * (16 * blocks) + s * 128 + l32 * 4);
+    if (k0 < K && K - k0 < 8) c[i] &= (1u << 4 * (K - k0)) - 1;
   }
-  codes[row * per_row + lane] = c;
-  if (lane % 4 == 0) scales[((long)(b / 8 * 2 + b % 2) * rows + row) * 4 + b % 8 / 2] = b < blocks ? scales_in[row * blocks + b] : 0;
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int row = row0 + i * 8 + (t >> 5);
+    if (row < rows) codes[(size_t)row * (stages * 32) + s * 32 + l32] = c[i];
+  }
+  const int h = t / ROWS, row = row0 + t % ROWS;
+  if (h < 2 && row < rows) {
+    u32 e = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int b = s * 8 + 2 * j + h;
+      if (b < blocks) e |= (u32)scales_in[(size_t)row * blocks + b] << (8 * j);
+    }
+    scales[(size_t)(2 * s + h) * rows + row] = e;
+  }
 }
 
 int check_mx(const char *what, int64_t rows, int32_t K, std::initializer_list<const void *> ptrs) {
@@ -118,8 +136,6 @@ int check_mx(const char *what, int64_t rows, int32_t K, std::initializer_list<co
     if (!p && rows) return fail(UNIT_E_ARG, "%s: null pointer", what);
   return UNIT_OK;
 }
-
-unsigned mx_grid(int64_t rows, int32_t K) { return (unsigned)((rows * mx_stages(K) * 32 + 255) / 256); }
 
 // run(rounds, workgroups, divider): 64 rows a workgroup while that makes two workgroups per CU, else 8
 template <class F>
@@ -201,8 +217,10 @@ extern "C" int unit_prepare_mxfp4(const void *codes_in, const void *scales_in, i
   if (int rc = check_aligned(what, {codes, scales})) return rc;
   if (int rc = check_device()) return rc;
   if (!rows) return UNIT_OK;
-  hipLaunchKernelGGL(prepare_kernel, dim3(mx_grid(rows, K)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const unsigned char *>(codes_in),
-                     static_cast<const unsigned char *>(scales_in), (long)rows, K, static_cast<u32 *>(codes), static_cast<unsigned char *>(scales));
+  by_stage(rows, K, [&](auto rounds, dim3 grid, FastDiv by_stages) {
+    hipLaunchKernelGGL((prepare_kernel<decltype(rounds)::value>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const unsigned char *>(codes_in),
+                       static_cast<const unsigned char *>(scales_in), (int)rows, K, static_cast<u32 *>(codes), static_cast<u32 *>(scales), by_stages);
+  });
   set_variant("mxprepare");
   return launched(what);
 }
