@@ -123,7 +123,7 @@ def test_gradients_are_the_differences_of_the_forward(dev, dtype):
 def test_large_groups(dev):
     """Tiles of the largest size, ragged on every side, both directions; integer operands, so sums are exact."""
     g = torch.Generator(device=dev).manual_seed(9)
-    for sizes, n, k in (([1500, 0, 700, 1801], 1544, 776), ([4000], 2048, 1032), ([300] * 12 + [9], 2056, 520)):
+    for sizes, n, k in (([1500, 0, 700, 1801], 1544, 776), ([4000], 2048, 1032), ([300] * 12 + [9], 2056, 520), ([2100, 0, 1500, 1200, 900], 1544, 520)):
         rows = sum(sizes) + 5
         ints = lambda *shape: torch.randint(-2, 3, shape, generator=g, device=dev).to(torch.bfloat16)
         x, w, dy, s = ints(rows, k), ints(len(sizes), n, k), ints(rows, n), torch.tensor(sizes, device=dev)

@@ -196,7 +196,6 @@ __device__ __forceinline__ int cols_swz(int row) {
 template <class Op, int DIR, class T, int NSTAGE, class Out>
 __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, int group, int first, int count, int x0, int high, int y0) {
   constexpr bool MX = Op::kMx, XT = DIR == GRAD_WEIGHT, YT = DIR != FORWARD;
-  constexpr int ES = MX ? 0 : 2;                     // bytes per element of the 16-bit forms
   constexpr int KK = T::BKB / 32, CPR = T::CPR, NW = T::NT / 64, RPL = 64 / CPR;
   constexpr int KS = T::BKB / 2;                     // cols: reduction elements of a stage
   constexpr int XL = T::XBYTES / 1024 / NW, YL = T::YBYTES / 1024 / NW;
@@ -359,7 +358,7 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
   // NX: how many of its row blocks this wave has rows for; the others are left out.
   auto step = [&](auto nxc, auto kkc, const char *rd_stage, int rd_kk, const Source &src, int issue_kt, int slot, auto has_read, auto has_issue, auto last)
                   __attribute__((always_inline)) {
-    constexpr int s = decltype(kkc)::value & 1, NX = decltype(nxc)::value, NM = NX * T::TY, NF = NX ? NX + T::TY : 0;
+    constexpr int s = decltype(kkc)::value & 1, NX = decltype(nxc)::value, NM = NX * T::TY, NF = NX ? NX + T::TY : 0, PER = NM ? NM : 1;
     if constexpr (NX == 0 && decltype(has_issue)::value) {
 #pragma unroll
       for (int f = 0; f < LPS; ++f) issue_one(src, issue_kt, slot, f, last);
@@ -373,11 +372,11 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
         acc[i][j] = Op::mma(yf[s][j], xf[s][i], acc[i][j]);
       if constexpr (decltype(has_read)::value) {
 #pragma unroll
-        for (int f = m * NF / NM; f < (m + 1) * NF / NM; ++f) load_one(rd_stage, rd_kk, s ^ 1, f);
+        for (int f = m * NF / PER; f < (m + 1) * NF / PER; ++f) load_one(rd_stage, rd_kk, s ^ 1, f);
       }
       if constexpr (decltype(has_issue)::value) {
 #pragma unroll
-        for (int f = m * LPS / NM; f < (m + 1) * LPS / NM; ++f) issue_one(src, issue_kt, slot, f, last);
+        for (int f = m * LPS / PER; f < (m + 1) * LPS / PER; ++f) issue_one(src, issue_kt, slot, f, last);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -579,6 +578,13 @@ int run_grouped_sizes(const char *what, const char *tag, const GroupedParams &p,
     case TILE_SMALL: return run_grouped_tile<Op, DIR, Tile<64, 64, 128, 2, 2>, 3, Out>(what, tag, p, s);
     case TILE_MIDDLE: return run_grouped_tile<Op, DIR, Tile<128, 128, 64, 2, 2>, 4, Out>(what, tag, p, s);
     default:
+      if constexpr (DIR != GRAD_WEIGHT) {
+        // One round of 192-row tiles rather than most of one of 256: bf16 8192 x 2048 -> 1024 over 16, 57.0 us as about 170 tiles of 256
+        // rows, 52.3 as 210 of 192; 16384 x 1024 -> 2048 over 32, more than a round either way, 91 and 102.
+        const long busy = p.groups < p.rows ? p.groups : p.rows, nts = ceil_div(DIR == FORWARD ? p.n : p.k, 256);
+        if ((p.rows + busy * 96) / 192 * nts <= 256 && !tuning_override("UNIT_AMD_GROUPED_TILE"))
+          return run_grouped_tile<Op, DIR, Tile<192, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
+      }
       return run_grouped_tile<Op, DIR, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
   }
 }
