@@ -579,8 +579,9 @@ int run_grouped_sizes(const char *what, const char *tag, const GroupedParams &p,
     case TILE_MIDDLE: return run_grouped_tile<Op, DIR, Tile<128, 128, 64, 2, 2>, 4, Out>(what, tag, p, s);
     default:
       if constexpr (DIR != GRAD_WEIGHT) {
-        // One round of 192-row tiles rather than most of one of 256: bf16 8192 x 2048 -> 1024 over 16, 57.0 us as about 170 tiles of 256
-        // rows, 52.3 as 210 of 192; 16384 x 1024 -> 2048 over 32, more than a round either way, 91 and 102.
+        // One round of 192-row tiles rather than most of one of 256: bf16 8192 x 2048 -> 1024 over 16, 57.0 us as 160 tiles of 256 rows,
+        // 52.3 as 196 of 192; 16384 x 1024 -> 2048 over 32, more than a round either way, 101 and 111 (means of 30 calls under a profiler).
+        // Sizes stay on the device, so the rule takes half a tile to spare for each group.
         const long busy = p.groups < p.rows ? p.groups : p.rows, nts = ceil_div(DIR == FORWARD ? p.n : p.k, 256);
         if ((p.rows + busy * 96) / 192 * nts <= 256 && !tuning_override("UNIT_AMD_GROUPED_TILE"))
           return run_grouped_tile<Op, DIR, Tile<192, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
