@@ -137,6 +137,18 @@ def test_dense_matches_64_bit_sums(dev, m, n, k, dtype, out):
     assert torch.equal(got, U.dense_mxfp4(U.quantize_mxfp4(x), wq, out))  # quantised on the way or before: the same bits
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("m", [1, 16, 17, 130])
+def test_dense_of_unaligned_rows(dev, m, dtype):
+    """Contiguous rows that begin one element into their memory: the products of the same values, one row or several."""
+    k, n = 712, 200
+    x, w = data((m, k), dtype, m, dev), data((n, k), "float32", 7, dev)
+    wq = U.quantize_mxfp4(w)
+    off = torch.cat((x.new_zeros(1), x.view(-1)))[1:].view(m, k)
+    assert off.data_ptr() % 16 == x.element_size()
+    near(U.dense_mxfp4(off, wq, "float32"), decode(*encode(x)), decode(*encode(w)), "float32")
+
+
 def test_dense_large_tiles(dev):
     """Several hundred rows and columns of tiles, uneven on every side; the sums in 64 bits on the GPU."""
     for m, n, k in ((2100, 2300, 1100), (4096, 1024, 2048), (700, 6000, 288)):
