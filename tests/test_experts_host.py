@@ -1,0 +1,55 @@
+"""What the expert layer does around its products, on the CPU: the operators are replaced by plain products that, like the kernels,
+leave no trace for autograd."""
+import pytest
+import torch
+
+from unit_amd import experts as X
+
+
+def _groups(sizes):
+    at = 0
+    for g, n in enumerate(sizes.tolist()):
+        yield g, slice(at, at + n)
+        at += n
+
+
+@pytest.fixture
+def products(monkeypatch):
+    """grouped_dense and grouped_dense_grad as plain products; the names of those that ran"""
+    ran = []
+
+    def forward(x, w, sizes, out_dtype):
+        ran.append("forward")
+        x, w = x.detach(), w.detach()
+        y = x.new_zeros((x.shape[0], w.shape[1]))
+        for g, r in _groups(sizes):
+            y[r] = x[r] @ w[g].T
+        return y
+
+    def backward(x, w, dy, sizes, out_dtype, weight_out_dtype):
+        ran.append("both")
+        x, w, dy = x.detach(), w.detach(), dy.detach()
+        dx, dw = torch.zeros_like(x), torch.zeros_like(w)
+        for g, r in _groups(sizes):
+            dx[r], dw[g] = dy[r] @ w[g], dy[r].T @ x[r]
+        return dx, dw
+
+    monkeypatch.setattr(X, "grouped_dense", forward)
+    monkeypatch.setattr(X, "grouped_dense_grad", backward)
+    return ran
+
+
+def operands(rows=7, experts=3, n=8, k=16, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    sizes = torch.tensor([2, 0, rows - 2][:experts])
+    return torch.randn((rows, k), generator=g), torch.randn((experts, n, k), generator=g), sizes
+
+
+@pytest.mark.parametrize("loss", [lambda y: y.sum(), lambda y: y.square().sum()], ids=["linear", "square"])
+def test_a_gradient_that_is_to_be_differentiated_again_is_refused(products, loss):
+    x, w, sizes = operands()
+    x.requires_grad_(), w.requires_grad_()
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(loss(X.expert_linear(x, w, sizes)), x, create_graph=True)
+    loss(X.expert_linear(x, w, sizes)).backward()  # the first derivative is there
+    assert x.grad.shape == x.shape and w.grad.shape == w.shape

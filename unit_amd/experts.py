@@ -24,13 +24,15 @@ class _ExpertLinear(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
+        if torch.is_grad_enabled():  # the products below leave no trace: a derivative of these gradients would lack its part
+            raise RuntimeError("expert_linear: its gradients have no derivative of their own (create_graph=True)")
         x, weight, group_sizes = ctx.saved_tensors
         dx, dw = grouped_dense_grad(x, weight, grad, group_sizes, _NAME[x.dtype], _NAME[weight.dtype])
         return dx, dw, None
 
 
 def expert_linear(x, weight, group_sizes):
-    """grouped_dense in x's type, differentiable in x and weight."""
+    """grouped_dense in x's type, differentiable in x and weight, once: a backward pass with create_graph=True is refused."""
     return _ExpertLinear.apply(x, weight, group_sizes)
 
 
