@@ -53,3 +53,21 @@ def test_a_gradient_that_is_to_be_differentiated_again_is_refused(products, loss
         torch.autograd.grad(loss(X.expert_linear(x, w, sizes)), x, create_graph=True)
     loss(X.expert_linear(x, w, sizes)).backward()  # the first derivative is there
     assert x.grad.shape == x.shape and w.grad.shape == w.shape
+
+
+@pytest.fixture
+def quantized(monkeypatch):
+    """a layer with MXFP4 weights whose product is a constant"""
+    monkeypatch.setattr(X, "grouped_dense_mxfp4", lambda x, w, sizes, out: torch.full((x.shape[0], w.shape[1]), 0.5, dtype=x.dtype))
+    weight = lambda *shape: X.Mxfp4Tensor(torch.empty(0, dtype=torch.uint8), shape)
+    return X.ExpertLayer(weight(3, 24, 16), weight(3, 16, 24), 2)
+
+
+def test_mxfp4_layer_refuses_rows_that_want_a_gradient(quantized):
+    x, logits = torch.randn(5, 16, requires_grad=True), torch.randn(5, 3, requires_grad=True)
+    with pytest.raises(ValueError, match="x: .*gradient"):
+        quantized(x, logits)
+    with torch.no_grad():
+        assert quantized(x, logits).shape == (5, 16)
+    quantized(x.detach(), logits).square().sum().backward()  # the router's gradient is whole
+    assert logits.grad is not None

@@ -50,7 +50,8 @@ def route(logits, top_k):
 class ExpertLayer:
     """y[t] = sum over t's experts e of share * down[e] . silu(up[e] . x[t]).
 
-    up (E, hidden, model) and down (E, model, hidden): float16 or bfloat16 tensors of x's type, or Mxfp4Tensors."""
+    up (E, hidden, model) and down (E, model, hidden): float16 or bfloat16 tensors of x's type, or Mxfp4Tensors, for which
+    x has no gradient (an x that asks for one is refused) and the logits have theirs."""
 
     def __init__(self, up, down, top_k):
         if up.shape[0] != down.shape[0] or up.shape[1] != down.shape[2] or up.shape[2] != down.shape[1]:
@@ -68,6 +69,8 @@ class ExpertLayer:
     def __call__(self, x, logits):
         if tuple(logits.shape) != (x.shape[0], self.up.shape[0]):
             raise ValueError(f"logits: expected ({x.shape[0]}, {self.up.shape[0]}), got {tuple(logits.shape)}")
+        if isinstance(self.up, Mxfp4Tensor) and x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("x: requires a gradient, which a layer with MXFP4 weights has none of; detach it or use torch.no_grad()")
         order, token, sizes, share = route(logits, self.top_k)
         if isinstance(self.up, Mxfp4Tensor):
             product = lambda a, w: grouped_dense_mxfp4(a, w, sizes, _NAME[x.dtype])  # noqa: E731
