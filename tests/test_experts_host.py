@@ -71,3 +71,14 @@ def test_mxfp4_layer_refuses_rows_that_want_a_gradient(quantized):
         assert quantized(x, logits).shape == (5, 16)
     quantized(x.detach(), logits).square().sum().backward()  # the router's gradient is whole
     assert logits.grad is not None
+
+
+def test_no_tokens(products, quantized):
+    g = torch.Generator().manual_seed(2)
+    r = lambda *s: torch.randn(s, generator=g).requires_grad_()
+    up, down, x, logits = r(3, 24, 16), r(3, 16, 24), r(0, 16), r(0, 3)
+    y = X.ExpertLayer(up, down, 2)(x, logits)
+    assert y.shape == (0, 16)
+    y.sum().backward()
+    assert x.grad.shape == (0, 16) and logits.grad.shape == (0, 3) and not up.grad.any() and not down.grad.any()
+    assert quantized(x.detach(), logits.detach()).shape == (0, 16)

@@ -79,7 +79,7 @@ class ExpertLayer:
         y = product(torch.nn.functional.silu(product(x[token], self.up)), self.down)
         back = torch.empty_like(order).scatter_(0, order, torch.arange(len(order), device=order.device))
         # every token's pairs side by side again: added in one order, whatever runs beside it
-        y = y[back].view(x.shape[0], self.top_k, -1)
+        y = y[back].view(x.shape[0], self.top_k, self.down.shape[1])
         return (y.float() * share.unsqueeze(-1)).sum(1).to(x.dtype)
 
 
