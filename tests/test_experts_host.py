@@ -82,3 +82,19 @@ def test_no_tokens(products, quantized):
     y.sum().backward()
     assert x.grad.shape == (0, 16) and logits.grad.shape == (0, 3) and not up.grad.any() and not down.grad.any()
     assert quantized(x.detach(), logits.detach()).shape == (0, 16)
+
+
+def test_gradients_that_begin_anywhere_reach_the_products_aligned(products, monkeypatch):
+    """Joined with other values the result gets its gradient as a part of theirs, at any element."""
+    x, w, sizes = operands()
+    x.requires_grad_(), w.requires_grad_()
+    seen, plain = [], X.grouped_dense_grad
+    monkeypatch.setattr(X, "grouped_dense_grad", lambda x, w, dy, *rest: (seen.append((dy.data_ptr() % 16, dy.is_contiguous())), plain(x, w, dy, *rest))[1])
+    y = X.expert_linear(x, w, sizes)
+    head = torch.ones(1, requires_grad=True)
+    torch.cat((head, y.flatten())).square().sum().backward()
+    assert seen == [(0, True)]
+    got = x.grad, w.grad
+    x.grad = w.grad = None
+    X.expert_linear(x, w, sizes).square().sum().backward()
+    assert torch.equal(got[0], x.grad) and torch.equal(got[1], w.grad)

@@ -1,8 +1,8 @@
-"""The expert layer on the GPU where it has little to do: no tokens."""
+"""The expert layer on the GPU at its edges: no tokens, gradients that begin on any element."""
 import pytest
 import torch
 
-from unit_amd.experts import ExpertLayer
+from unit_amd.experts import ExpertLayer, expert_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +23,16 @@ def test_no_tokens(dev, dtype):
     assert x.grad.shape == (0, 64) and not bool(up.grad.any()) and not bool(down.grad.any())
     with torch.no_grad():
         assert ExpertLayer(up, down, 2).quantized()(x, logits).shape == (0, 64)
+
+
+def test_gradients_that_begin_anywhere(dev):
+    x, _, up, _ = (t.requires_grad_() for t in make(40, 3, 64, 48, torch.bfloat16, dev))
+    sizes = torch.tensor([10, 0, 30], device=dev)
+    expert_linear(x, up, sizes).float().square().sum().backward()
+    want = x.grad, up.grad
+    x.grad = up.grad = None
+    head = torch.ones(1, device=dev, dtype=torch.bfloat16, requires_grad=True)
+    y = expert_linear(x, up, sizes)
+    parts = torch.cat((head, y.flatten()))
+    parts.backward(torch.cat((head.detach(), (2 * y.detach().float()).to(y.dtype).flatten())))
+    assert torch.equal(x.grad, want[0]) and torch.equal(up.grad, want[1])

@@ -27,6 +27,9 @@ class _ExpertLinear(torch.autograd.Function):
         if torch.is_grad_enabled():  # the products below leave no trace: a derivative of these gradients would lack its part
             raise RuntimeError("expert_linear: its gradients have no derivative of their own (create_graph=True)")
         x, weight, group_sizes = ctx.saved_tensors
+        grad = grad.contiguous()
+        if grad.data_ptr() % 16:  # a part of a larger gradient (torch.cat's, say): the kernels read 16 bytes at a time
+            grad = grad.clone()
         dx, dw = grouped_dense_grad(x, weight, grad, group_sizes, _NAME[x.dtype], _NAME[weight.dtype])
         return dx, dw, None
 
