@@ -98,3 +98,26 @@ def test_gradients_that_begin_anywhere_reach_the_products_aligned(products, monk
     x.grad = w.grad = None
     X.expert_linear(x, w, sizes).square().sum().backward()
     assert torch.equal(got[0], x.grad) and torch.equal(got[1], w.grad)
+
+
+@pytest.mark.parametrize("trained", ["x", "w"])
+def test_frozen_operands_have_no_gradient_computed(products, monkeypatch, trained):
+    x, w, sizes = operands()
+    x.requires_grad_(), w.requires_grad_()
+    X.expert_linear(x, w, sizes).square().sum().backward()
+    assert products == ["forward", "both"]
+    want = {"x": x.grad, "w": w.grad}[trained]
+    (w if trained == "x" else x).requires_grad_(False)
+    x.grad = w.grad = None
+
+    def one(data, weight, grad, group_sizes, out_dtype, weight_out_dtype, wanted):
+        products.append(wanted)
+        both = plain(data, weight, grad, group_sizes, out_dtype, weight_out_dtype)
+        return both[0] if wanted[0] else None, both[1] if wanted[1] else None
+
+    plain = X.grouped_dense_grad
+    monkeypatch.setattr(X, "_grouped_grad", one)
+    monkeypatch.setattr(X, "grouped_dense_grad", lambda *args: pytest.fail("both gradients were computed"))
+    X.expert_linear(x, w, sizes).square().sum().backward()
+    assert (trained == "x", trained == "w") in products
+    assert torch.equal({"x": x.grad, "w": w.grad}[trained], want)

@@ -1,7 +1,8 @@
-"""The expert layer on the GPU at its edges: no tokens, gradients that begin on any element."""
+"""The expert layer on the GPU at its edges: no tokens, gradients that begin on any element, frozen operands."""
 import pytest
 import torch
 
+import unit_amd as U
 from unit_amd.experts import ExpertLayer, expert_linear
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +37,26 @@ def test_gradients_that_begin_anywhere(dev):
     parts = torch.cat((head, y.flatten()))
     parts.backward(torch.cat((head.detach(), (2 * y.detach().float()).to(y.dtype).flatten())))
     assert torch.equal(x.grad, want[0]) and torch.equal(up.grad, want[1])
+
+
+def test_frozen_operands(dev):
+    """The same gradient with the other operand frozen, from its kernel alone and without the other's memory."""
+    x, _, up, _ = (t.requires_grad_() for t in make(40, 64, 256, 512, torch.float16, dev))
+    sizes = torch.zeros(64, dtype=torch.int64, device=dev)
+    sizes[3], sizes[50] = 10, 30
+    expert_linear(x, up, sizes).float().sum().backward()
+    want = x.grad, up.grad
+    for trained, frozen, i, kernel in ((x, up, 0, "groupeddx"), (up, x, 1, "groupeddw")):
+        frozen.requires_grad_(False)
+        x.grad = up.grad = None
+        y = expert_linear(x, up, sizes).float().sum()
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        y.backward()
+        torch.cuda.synchronize()
+        assert kernel in U.last_variant()
+        assert torch.equal(trained.grad, want[i]) and frozen.grad is None
+        if i == 0:  # 16 MiB of weight gradients are not allocated
+            assert torch.cuda.max_memory_allocated() - before < 4 << 20
+        frozen.requires_grad_()

@@ -9,7 +9,7 @@ import time
 
 import torch
 
-from .grouped import Mxfp4Tensor, grouped_dense, grouped_dense_grad, grouped_dense_mxfp4, quantize_mxfp4
+from .grouped import Mxfp4Tensor, _grouped_grad, grouped_dense, grouped_dense_grad, grouped_dense_mxfp4, quantize_mxfp4
 
 __all__ = ["ExpertLayer", "expert_linear", "route"]
 
@@ -30,8 +30,9 @@ class _ExpertLinear(torch.autograd.Function):
         grad = grad.contiguous()
         if grad.data_ptr() % 16:  # a part of a larger gradient (torch.cat's, say): the kernels read 16 bytes at a time
             grad = grad.clone()
-        dx, dw = grouped_dense_grad(x, weight, grad, group_sizes, _NAME[x.dtype], _NAME[weight.dtype])
-        return dx, dw, None
+        wanted = ctx.needs_input_grad[:2]  # a frozen operand's gradient is not computed
+        args = x, weight, grad, group_sizes, _NAME[x.dtype], _NAME[weight.dtype]
+        return *(grouped_dense_grad(*args) if all(wanted) else _grouped_grad(*args, wanted)), None
 
 
 def expert_linear(x, weight, group_sizes):

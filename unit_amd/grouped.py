@@ -249,6 +249,11 @@ def grouped_dense_grad(data, weight, grad, group_sizes, out_dtype="float32", wei
     both = _native.grouped_grad(data, weight, grad, group_sizes, out_dtype, weight_out_dtype)
     if both is not None:
         return both
+    return _grouped_grad(data, weight, grad, group_sizes, out_dtype, weight_out_dtype)
+
+
+def _grouped_grad(data, weight, grad, group_sizes, out_dtype, weight_out_dtype, wanted=(True, True)):
+    """(ddata, dweight), None in the place of one that is not wanted: it costs neither time nor memory"""
     dt, wdt = _out_dtype(out_dtype), _out_dtype(weight_out_dtype, "weight_out_dtype")
     data, weight, sizes, e, n, k = _grouped(data, weight, group_sizes)
     grad = _dev(grad, "grad", data.dtype, 2)
@@ -256,11 +261,14 @@ def grouped_dense_grad(data, weight, grad, group_sizes, out_dtype="float32", wei
     rows = data.shape[0]
     if tuple(grad.shape) != (rows, n):
         raise ValueError(f"grad: expected ({rows}, {n}), got {tuple(grad.shape)}")
-    ddata = torch.empty((rows, k), dtype=dt, device=data.device)
-    dweight = torch.empty((e, n, k), dtype=wdt, device=data.device)
     L, tail = _lib.load(), (rows, e, n, k, _stream())
-    check(L.unit_grouped_dense_grad_data(grad.data_ptr(), weight.data_ptr(), sizes.data_ptr(), sizes.element_size(), ddata.data_ptr(),
-                                         _CODE[data.dtype], _CODE[dt], *tail))
-    check(L.unit_grouped_dense_grad_weight(data.data_ptr(), grad.data_ptr(), sizes.data_ptr(), sizes.element_size(), dweight.data_ptr(),
-                                           _CODE[data.dtype], _CODE[wdt], *tail))
+    ddata = dweight = None
+    if wanted[0]:
+        ddata = torch.empty((rows, k), dtype=dt, device=data.device)
+        check(L.unit_grouped_dense_grad_data(grad.data_ptr(), weight.data_ptr(), sizes.data_ptr(), sizes.element_size(), ddata.data_ptr(),
+                                             _CODE[data.dtype], _CODE[dt], *tail))
+    if wanted[1]:
+        dweight = torch.empty((e, n, k), dtype=wdt, device=data.device)
+        check(L.unit_grouped_dense_grad_weight(data.data_ptr(), grad.data_ptr(), sizes.data_ptr(), sizes.element_size(), dweight.data_ptr(),
+                                               _CODE[data.dtype], _CODE[wdt], *tail))
     return ddata, dweight
