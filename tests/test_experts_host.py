@@ -121,3 +121,16 @@ def test_frozen_operands_have_no_gradient_computed(products, monkeypatch, traine
     X.expert_linear(x, w, sizes).square().sum().backward()
     assert (trained == "x", trained == "w") in products
     assert torch.equal({"x": x.grad, "w": w.grad}[trained], want)
+
+
+def test_arguments_are_refused_by_name(quantized):
+    x, w, sizes = operands()
+    with pytest.raises(TypeError, match="x: expected dtype .*float64"):
+        X.expert_linear(x.double(), w.double(), sizes)
+    with pytest.raises(TypeError, match="x: expected dtype .*int32"):
+        quantized(torch.zeros((5, 16), dtype=torch.int32), torch.zeros((5, 3)))
+    for up, down in ((torch.zeros(24, 16), torch.zeros(16, 24)), (torch.zeros(3, 24, 16), torch.zeros(3, 16))):
+        with pytest.raises(ValueError, match=r"expected \(E, hidden, model\)"):
+            X.ExpertLayer(up, down, 1)
+    with pytest.raises(ValueError, match="x: expected two axes"):
+        quantized(torch.zeros((5, 2, 16)), torch.zeros((5, 3)))

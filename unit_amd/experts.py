@@ -16,11 +16,18 @@ __all__ = ["ExpertLayer", "expert_linear", "route"]
 _NAME = {torch.float32: "float32", torch.float16: "float16", torch.bfloat16: "bfloat16"}
 
 
+def _name(x):
+    try:
+        return _NAME[x.dtype]
+    except KeyError:
+        raise TypeError(f"x: expected dtype {' or '.join(str(d) for d in _NAME)}, got {x.dtype}") from None
+
+
 class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, group_sizes):
         ctx.save_for_backward(x, weight, group_sizes)
-        return grouped_dense(x, weight, group_sizes, _NAME[x.dtype])
+        return grouped_dense(x, weight, group_sizes, _name(x))
 
     @staticmethod
     def backward(ctx, grad):
@@ -58,7 +65,7 @@ class ExpertLayer:
     x has no gradient (an x that asks for one is refused) and the logits have theirs."""
 
     def __init__(self, up, down, top_k):
-        if up.shape[0] != down.shape[0] or up.shape[1] != down.shape[2] or up.shape[2] != down.shape[1]:
+        if not len(up.shape) == len(down.shape) == 3 or up.shape[0] != down.shape[0] or up.shape[1] != down.shape[2] or up.shape[2] != down.shape[1]:
             raise ValueError(f"up {tuple(up.shape)}, down {tuple(down.shape)}: expected (E, hidden, model) and (E, model, hidden)")
         if isinstance(up, Mxfp4Tensor) != isinstance(down, Mxfp4Tensor):
             raise TypeError("up, down: both or neither in MXFP4")
@@ -71,13 +78,16 @@ class ExpertLayer:
         return ExpertLayer(quantize_mxfp4(self.up.detach()), quantize_mxfp4(self.down.detach()), self.top_k)
 
     def __call__(self, x, logits):
+        name = _name(x)
+        if x.dim() != 2:
+            raise ValueError(f"x: expected two axes, got shape {tuple(x.shape)}")
         if tuple(logits.shape) != (x.shape[0], self.up.shape[0]):
             raise ValueError(f"logits: expected ({x.shape[0]}, {self.up.shape[0]}), got {tuple(logits.shape)}")
         if isinstance(self.up, Mxfp4Tensor) and x.requires_grad and torch.is_grad_enabled():
             raise ValueError("x: requires a gradient, which a layer with MXFP4 weights has none of; detach it or use torch.no_grad()")
         order, token, sizes, share = route(logits, self.top_k)
         if isinstance(self.up, Mxfp4Tensor):
-            product = lambda a, w: grouped_dense_mxfp4(a, w, sizes, _NAME[x.dtype])  # noqa: E731
+            product = lambda a, w: grouped_dense_mxfp4(a, w, sizes, name)  # noqa: E731
         else:
             product = lambda a, w: expert_linear(a, w, sizes)  # noqa: E731
         y = product(torch.nn.functional.silu(product(x[token], self.up)), self.down)
