@@ -53,9 +53,12 @@ def test_frozen_operands(dev):
         torch.cuda.synchronize()
         torch.cuda.reset_peak_memory_stats()
         before = torch.cuda.memory_allocated()
+        ran = []
+        hook = trained.register_hook(lambda g: ran.append(U.last_variant()))  # on autograd's thread, like the calls
         y.backward()
         torch.cuda.synchronize()
-        assert kernel in U.last_variant()
+        hook.remove()
+        assert len(ran) == 1 and kernel in ran[0]
         assert torch.equal(trained.grad, want[i]) and frozen.grad is None
         if i == 0:  # 16 MiB of weight gradients are not allocated
             assert torch.cuda.max_memory_allocated() - before < 4 << 20
