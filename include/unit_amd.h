@@ -366,7 +366,8 @@ int unit_dense_mxfp4(const void *x, const void *xscales, int32_t x_dtype, const 
 /* ------------------------------------------------------------------ products grouped by expert
  * Rows sorted by group: sizes[0] rows of group 0, then sizes[1] of group 1, ...; sizes are `groups` int32 or int64 (size_bytes
  * 4 or 8) in device memory, read when the work runs.  A size counts as min(max(size, 0), rows left); rows behind the last
- * group's belong to none and give zeros.  Row operands may pass 2^31 bytes, a group's weight may not.  rows may be 0.
+ * group's belong to none and give zeros.  Row operands and results, a group's fp32 weight gradient among
+ * them, may pass 2^31 bytes; a group's weight may not.  rows may be 0.
  * 16-bit operands: N and K multiples of 8, pointers 16-byte aligned; sums in fp32, rounded once to out_dtype.
  *
  * forward: out (rows, N), out[r] = w[g(r)] x[r], w (groups, N, K) */

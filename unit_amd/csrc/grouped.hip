@@ -20,7 +20,8 @@ int check_groups(const char *what, const void *sizes, int size_bytes, int rows, 
   if (size_bytes != 4 && size_bytes != 8) return fail(UNIT_E_ARG, "%s: group sizes are 4- or 8-byte integers, got %d bytes", what, size_bytes);
   if (!sizes) return fail(UNIT_E_ARG, "%s: null pointer", what);
   if ((uintptr_t)sizes % size_bytes) return fail(UNIT_E_ARG, "%s: group sizes are not aligned to their type", what);
-  // 32-bit offsets inside one group's weight and inside one tile; the tensors themselves may be larger
+  // 32-bit offsets inside one group's weight and inside one tile (a tile of a weight's gradient in fp32 stays below 2^32 bytes with
+  // the 16-bit weight below 2^31); the tensors themselves may be larger
   if (!fits(w_bytes)) return fail(UNIT_E_ARG, "%s: a group's weight exceeds 2^31-1 bytes", what);
   if (rows > 1 << 30 || groups > 1 << 20 || n > 1 << 22 || k > 1 << 22) return fail(UNIT_E_ARG, "%s: sizes beyond 2^30 rows, 2^20 groups or 2^22 columns", what);
   return UNIT_OK;
@@ -72,7 +73,7 @@ extern "C" int unit_grouped_dense_grad_weight(const void *x, const void *dy, con
                                               int32_t rows, int32_t groups, int32_t N, int32_t K, unit_stream_t stream) {
   const char *what = "unit_grouped_dense_grad_weight";
   if (int rc = check_types(what, dtype, out_dtype)) return rc;
-  if (int rc = check_groups(what, sizes, size_bytes, rows, groups, N, K, (size_t)N * K * 4)) return rc;
+  if (int rc = check_groups(what, sizes, size_bytes, rows, groups, N, K, (size_t)N * K * 2)) return rc;
   if (int rc = check_f16(what, N, K)) return rc;
   if (int rc = check_ptrs(what, rows, {x, dy})) return rc;
   if (int rc = check_ptrs(what, true, {dw})) return rc;
