@@ -556,8 +556,12 @@ int run_grouped_tile(const char *what, const char *tag, const GroupedParams &p, 
 //   LARGE   256 x 256, one a CU: at least half of the CUs get one, 512 bytes of reduction and 2^32 products in all
 //             bf16 16384 x 1024 -> 2048 over 32: MIDDLE 103, LARGE *90    MXFP4 14826 x 384 -> 2176: MIDDLE *32.6, LARGE 39.5
 //             fp16 gradients 1000 x 520 -> 776 over 12: SMALL *17.6, MIDDLE 20.6, LARGE 36.4
-// Environment: UNIT_AMD_GROUPED_TILE=1..4 pins one.
-enum { TILE_FEW, TILE_SMALL, TILE_MIDDLE, TILE_LARGE };
+//   ROUND   192 x 256, one a CU, 16-bit forward products and data gradients: one round of them rather than most of one of 256.  Sizes
+//           stay on the device, so the rule takes half a tile to spare for each group.
+//             bf16 data gradient 8192 x 2048 -> 1024 over 16: LARGE 57.0 (160 tiles), ROUND *52.3 (196)
+//             bf16 16384 x 1024 -> 2048 over 32, more than a round either way: LARGE *101, ROUND 111 (means of 30 calls under a profiler)
+// Environment: UNIT_AMD_GROUPED_TILE=1..5 pins one (5 where there is no ROUND: LARGE).
+enum { TILE_FEW, TILE_SMALL, TILE_MIDDLE, TILE_LARGE, TILE_ROUND };
 inline int grouped_tile_size(const GroupedParams &p, int dir, bool mx) {
   if (const int pinned = tuning_override("UNIT_AMD_GROUPED_TILE")) return pinned - 1;
   const long rows = p.rows ? p.rows : 1, busy = p.groups < rows ? p.groups : rows, mean = (rows + busy - 1) / busy;
@@ -565,7 +569,10 @@ inline int grouped_tile_size(const GroupedParams &p, int dir, bool mx) {
   const long k = dir == FORWARD ? p.k : dir == GRAD_DATA ? p.n : mean, kbytes = mx ? k / 2 : k * 2;
   const auto tiles = [&](int x, int y) { return (xs + x - 1) / x * ((ys + y - 1) / y) * groups; };
   if (dir == FORWARD && xs <= 32 && tiles(32, 128) >= 64) return TILE_FEW;
-  if (xs >= 192 && ys >= 192 && kbytes >= 512 && tiles(256, 256) >= 128 && xs * ys * groups >= (1l << 32) / k) return TILE_LARGE;
+  if (xs >= 192 && ys >= 192 && kbytes >= 512 && tiles(256, 256) >= 128 && xs * ys * groups >= (1l << 32) / k) {
+    const bool round = !mx && dir != GRAD_WEIGHT && (p.rows + busy * 96) / 192 * ((ys + 255) / 256) <= 256;
+    return round ? TILE_ROUND : TILE_LARGE;
+  }
   return tiles(128, 128) >= 192 ? TILE_MIDDLE : TILE_SMALL;
 }
 
@@ -577,16 +584,10 @@ int run_grouped_sizes(const char *what, const char *tag, const GroupedParams &p,
       [[fallthrough]];
     case TILE_SMALL: return run_grouped_tile<Op, DIR, Tile<64, 64, 128, 2, 2>, 3, Out>(what, tag, p, s);
     case TILE_MIDDLE: return run_grouped_tile<Op, DIR, Tile<128, 128, 64, 2, 2>, 4, Out>(what, tag, p, s);
-    default:
-      if constexpr (DIR != GRAD_WEIGHT) {
-        // One round of 192-row tiles rather than most of one of 256: bf16 8192 x 2048 -> 1024 over 16, 57.0 us as 160 tiles of 256 rows,
-        // 52.3 as 196 of 192; 16384 x 1024 -> 2048 over 32, more than a round either way, 101 and 111 (means of 30 calls under a profiler).
-        // Sizes stay on the device, so the rule takes half a tile to spare for each group.
-        const long busy = p.groups < p.rows ? p.groups : p.rows, nts = ceil_div(DIR == FORWARD ? p.n : p.k, 256);
-        if ((p.rows + busy * 96) / 192 * nts <= 256 && !tuning_override("UNIT_AMD_GROUPED_TILE"))
-          return run_grouped_tile<Op, DIR, Tile<192, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
-      }
-      return run_grouped_tile<Op, DIR, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
+    case TILE_ROUND:
+      if constexpr (DIR != GRAD_WEIGHT) return run_grouped_tile<Op, DIR, Tile<192, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
+      [[fallthrough]];
+    default: return run_grouped_tile<Op, DIR, Tile<256, 256, 128, 2, 4>, 2, Out>(what, tag, p, s);
   }
 }
 
