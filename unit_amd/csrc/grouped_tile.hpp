@@ -556,10 +556,12 @@ int run_grouped_tile(const char *what, const char *tag, const GroupedParams &p, 
 //   LARGE   256 x 256, one a CU: at least half of the CUs get one, 512 bytes of reduction and 2^32 products in all
 //             bf16 16384 x 1024 -> 2048 over 32: MIDDLE 103, LARGE *90    MXFP4 14826 x 384 -> 2176: MIDDLE *32.6, LARGE 39.5
 //             fp16 gradients 1000 x 520 -> 776 over 12: SMALL *17.6, MIDDLE 20.6, LARGE 36.4
-//   ROUND   192 x 256, one a CU, 16-bit forward products and data gradients: one round of them rather than most of one of 256.  Sizes
-//           stay on the device, so the rule takes half a tile to spare for each group.
-//             bf16 data gradient 8192 x 2048 -> 1024 over 16: LARGE 57.0 (160 tiles), ROUND *52.3 (196)
-//             bf16 16384 x 1024 -> 2048 over 32, more than a round either way: LARGE *101, ROUND 111 (means of 30 calls under a profiler)
+//   ROUND   192 x 256, one a CU, 16-bit forward products and data gradients: one round of them rather than most of one of 256.  Only
+//           where it is one round however the rows fall on the groups (each may end one row into a tile): a second one costs more
+//           than the first gains.
+//             bf16 8192 x 2048 -> 1024 over 16 of 512 (192 tiles, 128 of LARGE): forward LARGE 54.3, ROUND *48.1; data gradient 53.2, *46.9
+//             bf16 5184 x 1024 -> 2304 (243, 189): forward LARGE 26.5, ROUND *24.7; data gradient 26.7, *24.7
+//             bf16 4835 x 3848 -> 2400 (260, 190): forward LARGE *93, ROUND 174     6240 x 1032 -> 1536 over 16 of 390 (288, 192): *27.7, 43.7
 // Environment: UNIT_AMD_GROUPED_TILE=1..5 pins one (5 where there is no ROUND: LARGE).
 enum { TILE_FEW, TILE_SMALL, TILE_MIDDLE, TILE_LARGE, TILE_ROUND };
 inline int grouped_tile_size(const GroupedParams &p, int dir, bool mx) {
@@ -570,7 +572,7 @@ inline int grouped_tile_size(const GroupedParams &p, int dir, bool mx) {
   const auto tiles = [&](int x, int y) { return (xs + x - 1) / x * ((ys + y - 1) / y) * groups; };
   if (dir == FORWARD && xs <= 32 && tiles(32, 128) >= 64) return TILE_FEW;
   if (xs >= 192 && ys >= 192 && kbytes >= 512 && tiles(256, 256) >= 128 && xs * ys * groups >= (1l << 32) / k) {
-    const bool round = !mx && dir != GRAD_WEIGHT && (p.rows + busy * 96) / 192 * ((ys + 255) / 256) <= 256;
+    const bool round = !mx && dir != GRAD_WEIGHT && (p.rows + busy * 191) / 192 * ((ys + 255) / 256) <= 256;
     return round ? TILE_ROUND : TILE_LARGE;
   }
   return tiles(128, 128) >= 192 ? TILE_MIDDLE : TILE_SMALL;
