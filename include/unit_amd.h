@@ -340,7 +340,7 @@ int unit_conv_chain_u8_status(const unit_chain_layer *layers, int32_t count, con
  * kb = K / 256 rounded up, the even element of a pair in the low half of its byte, zeros behind K; the scale of block b of a row
  * lies at [b / 8][b % 2][row][(b % 8) / 2] of [kb][2][rows][4]: a lane's four scales of a 128-byte stage are one dword.
  * 1 KiB more follows, which the products read (and use nothing of) at the end of the last tile. */
-enum { UNIT_F32 = 0, UNIT_F16 = 1, UNIT_BF16 = 2, UNIT_MXFP4 = 3 };
+enum { UNIT_F32 = 0, UNIT_F16 = 1, UNIT_BF16 = 2, UNIT_MXFP4 = 3, UNIT_MXFP8 = 4 };
 
 int unit_mxfp4_bytes(int64_t rows, int32_t K, size_t *codes, size_t *scales);
 
@@ -365,7 +365,7 @@ int unit_dense_mxfp4(const void *x, const void *xscales, int32_t x_dtype, const 
 
 /* ------------------------------------------------------------------ products grouped by expert
  * Rows sorted by group: sizes[0] rows of group 0, then sizes[1] of group 1, ...; sizes are `groups` int32 or int64 (size_bytes
- * 4 or 8) in device memory, read when the work runs.  A size counts as min(max(size, 0), rows left); rows behind the last
+ * 4 or 8) in device memory, read when the work runs; NULL where there is one group, of all rows.  A size counts as min(max(size, 0), rows left); rows behind the last
  * group's belong to none and give zeros.  Row operands and results, a group's fp32 weight gradient among
  * them, may pass 2^31 bytes; a group's weight may not.  rows may be 0.
  * 16-bit operands: N and K multiples of 8, pointers 16-byte aligned; sums in fp32, rounded once to out_dtype.
@@ -383,6 +383,40 @@ int unit_grouped_dense_grad_weight(const void *x, const void *dy, const void *si
 int unit_grouped_dense_mxfp4(const void *x, const void *xscales, int32_t x_dtype, const void *wcodes, const void *wscales,
                              const void *sizes, int32_t size_bytes, void *out, int32_t out_dtype, int32_t rows, int32_t groups,
                              int32_t N, int32_t K, void *ws, size_t ws_bytes, unit_stream_t stream);
+
+/* ------------------------------------------------------------------ gated feed-forward products
+ * h[r] = act(gate x[r]) * (up x[r]): a group's weight (2 N, K) holds gate's N rows, then up's; groups and sizes as above.  The
+ * activation and the product are of the sums in fp32, h is rounded once.  UNIT_SILU: z / (1 + exp(-z)).  UNIT_GELU_TANH:
+ * z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2.
+ *
+ * pre: NULL, or where gate x and up x are kept for the gradients, (rows, 2, N): in the operands' type (pre_dtype), or in MXFP8
+ * (UNIT_MXFP8; buffers of 2 * rows rows of N elements), rounded once from the same sums.  Zeros for rows of no group, as in out. */
+enum { UNIT_SILU = 0, UNIT_GELU_TANH = 1 };
+int unit_gated_dense(const void *x, const void *w, const void *sizes, int32_t size_bytes, void *out, int32_t dtype,
+                     int32_t out_dtype, int32_t activation, void *pre, void *pre_scales, int32_t pre_dtype, int32_t rows,
+                     int32_t groups, int32_t N, int32_t K, unit_stream_t stream);
+/* the same on MXFP4 operands, x and workspace as in unit_dense_mxfp4; wcodes, wscales of groups * 2 N rows; any N and K */
+int unit_gated_dense_mxfp4(const void *x, const void *xscales, int32_t x_dtype, const void *wcodes, const void *wscales,
+                           const void *sizes, int32_t size_bytes, void *out, int32_t out_dtype, int32_t activation, int32_t rows,
+                           int32_t groups, int32_t N, int32_t K, void *ws, size_t ws_bytes, unit_stream_t stream);
+/* the gradients of the gate for dh (rows, N): dpre (rows, 2, N), dpre[r][0] = dh u act'(g), dpre[r][1] = dh act(g) for kept
+ * g = pre[r][0], u = pre[r][1], computed in fp32 and rounded once to dtype.  unit_grouped_dense_grad_data and
+ * unit_grouped_dense_grad_weight take dpre from there, with 2 N for N. */
+int unit_gate_grad(const void *pre, const void *pre_scales, int32_t pre_dtype, const void *dh, void *dpre, int32_t dtype,
+                   int32_t activation, int32_t rows, int32_t N, unit_stream_t stream);
+
+/* ------------------------------------------------------------------ MXFP8
+ * Rows of 8-bit floats (e4m3: sign, four exponent bits, three mantissa bits, up to 448), 32 consecutive elements of a row sharing
+ * a scale 2^(s - 127), s one byte, 255 for a block that is NaN throughout: activations that wait for a backward pass.
+ * codes: rows of 32 * b bytes, b = K / 32 rounded up, zeros behind K, 16-byte aligned; scales: (rows, b) bytes. */
+int unit_mxfp8_bytes(int64_t rows, int32_t K, size_t *codes, size_t *scales);
+/* x (rows, K), contiguous, aligned to its elements.  A block's scale is the smallest power of two, at least 2^-127, for which its
+ * largest magnitude is at most 448; elements are x / scale rounded to the nearest element, ties to the even mantissa.  A block
+ * with an infinity or a NaN takes scale 255. */
+int unit_quantize_mxfp8(const void *x, int32_t dtype, int64_t rows, int32_t K, void *codes, void *scales, unit_stream_t stream);
+/* The values that codes and scales stand for, (rows, K), rounded once where dtype does not hold them. */
+int unit_dequantize_mxfp8(const void *codes, const void *scales, int64_t rows, int32_t K, void *out, int32_t dtype,
+                          unit_stream_t stream);
 
 /* ------------------------------------------------------------------ diagnostics */
 

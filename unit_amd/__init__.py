@@ -4,8 +4,9 @@ from .ops import (conv2d_NCHWc_int8, conv2d_NCHWc_int8_fused, conv2d_NCHWc_int8_
                   last_variant, pack_nchwc, prepack_conv_weight, prepack_conv_weight_f16,
                   prepack_dense_weight, unpack_nchwc, PreparedConvWeight, prepare_conv2d_weight,
                   PreparedGemmB, prepare_gemm_b, PreparedDenseWeight, prepare_dense_weight)
-from .grouped import (Mxfp4Tensor, dense_mxfp4, dequantize_mxfp4, grouped_dense, grouped_dense_grad, grouped_dense_mxfp4,
-                      prepare_mxfp4_weight, quantize_mxfp4)
+from .grouped import (Mxfp4Tensor, Mxfp8Tensor, dense_mxfp4, dequantize_mxfp4, dequantize_mxfp8, grouped_dense, grouped_dense_grad,
+                      grouped_dense_mxfp4, prepare_mxfp4_weight, quantize_mxfp4, quantize_mxfp8)
+from .gated import gated_dense, gated_dense_grad, gated_dense_mxfp4
 from .intrinsics import INTRINSICS
 from . import rng, workloads
 

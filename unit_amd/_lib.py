@@ -61,6 +61,12 @@ SYMBOLS = (
     "unit_grouped_dense_grad_data",
     "unit_grouped_dense_grad_weight",
     "unit_grouped_dense_mxfp4",
+    "unit_gated_dense",
+    "unit_gated_dense_mxfp4",
+    "unit_gate_grad",
+    "unit_mxfp8_bytes",
+    "unit_quantize_mxfp8",
+    "unit_dequantize_mxfp8",
     "unit_mfma_tile_i8",
     "unit_mfma_tile_f16",
     "unit_mfma_peak",
@@ -152,6 +158,12 @@ def load():
     for name in ("unit_grouped_dense", "unit_grouped_dense_grad_data", "unit_grouped_dense_grad_weight"):
         getattr(L, name).argtypes = [vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp]
     L.unit_grouped_dense_mxfp4.argtypes = [vp, vp, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, vp, size, vp]
+    L.unit_gated_dense.argtypes = [vp, vp, vp, i32, vp, i32, i32, i32, vp, vp, i32, i32, i32, i32, i32, vp]
+    L.unit_gated_dense_mxfp4.argtypes = [vp, vp, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, size, vp]
+    L.unit_gate_grad.argtypes = [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp]
+    L.unit_mxfp8_bytes.argtypes = [i64, i32, sizep, sizep]
+    L.unit_quantize_mxfp8.argtypes = [vp, i32, i64, i32, vp, vp, vp]
+    L.unit_dequantize_mxfp8.argtypes = [vp, vp, i64, i32, vp, i32, vp]
     L.unit_mfma_tile_i8.argtypes = [vp, vp, vp, vp]
     L.unit_mfma_tile_f16.argtypes = [vp, vp, vp, vp]
     L.unit_mfma_peak.argtypes = [i32, i32, i32, vp, vp]

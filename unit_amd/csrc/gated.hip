@@ -1,0 +1,156 @@
+// Gated feed-forward products: entry points, and the gradients of the gate itself.
+#include "grouped_checks.hpp"
+#include "gated.hpp"
+
+namespace unit {
+namespace {
+
+int check_activation(const char *what, int code, Activation *a) {
+  return activation_of(code, a) ? UNIT_OK : fail(UNIT_E_ARG, "%s: activation must be UNIT_SILU or UNIT_GELU_TANH, got %d", what, code);
+}
+
+// both halves of a weight are products of N columns each
+int check_gated(const char *what, const void *sizes, int size_bytes, int rows, int groups, int N, int K, size_t w_bytes) {
+  if (N > 1 << 21) return fail(UNIT_E_ARG, "%s: more than 2^21 columns", what);
+  return check_groups(what, sizes, size_bytes, rows, groups, N, K, w_bytes);
+}
+
+// dpre from dh and the pre-activations, eight columns a lane: 16 bytes of each of three operands in, of each of two results out (six,
+// eight and two in MXFP8), which is what it is bound by.
+template <class Half, bool MX8, int ROUNDS>
+__global__ __launch_bounds__(256) void gate_grad_kernel(const char *pre, const unsigned char *scales, const Half *dh, Half *dpre, int pieces, int N, Activation act,
+                                                        FastDiv by_row) {
+  typedef Half v8h __attribute__((ext_vector_type(8)));
+  const int first = (int)blockIdx.x * (256 * ROUNDS) + (int)threadIdx.x, blocks = mx8_blocks(N);
+  v4u z[ROUNDS][2], d[ROUNDS];
+  u32 s[ROUNDS][2];
+  int row[ROUNDS], c[ROUNDS];
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    by_row.divmod(min(first + i * 256, pieces - 1), row[i], c[i]);
+    d[i] = *reinterpret_cast<const v4u *>(dh + (size_t)row[i] * N + c[i] * 8);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const size_t half = (size_t)row[i] * 2 + h;
+      if constexpr (MX8) {
+        const v2u codes = *reinterpret_cast<const v2u *>(pre + half * (blocks * 32) + c[i] * 8);
+        z[i][h] = v4u{codes[0], codes[1], 0, 0};
+        s[i][h] = scales[half * blocks + (c[i] >> 2)];
+      } else {
+        z[i][h] = *reinterpret_cast<const v4u *>(pre + (half * N + c[i] * 8) * 2);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    if (first + i * 256 >= pieces) break;
+    float f[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (MX8) {
+        const float p = mx8_power(s[i][h]);
+        const v4f lo = four_values8(z[i][h][0], p), hi = four_values8(z[i][h][1], p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[h][j] = j < 4 ? lo[j] : hi[j - 4];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[h][j] = (float)__builtin_bit_cast(v8h, z[i][h])[j];
+      }
+    }
+    v8h dg, du;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float slope;
+      const float a = act_both(act, f[0][j], &slope), g = (float)__builtin_bit_cast(v8h, d[i])[j];
+      // the operands of the products that follow: rounded to their type here, once
+      dg[j] = (Half)(g * f[1][j] * slope);
+      du[j] = (Half)(g * a);
+    }
+    Half *dst = dpre + (size_t)row[i] * 2 * N + c[i] * 8;
+    *reinterpret_cast<v8h *>(dst) = dg;
+    *reinterpret_cast<v8h *>(dst + N) = du;
+  }
+}
+
+template <class Half, bool MX8>
+int run_gate_grad(const char *what, const void *pre, const void *scales, const void *dh, void *dpre, int rows, int N, const Activation &act, hipStream_t s) {
+  const FastDiv by_row = FastDiv::make(N / 8);
+  const int slice = (1 << 30) / (N / 8);  // rows whose pieces are counted in 31 bits
+  for (int row = 0; row < rows; row += slice) {
+    const int pieces = (rows - row < slice ? rows - row : slice) * (N / 8);
+    const size_t pre_row = MX8 ? (size_t)mx8_blocks(N) * 64 : (size_t)N * 4;
+    const char *z = static_cast<const char *>(pre) + row * pre_row;
+    const unsigned char *zs = MX8 ? static_cast<const unsigned char *>(scales) + (size_t)row * 2 * mx8_blocks(N) : nullptr;
+    const Half *d = static_cast<const Half *>(dh) + (size_t)row * N;
+    Half *out = static_cast<Half *>(dpre) + (size_t)row * 2 * N;
+    if (pieces >= 512 * 1024)  // two pieces a lane while that makes four workgroups a CU
+      hipLaunchKernelGGL((gate_grad_kernel<Half, MX8, 2>), dim3((unsigned)((pieces + 511) / 512)), dim3(256), 0, s, z, zs, d, out, pieces, N, act, by_row);
+    else
+      hipLaunchKernelGGL((gate_grad_kernel<Half, MX8, 1>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, z, zs, d, out, pieces, N, act, by_row);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: launch: %s", what, hipGetErrorString(e));
+    if (row > rows - slice) break;  // row + slice may pass 2^31
+  }
+  set_variant(MX8 ? "gategrad_mx8" : "gategrad");
+  return UNIT_OK;
+}
+
+}  // namespace
+}  // namespace unit
+
+using namespace unit;
+
+extern "C" int unit_gated_dense(const void *x, const void *w, const void *sizes, int32_t size_bytes, void *out, int32_t dtype, int32_t out_dtype, int32_t activation,
+                                void *pre, void *pre_scales, int32_t pre_dtype, int32_t rows, int32_t groups, int32_t N, int32_t K, unit_stream_t stream) {
+  const char *what = "unit_gated_dense";
+  Activation act;
+  if (int rc = check_types(what, dtype, out_dtype)) return rc;
+  if (int rc = check_activation(what, activation, &act)) return rc;
+  if (int rc = check_gated(what, sizes, size_bytes, rows, groups, N, K, (size_t)N * K * 4)) return rc;
+  if (int rc = check_f16(what, N, K)) return rc;
+  if (pre && pre_dtype != dtype && pre_dtype != UNIT_MXFP8) return fail(UNIT_E_ARG, "%s: pre_dtype must be the operands' type or UNIT_MXFP8, got %d", what, pre_dtype);
+  const int gate = !pre ? GATE_ONLY : pre_dtype == UNIT_MXFP8 ? GATE_KEEP8 : GATE_KEEP;
+  if (int rc = check_ptrs(what, rows, {x, w, out})) return rc;
+  if (int rc = check_aligned(what, {pre})) return rc;
+  if (gate == GATE_KEEP8 && rows && !pre_scales) return fail(UNIT_E_ARG, "%s: null pointer", what);
+  if (int rc = check_device()) return rc;
+  if (!rows) return UNIT_OK;
+  GatedParams p{{static_cast<const char *>(x), static_cast<const char *>(w), nullptr, nullptr, static_cast<char *>(out), sizes, size_bytes, groups, rows, N, K},
+                act, static_cast<char *>(pre), static_cast<char *>(pre_scales)};
+  return (dtype == UNIT_F16 ? run_gated_f16 : run_gated_bf16)(what, gate, p, out_dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int unit_gated_dense_mxfp4(const void *x, const void *xscales, int32_t x_dtype, const void *wcodes, const void *wscales, const void *sizes,
+                                      int32_t size_bytes, void *out, int32_t out_dtype, int32_t activation, int32_t rows, int32_t groups, int32_t N, int32_t K, void *ws,
+                                      size_t ws_bytes, unit_stream_t stream) {
+  const char *what = "unit_gated_dense_mxfp4";
+  Activation act;
+  if (int rc = check_activation(what, activation, &act)) return rc;
+  if (int rc = check_gated(what, sizes, size_bytes, rows, groups, N, K, N > 0 && K > 0 ? mx_code_bytes(2l * N, K) : 0)) return rc;
+  GatedParams p{{static_cast<const char *>(x), static_cast<const char *>(wcodes), static_cast<const u32 *>(xscales), static_cast<const u32 *>(wscales),
+                 static_cast<char *>(out), sizes, size_bytes, groups, rows, N, K, x_dtype}, act, nullptr, nullptr};
+  bool run;
+  if (int rc = mxfp4_rows(what, &p, out_dtype, ws, ws_bytes, static_cast<hipStream_t>(stream), [](const GroupedParams &) { return false; }, &run)) return rc;
+  return run ? run_gated_mx(what, p, out_dtype, static_cast<hipStream_t>(stream)) : UNIT_OK;
+}
+
+extern "C" int unit_gate_grad(const void *pre, const void *pre_scales, int32_t pre_dtype, const void *dh, void *dpre, int32_t dtype, int32_t activation, int32_t rows,
+                              int32_t N, unit_stream_t stream) {
+  const char *what = "unit_gate_grad";
+  Activation act;
+  if (int rc = check_types(what, dtype, dtype)) return rc;
+  if (int rc = check_activation(what, activation, &act)) return rc;
+  if (pre_dtype != dtype && pre_dtype != UNIT_MXFP8) return fail(UNIT_E_ARG, "%s: pre_dtype must be dtype or UNIT_MXFP8, got %d", what, pre_dtype);
+  if (rows < 0 || N <= 0 || N % 8) return fail(UNIT_E_ARG, "%s: rows must not be negative and N a positive multiple of 8", what);
+  if (rows > 1 << 30 || N > 1 << 21) return fail(UNIT_E_ARG, "%s: sizes beyond 2^30 rows or 2^21 columns", what);
+  if (int rc = check_ptrs(what, rows, {pre, dh, dpre})) return rc;
+  if (pre_dtype == UNIT_MXFP8 && rows && !pre_scales) return fail(UNIT_E_ARG, "%s: null pointer", what);
+  if (int rc = check_device()) return rc;
+  if (!rows) return UNIT_OK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == UNIT_F16)
+    return pre_dtype == UNIT_MXFP8 ? run_gate_grad<_Float16, true>(what, pre, pre_scales, dh, dpre, rows, N, act, s)
+                                   : run_gate_grad<_Float16, false>(what, pre, pre_scales, dh, dpre, rows, N, act, s);
+  return pre_dtype == UNIT_MXFP8 ? run_gate_grad<__bf16, true>(what, pre, pre_scales, dh, dpre, rows, N, act, s)
+                                 : run_gate_grad<__bf16, false>(what, pre, pre_scales, dh, dpre, rows, N, act, s);
+}

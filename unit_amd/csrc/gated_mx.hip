@@ -1,0 +1,25 @@
+// MXFP4 gated products.
+#include "gated_tile.hpp"
+
+namespace unit {
+namespace {
+
+template <class Out>
+int run(const char *what, const GatedParams &p, hipStream_t s) {
+  const char *tag = "mxgated";
+  switch (gated_tile_size(p, true)) {
+    case TILE_FEW: return run_grouped_tile<OpMx, FORWARD, Tile<32, 128, 128, 1, 2>, 2, Out, GATE_ONLY>(what, tag, p, s);
+    case TILE_SMALL: return run_grouped_tile<OpMx, FORWARD, Tile<64, 128, 128, 2, 2>, 3, Out, GATE_ONLY>(what, tag, p, s);
+    case TILE_MIDDLE: return run_grouped_tile<OpMx, FORWARD, Tile<128, 128, 128, 2, 2>, 2, Out, GATE_ONLY>(what, tag, p, s);
+    default: return run_grouped_tile<OpMx, FORWARD, Tile<256, 256, 128, 2, 4>, 2, Out, GATE_ONLY>(what, tag, p, s);
+  }
+}
+
+}  // namespace
+
+int run_gated_mx(const char *what, const GatedParams &p, int out_dtype, hipStream_t s) {
+  if (out_dtype == UNIT_F32) return run<float>(what, p, s);
+  return out_dtype == UNIT_F16 ? run<_Float16>(what, p, s) : run<__bf16>(what, p, s);
+}
+
+}  // namespace unit

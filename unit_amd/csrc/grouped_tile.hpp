@@ -15,19 +15,25 @@
 // last (weight gradient) read as zeros, and rows past a tile's last valid one read as zeros or stay in the tensor.  A reduction that ends
 // inside a stage of rows: lanes whose chunk lies past its end are sent out of the descriptor, on both sides, so that what
 // lies behind (NaN, say) meets nothing.
+//
+// A gated product (GATE, gated.hpp) is a forward product whose tile of Y holds as many rows of the gate's weight as of the up projection's,
+// 32 by 32 within each wave's share: a lane then has gate x and up x of the same columns in two of its accumulators, and the activation, the
+// product and what is kept of them for the backward pass happen on the way out.
 #pragma once
-#include "grouped.hpp"
+#include "gated.hpp"
 #include "mma_dma.hpp"
 
 namespace unit {
 
 struct OpHalf {
   using acc_t = v16f;
+  using half_t = _Float16;
   static constexpr bool kMx = false;
   static __device__ __forceinline__ acc_t mma(v4i x, v4i y, acc_t c) { return OpF16::mma(x, y, c); }
 };
 struct OpBF16 {
   using acc_t = v16f;
+  using half_t = __bf16;
   static constexpr bool kMx = false;
   static __device__ __forceinline__ acc_t mma(v4i x, v4i y, acc_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, x), __builtin_bit_cast(v8b, y), c, 0, 0, 0);
@@ -36,6 +42,7 @@ struct OpBF16 {
 // 64 elements of 4 bits are 32 bytes like 16 of 16 bits: the tiling in bytes is the same.  S: which byte of the scale dwords
 struct OpMx {
   using acc_t = v16f;
+  using half_t = __bf16;  // of nothing: its gated products keep no pre-activations
   static constexpr bool kMx = true;
   template <int S>
   static __device__ __forceinline__ acc_t mma(v4i x, v4i y, acc_t c, int sx, int sy) {
@@ -192,9 +199,121 @@ __device__ __forceinline__ int cols_swz(int row) {
   return WIDTH == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3);
 }
 
-// One tile: rows x0 .. x0 + high - 1 of the group's (weight gradient: rows of dw), columns y0 .. y0 + BY - 1.
-template <class Op, int DIR, class T, int NSTAGE, class Out>
-__device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, int group, int first, int count, int x0, int high, int y0) {
+// 32 rows of results of a wave, BLOCKS * 32 columns: put in order in LDS of the wave's own, then written in runs of 16 bytes a lane.
+// rows: that LDS; dst: column 0 of the first of `high` rows that are `ld` elements apart and have `width` columns; y: the wave's first
+// column; value(j, r): columns 32 j + 8 r + 4 half .. + 3 of row l32.
+template <class E, int BLOCKS>
+struct RowsOut {
+  static constexpr int ES = (int)sizeof(E), PITCH = BLOCKS * 32 * ES + 16, PER = 16 / ES, RUNS = BLOCKS * 32 / PER;  // elements per run, runs per row
+  template <class F>
+  static __device__ __forceinline__ void put(char *rows, char *dst, long ld, int high, int width, int y, F value) {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+    typedef E v4e __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const v4f f = value(j, r);
+        v4e v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (E)f[e];
+        *reinterpret_cast<v4e *>(rows + l32 * PITCH + (j * 32 + 8 * r + 4 * half) * ES) = v;
+      }
+    const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(dst, 0, -1, 0x00020000);
+#pragma unroll
+    for (int k = 0; k < 32 * RUNS / 64; ++k) {
+      const int row = (k * 64 + lane) / RUNS, c = (k * 64 + lane) % RUNS * PER, at = y + c;
+      const v4u v = *reinterpret_cast<const v4u *>(rows + row * PITCH + c * ES);
+      if (row >= high || at >= width) continue;
+      const u32 off = ((u32)row * (u32)ld + (u32)at) * (u32)ES;
+      if (ld % PER == 0 && at + PER <= width) {
+        store_result<kRowPolicy>(out, off, v);
+      } else if (at + PER <= width) {  // rows begin on any element: the same 16 bytes, unaligned
+        typedef u32 v4un __attribute__((ext_vector_type(4), aligned(2)));
+        *reinterpret_cast<v4un *>(dst + off) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (at + e < width) {
+            if constexpr (ES == 4)
+              store_result<kRowPolicy>(out, off + e * 4, v[e]);
+            else
+              store_result<kRowPolicy>(out, off + e * 2, (unsigned short)(v[e / 2] >> (e % 2 * 16)));
+          }
+      }
+    }
+  }
+};
+
+// The same for MXFP8, which keeps whole blocks: each of a row's BLOCKS blocks is in two lanes, 16 columns each.
+template <int BLOCKS, class F>
+__device__ __forceinline__ void put_mx8(char *rows, char *codes, char *scales, int blocks, int high, int width, int y, F value) {
+  constexpr int PITCH = BLOCKS * 32 + 16, RUNS = BLOCKS * 2;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < BLOCKS; ++j) {
+    v4f f[4];
+    u32 top = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      f[r] = value(j, r);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (y + j * 32 + 8 * r + 4 * half + e >= width) f[r][e] = 0;  // zeros behind the row's end
+      const v4u bits = __builtin_bit_cast(v4u, f[r]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, bits[e] & 0x7fffffffu);
+    }
+    top = max(top, (u32)__shfl_xor((int)top, 32));
+    const u32 s = mx8_scale(top);
+    const float p = mx_power(s == 255 ? 127 : s);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) *reinterpret_cast<u32 *>(rows + l32 * PITCH + j * 32 + 8 * r + 4 * half) = four_codes8(f[r], p);
+    if (half == 0 && l32 < high && y + j * 32 < width) scales[(long)l32 * 2 * blocks + (y >> 5) + j] = (char)s;
+  }
+#pragma unroll
+  for (int k = 0; k < (32 * RUNS + 63) / 64; ++k) {
+    const int row = (k * 64 + lane) / RUNS, c = (k * 64 + lane) % RUNS * 16;
+    const v4u v = *reinterpret_cast<const v4u *>(rows + row * PITCH + c);
+    if (row < high && y + c < blocks * 32) *reinterpret_cast<v4u *>(codes + (long)row * 2 * blocks * 32 + y + c) = v;
+  }
+}
+
+// A wave's results of a gated product: acc[i][j] holds gate x, acc[i][j + TY / 2] up x.  The activation is of the sums in fp32; h and what
+// is kept are rounded from them once each.
+template <class T, int GATE, class Half, class Out, class Acc>
+__device__ __forceinline__ void gated_results(const GatedParams &p, char *rows, const Acc &acc, int blocks, long row0, int x0, int high, int y) {
+  constexpr int CB = T::TY / 2;
+#pragma unroll
+  for (int i = 0; i < T::TX; ++i) {
+    if (i >= blocks) break;
+    const int left = high - x0 - i * 32;
+    const long row = row0 + x0 + i * 32;
+    auto part = [&](int j, int r) __attribute__((always_inline)) { return v4f{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]}; };
+    if constexpr (GATE == GATE_KEEP) {
+      char *pre = p.pre + row * 2 * p.n * 2;
+      RowsOut<Half, CB>::put(rows, pre, 2l * p.n, left, p.n, y, part);
+      RowsOut<Half, CB>::put(rows, pre + 2l * p.n, 2l * p.n, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) { return part(j + CB, r); });
+    }
+    if constexpr (GATE == GATE_KEEP8) {
+      const int nb = mx8_blocks(p.n);
+      char *codes = p.pre + row * 2 * nb * 32, *scales = p.pre_scales + row * 2 * nb;
+      put_mx8<CB>(rows, codes, scales, nb, left, p.n, y, part);
+      put_mx8<CB>(rows, codes + nb * 32l, scales + nb, nb, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) { return part(j + CB, r); });
+    }
+    RowsOut<Out, CB>::put(rows, p.out + row * p.n * (long)sizeof(Out), p.n, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) {
+      const v4f g = part(j, r), u = part(j + CB, r);
+      v4f h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = act_value(p.act, g[e]) * u[e];
+      return h;
+    });
+  }
+}
+
+// One tile: rows x0 .. x0 + high - 1 of the group's (weight gradient: rows of dw), columns y0 .. y0 + BY - 1 (gated: BY / 2 of them).
+template <class Op, int DIR, class T, int NSTAGE, class Out, int GATE = GATE_NONE>
+__device__ __forceinline__ void compute_tile(const GateParams<GATE> &p, char *lds, int group, int first, int count, int x0, int high, int y0) {
   constexpr bool MX = Op::kMx, XT = DIR == GRAD_WEIGHT, YT = DIR != FORWARD;
   constexpr int KK = T::BKB / 32, CPR = T::CPR, NW = T::NT / 64, RPL = 64 / CPR;
   constexpr int KS = T::BKB / 2;                     // cols: reduction elements of a stage
@@ -213,6 +332,14 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
   const u32 ring = (u32)(uintptr_t)(lptr_t)lds;
 
   const int ys = DIR == FORWARD ? p.n : p.k;  // columns of the result
+  const int wrows = GATE ? 2 * p.n : p.n;     // rows of a group's weight
+  constexpr int WCOLS = T::TY * 32 / (GATE ? 2 : 1);  // columns of the result per wave
+  // the weight's row, counted from y0, that lies in row `row` of the tile of Y
+  auto yrow_of = [&](int row) __attribute__((always_inline)) {
+    if constexpr (!GATE) return row;
+    const int block = row / 32 % T::TY;
+    return (block >= T::TY / 2 ? p.n : 0) + row / (T::TY * 32) * WCOLS + block % (T::TY / 2 ? T::TY / 2 : 1) * 32 + row % 32;
+  };
   const bool live = group < p.groups;
 
   // operand bases (of this tile's first row or column), bytes per row, and how many bytes lie behind the base
@@ -230,14 +357,14 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
     xb = p.x + (long)(first + x0) * xld, xleft = (long)high * xld;
     if constexpr (YT)
       yb = p.y + (long)group * p.n * yld + 2l * y0, yleft = (long)p.n * yld - 2l * y0;
-    else
-      yb = p.y + ((long)group * p.n + y0) * yld, yleft = (long)min(ys - y0, T::BY) * yld;
+    else  // gated: what lies between the gate's last row and the up projection's first one is read and meets no result
+      yb = p.y + ((long)group * wrows + y0) * yld, yleft = (GATE ? (long)(wrows - y0) : (long)min(ys - y0, T::BY)) * yld;
   }
   const long xstep = XT ? (long)KS * xld : T::BKB, ystep = YT ? (long)KS * yld : T::BKB;  // bytes from stage to stage
 
   // this lane's chunk of each load
   u32 xoff[XL], yoff[YL];
-  auto offset = [&](auto cols, auto width, int load, long ld) __attribute__((always_inline)) {
+  auto offset = [&](auto cols, auto width, int load, long ld, auto row_of) __attribute__((always_inline)) {
     constexpr int W = decltype(width)::value;
     if constexpr (decltype(cols)::value) {
       constexpr int CPW = W / 8;
@@ -245,23 +372,24 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
       return (u32)row * (u32)ld + (u32)(((lane % CPW) ^ cols_swz<W>(row)) << 4);
     } else {
       const int row = load * RPL + lane / CPR;
-      return (u32)row * (u32)ld + (u32)(((lane % CPR) ^ swz<T::BKB>(row)) << 4);
+      return (u32)row_of(row) * (u32)ld + (u32)(((lane % CPR) ^ swz<T::BKB>(row)) << 4);
     }
   };
+  auto same = [](int row) __attribute__((always_inline)) { return row; };
 #pragma unroll
-  for (int i = 0; i < XL; ++i) xoff[i] = offset(std::integral_constant<bool, XT>{}, std::integral_constant<int, T::BX>{}, wave * XL + i, xld);
+  for (int i = 0; i < XL; ++i) xoff[i] = offset(std::integral_constant<bool, XT>{}, std::integral_constant<int, T::BX>{}, wave * XL + i, xld, same);
 #pragma unroll
-  for (int i = 0; i < YL; ++i) yoff[i] = offset(std::integral_constant<bool, YT>{}, std::integral_constant<int, T::BY>{}, wave * YL + i, yld);
+  for (int i = 0; i < YL; ++i) yoff[i] = offset(std::integral_constant<bool, YT>{}, std::integral_constant<int, T::BY>{}, wave * YL + i, yld, yrow_of);
   // MXFP4: the scales of a stage, X rows then Y rows, each [half][row] dwords, 64 pieces of four rows per load
   const char *sptr = nullptr;
   long sstep = 0;
   if constexpr (MX) {
     const int c = min((wave % PIECE) * 64 + lane, (T::BX + T::BY) / 2 - 1), cy = c - T::BX / 2;
-    const long xrows = p.rows, yrows = (long)p.groups * p.n;
+    const long xrows = p.rows, yrows = (long)p.groups * wrows;
     if (c < T::BX / 2)
       sptr = reinterpret_cast<const char *>(p.xs + c / (T::BX / 4) * xrows + first + x0 + c % (T::BX / 4) * 4), sstep = xrows * 8;
     else
-      sptr = reinterpret_cast<const char *>(p.ys + cy / (T::BY / 4) * yrows + (long)group * p.n + y0 + cy % (T::BY / 4) * 4), sstep = yrows * 8;
+      sptr = reinterpret_cast<const char *>(p.ys + cy / (T::BY / 4) * yrows + (long)group * wrows + y0 + yrow_of(cy % (T::BY / 4) * 4)), sstep = yrows * 8;
   }
 
   struct Source {
@@ -435,7 +563,7 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
       stage(nxc, kt, kt % NSTAGE, no{}, no{}, no{}, no{});
     };
     // a wave without columns has no rows either
-    const int blocks = y0 + wy * (T::TY * 32) < ys ? blocks_x : 0;
+    const int blocks = y0 + wy * WCOLS < ys ? blocks_x : 0;
     if (blocks == T::TX)
       loop(std::integral_constant<int, T::TX>{});
     else if (blocks == 0)
@@ -450,6 +578,14 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
 
   // Results, rounded once, here: each wave puts 32 rows of its columns in order in LDS of its own and writes them in runs of 16 bytes a lane.
   // (Straight from the registers, 2 bytes a lane: experts of 16384 x 1024 -> 2048 102.7 us, 96.2 like this.)
+  if constexpr (GATE) {
+    static_assert(T::TY % 2 == 0 && DIR == FORWARD, "a wave has the gate's columns and the up projection's");
+    constexpr int PITCH = RowsOut<float, T::TY / 2>::PITCH;  // of the widest
+    static_assert(NW * 32 * PITCH <= NSTAGE * STAGE, "the waves' rows fit the ring");
+    __syncthreads();  // the ring is read out
+    gated_results<T, GATE, typename Op::half_t, Out>(p, lds + wave * (32 * PITCH), acc, blocks_x, (long)first + x0, block0 * 32, high, y0 + wy * WCOLS);
+    return;
+  }
   constexpr int ES_OUT = (int)sizeof(Out), PITCH = T::TY * 32 * ES_OUT + 16, PER = 16 / ES_OUT, RUNS = T::TY * 32 / PER;  // elements per run, runs per row
   static_assert(NW * 32 * PITCH <= NSTAGE * STAGE, "the waves' rows fit the ring");
   __syncthreads();  // the ring is read out
@@ -500,8 +636,8 @@ __device__ __forceinline__ void compute_tile(const GroupedParams &p, char *lds, 
   }
 }
 
-template <class Op, int DIR, class T, int NSTAGE, class Out>
-__global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nts, int xts) {
+template <class Op, int DIR, class T, int NSTAGE, class Out, int GATE = GATE_NONE>
+__global__ __launch_bounds__(T::NT, 2) void grouped_tile(GateParams<GATE> p, int nts, int xts) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63;
   if constexpr (DIR == GRAD_WEIGHT) {
@@ -514,22 +650,22 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GroupedParams p, int nt
   } else {
     const GroupTileOf g = find_tile<T::BX, 4>(p, nts, (int)blockIdx.x, lane);
     if (!g.any) return;
-    compute_tile<Op, DIR, T, NSTAGE, Out>(p, lds, g.group, g.first, g.count, g.x0, g.high, g.nt * T::BY);
+    compute_tile<Op, DIR, T, NSTAGE, Out, GATE>(p, lds, g.group, g.first, g.count, g.x0, g.high, g.nt * (GATE ? T::BY / 2 : T::BY));
   }
 }
 
-template <class Op, int DIR, class T, int NSTAGE, class Out>
-int run_grouped_tile(const char *what, const char *tag, const GroupedParams &p, hipStream_t s) {
+template <class Op, int DIR, class T, int NSTAGE, class Out, int GATE = GATE_NONE>
+int run_grouped_tile(const char *what, const char *tag, const GateParams<GATE> &p, hipStream_t s) {
   constexpr int lds = NSTAGE * (T::STAGE + (Op::kMx ? ((T::BX + T::BY) * 8 + 1023) / 1024 * 1024 : 0));
   static_assert(lds <= kMaxLds, "ring does not fit the LDS");
-  auto kern = grouped_tile<Op, DIR, T, NSTAGE, Out>;
+  auto kern = grouped_tile<Op, DIR, T, NSTAGE, Out, GATE>;
   static thread_local bool allowed = false;
   if (!allowed && lds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds);
     if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: hipFuncSetAttribute: %s", what, hipGetErrorString(e));
     allowed = true;
   }
-  const int ys = DIR == FORWARD ? p.n : p.k, nts = ceil_div(ys, T::BY), xts = ceil_div(p.n, T::BX);
+  const int ys = DIR == FORWARD ? p.n : p.k, nts = ceil_div(ys, GATE ? T::BY / 2 : T::BY), xts = ceil_div(p.n, T::BX);
   long wgs;
   if (DIR == GRAD_WEIGHT) {
     wgs = (long)p.groups * nts * xts;

@@ -3,11 +3,13 @@
 the reference, whose dense operators (apps/cpu/relay/int8-gemm.py:14-16, apps/gpu/gemm.py:8-20) these stand beside.
 
   quantize_mxfp4, dequantize_mxfp4   floats <-> 4-bit floats with a power of two per 32 elements
+  quantize_mxfp8, dequantize_mxfp8   floats <-> 8-bit floats with a power of two per 32 elements: activations kept for a backward pass
   prepare_mxfp4_weight               a checkpoint's codes and scales, laid out once for the products
   dense_mxfp4                        x . W^T with both operands in MXFP4
   grouped_dense, grouped_dense_grad  rows sorted by expert times their expert's weight, and the gradients
   grouped_dense_mxfp4                the same product with MXFP4 operands
 """
+import contextlib
 import ctypes
 import math
 
@@ -15,12 +17,12 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .ops import _Calls, _dev, _stream
+from .ops import _Calls, _dev, _device, _stream
 
-__all__ = ["Mxfp4Tensor", "quantize_mxfp4", "dequantize_mxfp4", "prepare_mxfp4_weight", "dense_mxfp4", "grouped_dense",
+__all__ = ["Mxfp4Tensor", "Mxfp8Tensor", "quantize_mxfp8", "dequantize_mxfp8", "quantize_mxfp4", "dequantize_mxfp4", "prepare_mxfp4_weight", "dense_mxfp4", "grouped_dense",
            "grouped_dense_grad", "grouped_dense_mxfp4"]
 
-_MXFP4 = 3
+_MXFP4, _MXFP8 = 3, 4
 _CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _OUT = {"float32": torch.float32, "float16": torch.float16, "bfloat16": torch.bfloat16}
 
@@ -208,17 +210,94 @@ def grouped_dense_mxfp4(data, weight, group_sizes, out_dtype="float32"):
     return _mxfp4_product(data, weight, group_sizes, out_dtype, 3) if out is None else out
 
 
+# ------------------------------------------------------------------------------- MXFP8
+def _on(t):
+    """the device that t lives on as the current one, so that its current stream is what the work runs on"""
+    if _device is not None and t.device.index == _device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _mxfp8_bytes(rows, k):
+    codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
+    check(_lib.load().unit_mxfp8_bytes(rows, k, ctypes.byref(codes), ctypes.byref(scales)))
+    return codes.value, scales.value
+
+
+class Mxfp8Tensor:
+    """Rows in MXFP8: along the last axis blocks of 32 elements share a power of two, elements are 8-bit floats (e4m3: three mantissa
+    bits, up to 448).  33 bytes for 32 elements: what a training step keeps of its activations until the backward pass.  `buf` holds the
+    codes, then the scales (include/unit_amd.h); made by quantize_mxfp8 and gated_dense, read back by dequantize_mxfp8."""
+
+    __slots__ = ("buf", "shape")
+
+    def __init__(self, buf, shape):
+        self.buf, self.shape = buf, shape
+
+    @property
+    def device(self):
+        return self.buf.device
+
+    def _pointers(self):
+        """addresses of codes and scales, rows, length of a row"""
+        rows = math.prod(self.shape[:-1])
+        codes, scales = _mxfp8_bytes(rows, self.shape[-1])
+        if self.buf.numel() < codes + scales:
+            raise ValueError(f"{self!r}: a buffer of {self.buf.numel()} bytes, {codes + scales} needed")
+        return self.buf.data_ptr(), self.buf.data_ptr() + codes, rows, self.shape[-1]
+
+    def __repr__(self):
+        return f"Mxfp8Tensor(shape={self.shape}, device='{self.device}')"
+
+
+def _mxfp8_empty(shape, device):
+    return Mxfp8Tensor(torch.empty((sum(_mxfp8_bytes(math.prod(shape[:-1]), shape[-1])),), dtype=torch.uint8, device=device), tuple(shape))
+
+
+def quantize_mxfp8(x):
+    """x of two or three axes, float32, float16 or bfloat16 -> Mxfp8Tensor of the same shape.
+
+    The scale of a block is the smallest power of two, 2^-127 at least, for which its largest magnitude is at most 448; elements are
+    x / scale rounded to the nearest 8-bit float, ties to the even mantissa, so nothing saturates.  A block that holds an infinity or
+    a NaN becomes NaN throughout."""
+    x = _floats(x, "x", tuple(_CODE))
+    if x.dim() not in (2, 3):
+        raise ValueError(f"x: expected two axes or three, got shape {tuple(x.shape)}")
+    with _on(x):
+        q = _mxfp8_empty(x.shape, x.device)
+        codes, scales, rows, k = q._pointers()
+        check(_lib.load().unit_quantize_mxfp8(x.data_ptr(), _CODE[x.dtype], rows, k, codes, scales, _stream()))
+    return q
+
+
+def dequantize_mxfp8(q, out_dtype="float32"):
+    """The values that an Mxfp8Tensor stands for, rounded once where out_dtype does not hold them.  The type that was quantised holds them all
+    but for the power of two above its largest value, which magnitudes within a thirty-second of it become: infinite."""
+    dt = _out_dtype(out_dtype)
+    if not isinstance(q, Mxfp8Tensor):
+        raise TypeError(f"q: expected an Mxfp8Tensor, got {type(q).__name__}")
+    with _on(q.buf):
+        codes, scales, rows, k = q._pointers()
+        out = torch.empty(q.shape, dtype=dt, device=q.device)
+        check(_lib.load().unit_dequantize_mxfp8(codes, scales, rows, k, out.data_ptr(), _CODE[dt], _stream()))
+    return out
+
+
 # ------------------------------------------------------------------------------- 16-bit operands
+_NAME = {v: k for k, v in _OUT.items()}
 _HALVES = (torch.float16, torch.bfloat16)
 
 
 def _grouped(data, weight, group_sizes):
-    data = _floats(data, "data", _HALVES, 2)
-    weight = _dev(weight, "weight", data.dtype, 3)
+    if isinstance(data, Mxfp8Tensor):
+        weight = _floats(weight, "weight", _HALVES, 3)
+    else:
+        data = _floats(data, "data", _HALVES, 2)
+        weight = _dev(weight, "weight", data.dtype, 3)
     _same_device(weight, "weight", data)
     sizes = _sizes(group_sizes, data)
     e, n, k = weight.shape
-    if data.shape[1] != k:
+    if len(data.shape) != 2 or data.shape[1] != k:
         raise ValueError(f"data: expected (rows, {k}), got {tuple(data.shape)}")
     if sizes.shape[0] != e:
         raise ValueError(f"group_sizes: expected {e} entries, got {sizes.shape[0]}")
@@ -245,7 +324,7 @@ def grouped_dense(data, weight, group_sizes, out_dtype="float32"):
 def grouped_dense_grad(data, weight, grad, group_sizes, out_dtype="float32", weight_out_dtype="float32"):
     """The gradients of grouped_dense for grad (rows, N), of data's type: (ddata (rows, K), dweight (E, N, K)), in out_dtype and
     weight_out_dtype.  ddata is zero in rows of no expert, dweight for experts without rows; sums in float32, in the order of
-    the rows whatever runs beside it."""
+    the rows whatever runs beside it.  data may be kept in MXFP8 (rows, K), grad is then of weight's type and so are the rows again."""
     both = _native.grouped_grad(data, weight, grad, group_sizes, out_dtype, weight_out_dtype)
     if both is not None:
         return both
@@ -256,19 +335,27 @@ def _grouped_grad(data, weight, grad, group_sizes, out_dtype, weight_out_dtype, 
     """(ddata, dweight), None in the place of one that is not wanted: it costs neither time nor memory"""
     dt, wdt = _out_dtype(out_dtype), _out_dtype(weight_out_dtype, "weight_out_dtype")
     data, weight, sizes, e, n, k = _grouped(data, weight, group_sizes)
-    grad = _dev(grad, "grad", data.dtype, 2)
+    grad = _dev(grad, "grad", weight.dtype, 2)
     _same_device(grad, "grad", data)
     rows = data.shape[0]
     if tuple(grad.shape) != (rows, n):
         raise ValueError(f"grad: expected ({rows}, {n}), got {tuple(grad.shape)}")
-    L, tail = _lib.load(), (rows, e, n, k, _stream())
+    with _on(weight) if isinstance(data, Mxfp8Tensor) else contextlib.nullcontext():
+        return _product_grads(data, weight, grad, sizes, (rows, e, n, k), dt, wdt, wanted)
+
+
+def _product_grads(data, weight, grad, sizes, shape, dt, wdt, wanted):
+    """the gradients' two products; sizes None: one group, whose weight may have two axes"""
+    rows, e, n, k = shape
+    L, tail, code = _lib.load(), (*shape, _stream()), _CODE[weight.dtype]
+    groups = (None, 4) if sizes is None else (sizes.data_ptr(), sizes.element_size())
     ddata = dweight = None
     if wanted[0]:
-        ddata = torch.empty((rows, k), dtype=dt, device=data.device)
-        check(L.unit_grouped_dense_grad_data(grad.data_ptr(), weight.data_ptr(), sizes.data_ptr(), sizes.element_size(), ddata.data_ptr(),
-                                             _CODE[data.dtype], _CODE[dt], *tail))
+        ddata = torch.empty((rows, k), dtype=dt, device=weight.device)
+        check(L.unit_grouped_dense_grad_data(grad.data_ptr(), weight.data_ptr(), *groups, ddata.data_ptr(), code, _CODE[dt], *tail))
     if wanted[1]:
-        dweight = torch.empty((e, n, k), dtype=wdt, device=data.device)
-        check(L.unit_grouped_dense_grad_weight(data.data_ptr(), grad.data_ptr(), sizes.data_ptr(), sizes.element_size(), dweight.data_ptr(),
-                                               _CODE[data.dtype], _CODE[wdt], *tail))
+        if isinstance(data, Mxfp8Tensor):
+            data = dequantize_mxfp8(data, _NAME[weight.dtype])
+        dweight = torch.empty(weight.shape, dtype=wdt, device=weight.device)
+        check(L.unit_grouped_dense_grad_weight(data.data_ptr(), grad.data_ptr(), *groups, dweight.data_ptr(), code, _CODE[wdt], *tail))
     return ddata, dweight
