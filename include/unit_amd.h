@@ -399,11 +399,18 @@ int unit_gated_dense(const void *x, const void *w, const void *sizes, int32_t si
 int unit_gated_dense_mxfp4(const void *x, const void *xscales, int32_t x_dtype, const void *wcodes, const void *wscales,
                            const void *sizes, int32_t size_bytes, void *out, int32_t out_dtype, int32_t activation, int32_t rows,
                            int32_t groups, int32_t N, int32_t K, void *ws, size_t ws_bytes, unit_stream_t stream);
-/* the gradients of the gate for dh (rows, N): dpre (rows, 2, N), dpre[r][0] = dh u act'(g), dpre[r][1] = dh act(g) for kept
- * g = pre[r][0], u = pre[r][1], computed in fp32 and rounded once to dtype.  unit_grouped_dense_grad_data and
- * unit_grouped_dense_grad_weight take dpre from there, with 2 N for N. */
-int unit_gate_grad(const void *pre, const void *pre_scales, int32_t pre_dtype, const void *dh, void *dpre, int32_t dtype,
-                   int32_t activation, int32_t rows, int32_t N, unit_stream_t stream);
+/* its gradients for dh (rows, N): dx (rows, K) and dw (groups, 2 N, K), either of them NULL where it is not wanted, zeros for rows of
+ * no group and for groups without rows.  x (rows, K) in dtype or in MXFP8 (x_dtype UNIT_MXFP8), not read where there is pre and no
+ * dw; pre what unit_gated_dense kept, or NULL: gate x and up x are then computed from x again.  The gate's gradients, dh u act'(g) and
+ * dh act(g), are computed in fp32 and rounded to dtype, the type of w, dh and of the products that follow; those sum in fp32 and
+ * round once to dx_dtype and dw_dtype (UNIT_F32 or dtype).  ws: unit_gated_dense_grad_ws_bytes, 16-byte aligned, of any
+ * contents, the call's alone until it has run on the stream. */
+int unit_gated_dense_grad_ws_bytes(int32_t x_dtype, int32_t dtype, int32_t rows, int32_t groups, int32_t N, int32_t K,
+                                   size_t *bytes);
+int unit_gated_dense_grad(const void *x, const void *x_scales, int32_t x_dtype, const void *w, const void *dh, const void *pre,
+                          const void *pre_scales, int32_t pre_dtype, const void *sizes, int32_t size_bytes, void *dx,
+                          int32_t dx_dtype, void *dw, int32_t dw_dtype, int32_t dtype, int32_t activation, int32_t rows,
+                          int32_t groups, int32_t N, int32_t K, void *ws, size_t ws_bytes, unit_stream_t stream);
 
 /* ------------------------------------------------------------------ MXFP8
  * Rows of 8-bit floats (e4m3: sign, four exponent bits, three mantissa bits, up to 448), 32 consecutive elements of a row sharing

@@ -61,12 +61,22 @@ def test_gated_mxfp4_arguments(L):
         said(L, call(**change), text)
 
 
-def test_gate_gradient_arguments(L):
-    ok = dict(pre=16, pre_scales=None, pre_dtype=1, dh=16, dpre=16, dtype=1, act=0, rows=4, n=16, stream=None)
-    call = lambda **change: L.unit_gate_grad(*{**ok, **change}.values())
-    for change, text in ((dict(pre=None), "null"), (dict(dh=None), "null"), (dict(dpre=None), "null"), (dict(pre_dtype=4), "null"), (dict(pre_dtype=2), "pre_dtype"),
-                         (dict(pre_dtype=0), "pre_dtype"), (dict(dtype=0), "dtype"), (dict(act=2), "activation"), (dict(rows=-1), "negative"), (dict(n=12), "multiple of 8"),
-                         (dict(n=0), "multiple of 8"), (dict(n=1 << 22), "2^21"), (dict(pre=8), "aligned"), (dict(dh=8), "aligned"), (dict(dpre=8), "aligned")):
+def test_gated_gradient_arguments(L):
+    need = ctypes.c_size_t()
+    assert L.unit_gated_dense_grad_ws_bytes(1, 1, 4, 2, 16, 16, ctypes.byref(need)) == 0 and need.value == 256
+    assert L.unit_gated_dense_grad_ws_bytes(4, 2, 1000, 2, 24, 40, ctypes.byref(need)) == 0 and need.value == 1000 * 96 + 1000 * 80
+    assert L.unit_gated_dense_grad_ws_bytes(1, 1, 0, 2, 16, 16, ctypes.byref(need)) == 0 and need.value == 0
+    said(L, L.unit_gated_dense_grad_ws_bytes(2, 1, 4, 2, 16, 16, ctypes.byref(need)), "x_dtype")
+    said(L, L.unit_gated_dense_grad_ws_bytes(1, 1, 4, 2, 16, 16, None), "null")
+    ok = dict(x=16, x_scales=None, x_dtype=1, w=16, dh=16, pre=16, pre_scales=None, pre_dtype=1, sizes=16, size_bytes=4, dx=16, dx_dtype=0, dw=16, dw_dtype=1, dtype=1,
+              act=0, rows=4, groups=2, n=16, k=16, ws=16, bytes=1 << 20, stream=None)
+    call = lambda **change: L.unit_gated_dense_grad(*{**ok, **change}.values())
+    for change, text in ((dict(x=None), "null"), (dict(w=None), "null"), (dict(dh=None), "null"), (dict(ws=None), "null"), (dict(sizes=None), "null"),
+                         (dict(pre=None, x=None, dw=None), "null"), (dict(x_dtype=4), "null"), (dict(pre_dtype=4), "null"), (dict(x_dtype=2), "x_dtype"),
+                         (dict(pre_dtype=2), "pre_dtype"), (dict(dtype=0, x_dtype=0), "dtype"), (dict(dx_dtype=2), "dx"), (dict(dw_dtype=2), "dw"), (dict(act=2), "activation"),
+                         (dict(rows=-1), "negative"), (dict(groups=0), "positive"), (dict(n=12), "multiples of 8"), (dict(k=12), "multiples of 8"), (dict(n=1 << 22), "2^21"),
+                         (dict(n=1 << 16, k=1 << 15), "2^31"), (dict(bytes=100), "needed"), (dict(size_bytes=3), "4- or 8-byte"), (dict(x=8), "aligned"), (dict(w=8), "aligned"),
+                         (dict(dh=8), "aligned"), (dict(pre=8), "aligned"), (dict(dx=8), "aligned"), (dict(dw=8), "aligned"), (dict(ws=8), "aligned")):
         said(L, call(**change), text)
 
 

@@ -339,3 +339,60 @@ def test_refusals(dev):
     ):
         with pytest.raises(error, match=text):
             call()
+
+
+@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5])
+def test_gradients_on_every_tile(dev, tile, monkeypatch):
+    monkeypatch.setenv("UNIT_AMD_GROUPED_TILE", str(tile))
+    for case in ((None, 40, 72, 136), ([70, 0, 300, 33], 7, 328, 200)):
+        x, w, dy, s = operands(case, "float16", dev)
+        _, _, exact, off = forward(x, w, case[0], "silu")
+        got = U.gated_dense_grad(x, w, dy, s, "silu")
+        dx, dxo, dw, dwo = gradients(x, w, dy, case[0], "silu", exact, off + ROUND["float16"] * (exact.abs() + off) + TINY["float16"], "float16")
+        near(got[0], dx, dxo, "float32")
+        near(got[1], dw, dwo, "float32")
+
+
+@pytest.mark.parametrize("rows,sizes", [(3, None), (70, [20, 0, 45])])
+def test_the_python_path_gives_the_native_calls_results(dev, rows, sizes, monkeypatch):
+    from unit_amd import gated as G, grouped
+    x, w, dy, s = operands((sizes, rows - sum(sizes or []), 72, 136), "bfloat16", dev)
+
+    def everything():
+        wq = U.quantize_mxfp4(w)
+        h, pre = U.gated_dense(x, w, s, "gelu_tanh", "bfloat16", keep="pre")
+        _, pre8 = U.gated_dense(x, w, s, "gelu_tanh", "bfloat16", keep="mxfp8")
+        x8 = U.quantize_mxfp8(x)
+        out = [h, pre, U.dequantize_mxfp8(pre8), U.dequantize_mxfp8(x8, "bfloat16"), U.gated_dense(x, w, s), U.gated_dense_mxfp4(x, wq, s, "silu", "float16"),
+               U.gated_dense_mxfp4(U.quantize_mxfp4(x), wq, s)]
+        for data, kept in ((x, pre), (x, None), (x8, pre8), (x8, None)):
+            out += U.gated_dense_grad(data, w, dy, s, "gelu_tanh", kept, "bfloat16", "float32")
+        return out
+
+    native = everything()
+    calls = []
+
+    class Declines:
+        def __getattr__(self, name):
+            return lambda *a: calls.append(name)
+
+    monkeypatch.setattr(G, "_native_gated", Declines())
+    monkeypatch.setattr(grouped, "_native_gated", Declines())
+    for a, b in zip(native, everything()):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+    assert set(calls) == {"quantize8", "dequantize8", "gated", "gated_mx", "gated_grad"}
+
+
+def test_the_common_case_is_native(dev):
+    """Each native call takes the operands that a user's program has, rather than leave them to the Python operator."""
+    from unit_amd.grouped import _native_gated as native
+    x, w, dy, _ = operands((None, 6, 72, 136), "float16", dev)
+    h, pre8 = native.gated(x, w, None, "silu", "float16", "mxfp8")
+    assert h.shape == (6, 72) and pre8.shape == (6, 2, 72)
+    assert native.gated(x, w, None, "silu", "float32", None) is not None and native.gated(x, w, None, "silu", "float32", "pre") is not None
+    x8 = native.quantize8(x)
+    assert native.dequantize8(x8, "float16").shape == x.shape
+    assert native.gated_mx(x, U.quantize_mxfp4(w), None, "silu", "float16").shape == (6, 72)
+    for data, pre in ((x, None), (x8, None), (x, pre8), (x8, pre8)):
+        assert native.gated_grad(data, w, dy, None, "silu", pre, "float16", "float32") is not None
+    assert native.gated(x, w, None, "relu", "float16", None) is None and native.gated(x.float(), w, None, "silu", "float16", None) is None

@@ -63,7 +63,8 @@ SYMBOLS = (
     "unit_grouped_dense_mxfp4",
     "unit_gated_dense",
     "unit_gated_dense_mxfp4",
-    "unit_gate_grad",
+    "unit_gated_dense_grad_ws_bytes",
+    "unit_gated_dense_grad",
     "unit_mxfp8_bytes",
     "unit_quantize_mxfp8",
     "unit_dequantize_mxfp8",
@@ -160,7 +161,8 @@ def load():
     L.unit_grouped_dense_mxfp4.argtypes = [vp, vp, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, vp, size, vp]
     L.unit_gated_dense.argtypes = [vp, vp, vp, i32, vp, i32, i32, i32, vp, vp, i32, i32, i32, i32, i32, vp]
     L.unit_gated_dense_mxfp4.argtypes = [vp, vp, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, size, vp]
-    L.unit_gate_grad.argtypes = [vp, vp, i32, vp, vp, i32, i32, i32, i32, vp]
+    L.unit_gated_dense_grad_ws_bytes.argtypes = [i32, i32, i32, i32, i32, i32, sizep]
+    L.unit_gated_dense_grad.argtypes = [vp, vp, i32, vp, vp, vp, vp, i32, vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, size, vp]
     L.unit_mxfp8_bytes.argtypes = [i64, i32, sizep, sizep]
     L.unit_quantize_mxfp8.argtypes = [vp, i32, i64, i32, vp, vp, vp]
     L.unit_dequantize_mxfp8.argtypes = [vp, vp, i64, i32, vp, i32, vp]

@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -56,7 +57,22 @@ struct GroupedLibrary {
 };
 GroupedLibrary glib;
 constexpr int kGroupedFunctions = sizeof(GroupedLibrary) / sizeof(void *);
-PyObject *mx_type, *n_shape;  // grouped.Mxfp4Tensor
+
+// those of the gated products and of MXFP8 (bind_gated)
+struct GatedLibrary {
+  decltype(&unit_mxfp4_bytes) mx_bytes;
+  decltype(&unit_mxfp4_workspace_bytes) mx_workspace;
+  decltype(&unit_mxfp8_bytes) mx8_bytes;
+  decltype(&unit_quantize_mxfp8) quantize8;
+  decltype(&unit_dequantize_mxfp8) dequantize8;
+  decltype(&unit_gated_dense) gated;
+  decltype(&unit_gated_dense_mxfp4) gated_mx;
+  decltype(&unit_gated_dense_grad_ws_bytes) grad_workspace;
+  decltype(&unit_gated_dense_grad) grad;
+};
+GatedLibrary tlib;
+constexpr int kGatedFunctions = sizeof(GatedLibrary) / sizeof(void *);
+PyObject *mx_type, *mx8_type, *n_shape;  // grouped.Mxfp4Tensor, grouped.Mxfp8Tensor
 
 // ops.PreparedConvWeight, PreparedDenseWeight, PreparedGemmB; torch.int8, torch.float16
 PyObject *conv_weight_type, *dense_weight_type, *gemm_b_type, *dtype_s8, *dtype_f16;
@@ -393,7 +409,7 @@ const at::Tensor *floats(PyObject *o, int *code) {
   return *code >= 0 ? operand(o, t.scalar_type(), (int)t.dim()) : nullptr;
 }
 
-// an Mxfp4Tensor: its buffer, sizes of its shape (dims of them) and its rows
+// an Mxfp4Tensor or Mxfp8Tensor: its buffer, sizes of its shape (dims of them) and its rows
 struct Mx {
   at::Tensor buf;
   int64_t size[3], rows;
@@ -401,8 +417,8 @@ struct Mx {
   size_t codes;  // bytes before the scales
   char *data() const { return static_cast<char *>(buf.data_ptr()); }
 };
-bool mx_operand(PyObject *o, Mx *q) {
-  if ((PyObject *)Py_TYPE(o) != mx_type) return false;
+bool mx_operand(PyObject *o, Mx *q, PyObject *kind, decltype(&unit_mxfp4_bytes) bytes) {
+  if ((PyObject *)Py_TYPE(o) != kind) return false;
   PyObject *shape = PyObject_GetAttr(o, n_shape);
   if (!shape) return PyErr_Clear(), false;
   bool ok = PyTuple_CheckExact(shape) && PyTuple_GET_SIZE(shape) >= 2 && PyTuple_GET_SIZE(shape) <= 3;
@@ -419,11 +435,12 @@ bool mx_operand(PyObject *o, Mx *q) {
   if (!buf) return PyErr_Clear(), false;
   const at::Tensor *t = operand(buf, at::kByte, 1);
   size_t scales;
-  ok = t && glib.mx_bytes(q->rows, (int32_t)q->size[q->dims - 1], &q->codes, &scales) == UNIT_OK && (size_t)t->numel() >= q->codes + scales;
+  ok = t && bytes(q->rows, (int32_t)q->size[q->dims - 1], &q->codes, &scales) == UNIT_OK && (size_t)t->numel() >= q->codes + scales;
   if (ok) q->buf = *t;
   Py_DECREF(buf);
   return ok;
 }
+bool mx_operand(PyObject *o, Mx *q) { return mx_operand(o, q, mx_type, glib.mx_bytes); }
 
 template <class F>
 int without_gil(F &&call) {
@@ -566,6 +583,225 @@ PyObject *grouped_grad(PyObject *const *a, Py_ssize_t n) {
   return both;
 }
 
+// ------------------------------------------------------------------------------- gated products and MXFP8
+// work goes to the current device's stream: operands that live on another device are the Python operator's
+bool here(const at::Tensor &t) { return t.device().index() == c10::hip::current_device(); }
+
+// an empty Mxfp8Tensor; its codes and scales
+PyObject *mx8_empty(const at::Tensor &like, at::IntArrayRef shape, char **codes, char **scales) {
+  int64_t rows = 1;
+  for (size_t i = 0; i + 1 < shape.size(); ++i) rows *= shape[i];
+  size_t c, s;
+  if (tlib.mx8_bytes(rows, (int32_t)shape.back(), &c, &s) != UNIT_OK) return nullptr;
+  at::Tensor buf = result(like, {(int64_t)(c + s)}, at::kByte);
+  *codes = static_cast<char *>(buf.data_ptr());
+  *scales = *codes + c;
+  PyObject *sizes = PyTuple_New((Py_ssize_t)shape.size());
+  for (size_t i = 0; sizes && i < shape.size(); ++i) PyTuple_SET_ITEM(sizes, (Py_ssize_t)i, PyLong_FromLongLong(shape[i]));
+  PyObject *b = THPVariable_Wrap(std::move(buf));
+  PyObject *q = sizes && b ? PyObject_CallFunctionObjArgs(mx8_type, b, sizes, nullptr) : nullptr;
+  Py_XDECREF(sizes);
+  Py_XDECREF(b);
+  if (!q) throw std::bad_alloc();
+  return q;
+}
+
+bool mx8_operand(PyObject *o, Mx *q) { return mx_operand(o, q, mx8_type, tlib.mx8_bytes) && here(q->buf); }
+
+PyObject *pair_of(PyObject *first, PyObject *second) {
+  PyObject *both = first && second ? PyTuple_New(2) : nullptr;
+  if (!both) {
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    throw std::bad_alloc();
+  }
+  PyTuple_SET_ITEM(both, 0, first);
+  PyTuple_SET_ITEM(both, 1, second);
+  return both;
+}
+
+// (x)
+PyObject *quantize8(PyObject *const *a, Py_ssize_t n) {
+  int code;
+  const at::Tensor *x = n == 1 ? floats(a[0], &code) : nullptr;
+  if (!x || x->dim() < 2 || x->dim() > 3 || !small(*x) || !here(*x)) Py_RETURN_NONE;
+  char *codes, *scales;
+  PyObject *q = mx8_empty(*x, x->sizes(), &codes, &scales);
+  if (!q) Py_RETURN_NONE;
+  const int32_t k = (int32_t)x->size(-1);
+  const int64_t rows = k ? x->numel() / k : 0;
+  void *s = stream(), *src = x->data_ptr();
+  if (without_gil([&] { return tlib.quantize8(src, code, rows, k, codes, scales, s); }) == UNIT_OK) return q;
+  Py_DECREF(q);
+  Py_RETURN_NONE;
+}
+
+// (q, out_dtype)
+PyObject *dequantize8(PyObject *const *a, Py_ssize_t n) {
+  Mx q;
+  at::ScalarType type;
+  if (n != 2 || !mx8_operand(a[0], &q) || !out_type(a[1], &type)) Py_RETURN_NONE;
+  at::Tensor out = result(q.buf, at::IntArrayRef(q.size, q.dims), type);
+  void *s = stream(), *dst = out.data_ptr();
+  char *src = q.data();
+  if (without_gil([&] { return tlib.dequantize8(src, src + q.codes, q.rows, (int32_t)q.size[q.dims - 1], dst, float_code(type), s); }) != UNIT_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+bool activation(PyObject *o, int *code) {
+  if (!PyUnicode_CheckExact(o)) return false;
+  if (PyUnicode_CompareWithASCIIString(o, "silu") == 0) return *code = UNIT_SILU, true;
+  if (PyUnicode_CompareWithASCIIString(o, "gelu_tanh") == 0) return *code = UNIT_GELU_TANH, true;
+  return false;
+}
+
+// the weight of a gated product, (2 N, K), or (E, 2 N, K) with group sizes; rows: of the data, (rows, K)
+struct Gated {
+  const at::Tensor *w, *sizes = nullptr;
+  void *groups_at = nullptr;
+  int32_t rows, groups = 1, cols, k;
+  int width = 4;
+  bool take(const at::Tensor &weight_of, int64_t r, int64_t both, int64_t kk, int64_t lead, PyObject *group) {
+    if (both % 2 || r > INT_MAX) return false;
+    rows = (int32_t)r, cols = (int32_t)(both / 2), k = (int32_t)kk, groups = (int32_t)lead;
+    if (group == Py_None) return true;
+    sizes = group_sizes(group, lead, weight_of);
+    if (!sizes) return false;
+    groups_at = sizes->data_ptr();
+    width = (int)sizes->element_size();
+    return true;
+  }
+  bool operands(PyObject *weight, at::ScalarType type, PyObject *group) {
+    const bool grouped = group != Py_None;
+    w = operand(weight, type, grouped ? 3 : 2);
+    return w && small(*w) && here(*w) && take(*w, 0, w->size(-2), w->size(-1), grouped ? w->size(0) : 1, group);
+  }
+};
+
+// (data, weight, group sizes or None, activation, out_dtype, keep)
+PyObject *gated(PyObject *const *a, Py_ssize_t n) {
+  Gated g;
+  at::ScalarType type;
+  int code, act;
+  const at::Tensor *x = n == 6 ? floats(a[0], &code) : nullptr;
+  if (!x || code == UNIT_F32 || x->dim() != 2 || !small(*x) || !g.operands(a[1], x->scalar_type(), a[2]) || !activation(a[3], &act) || !out_type(a[4], &type) ||
+      x->size(1) != g.k || x->device() != g.w->device())
+    Py_RETURN_NONE;
+  g.rows = (int32_t)x->size(0);
+  int keep = 0;
+  if (a[5] != Py_None) {
+    if (!PyUnicode_CheckExact(a[5])) Py_RETURN_NONE;
+    keep = PyUnicode_CompareWithASCIIString(a[5], "pre") == 0 ? 1 : PyUnicode_CompareWithASCIIString(a[5], "mxfp8") == 0 ? 2 : 3;
+    if (keep == 3) Py_RETURN_NONE;
+  }
+  at::Tensor out = result(*x, {g.rows, g.cols}, type), pre;
+  char *kept = nullptr, *scales = nullptr;
+  PyObject *q = nullptr;
+  if (keep == 1) {
+    pre = result(*x, {g.rows, 2, g.cols}, x->scalar_type());
+    kept = static_cast<char *>(pre.data_ptr());
+  } else if (keep == 2 && !(q = mx8_empty(*x, {g.rows, 2, g.cols}, &kept, &scales))) {
+    Py_RETURN_NONE;
+  }
+  void *s = stream(), *xp = x->data_ptr(), *wp = g.w->data_ptr(), *o = out.data_ptr();
+  const int rc = without_gil([&] {
+    return tlib.gated(xp, wp, g.groups_at, g.width, o, code, float_code(type), act, kept, scales, keep == 2 ? (int)UNIT_MXFP8 : code, g.rows, g.groups, g.cols, g.k, s);
+  });
+  if (rc != UNIT_OK) {
+    Py_XDECREF(q);
+    Py_RETURN_NONE;
+  }
+  PyObject *h = THPVariable_Wrap(std::move(out));
+  if (!keep) return h;
+  return pair_of(h, q ? q : THPVariable_Wrap(std::move(pre)));
+}
+
+// (data, weight, group sizes or None, activation, out_dtype)
+PyObject *gated_mx(PyObject *const *a, Py_ssize_t n) {
+  Mx w, q;
+  Gated g;
+  at::ScalarType type;
+  int act;
+  if (n != 5 || !mx_operand(a[1], &w, mx_type, tlib.mx_bytes) || !here(w.buf) || !activation(a[3], &act) || !out_type(a[4], &type)) Py_RETURN_NONE;
+  if (w.dims != (a[2] == Py_None ? 2 : 3)) Py_RETURN_NONE;
+  int code;
+  const at::Tensor *x = floats(a[0], &code);
+  const int64_t k = w.size[w.dims - 1];
+  size_t need = 0;
+  at::Tensor ws;
+  void *xp, *xsp = nullptr;
+  int64_t rows;
+  if (x) {
+    if (x->dim() != 2 || !small(*x) || x->size(1) != k) Py_RETURN_NONE;
+    rows = x->size(0);
+    if (tlib.mx_workspace((int32_t)rows, (int32_t)k, &need) != UNIT_OK) Py_RETURN_NONE;
+    ws = result(*x, {(int64_t)need}, at::kByte);
+    xp = x->data_ptr();
+  } else {
+    code = UNIT_MXFP4;
+    if (!mx_operand(a[0], &q, mx_type, tlib.mx_bytes) || q.dims != 2 || q.size[1] != k) Py_RETURN_NONE;
+    x = &q.buf;
+    rows = q.rows;
+    xp = q.data();
+    xsp = q.data() + q.codes;
+  }
+  if (x->device() != w.buf.device() || !g.take(w.buf, rows, w.size[w.dims - 2], k, w.dims == 3 ? w.size[0] : 1, a[2])) Py_RETURN_NONE;
+  at::Tensor out = result(*x, {g.rows, g.cols}, type);
+  void *s = stream(), *o = out.data_ptr(), *wsp = need ? ws.data_ptr() : nullptr;
+  char *wp = w.data();
+  const int rc = without_gil([&] {
+    return tlib.gated_mx(xp, xsp, code, wp, wp + w.codes, g.groups_at, g.width, o, float_code(type), act, g.rows, g.groups, g.cols, g.k, wsp, need, s);
+  });
+  if (rc != UNIT_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// rows or pre-activations of a gradient: a tensor of `type`, or MXFP8
+struct Kept {
+  Mx q;
+  const at::Tensor *t = nullptr;
+  void *at = nullptr, *scales = nullptr;
+  int code = 0;
+  // sizes: what it has to have
+  bool take(PyObject *o, at::ScalarType type, at::IntArrayRef sizes) {
+    if (mx8_operand(o, &q)) {
+      if (!at::IntArrayRef(q.size, q.dims).equals(sizes)) return false;
+      at = q.data(), scales = q.data() + q.codes, code = UNIT_MXFP8, t = &q.buf;
+      return true;
+    }
+    t = operand(o, type, (int)sizes.size());
+    if (!t || !t->sizes().equals(sizes)) return false;
+    at = t->data_ptr(), code = float_code(type);
+    return true;
+  }
+};
+
+// (data, weight, grad, group sizes or None, activation, pre or None, out_dtype, weight_out_dtype)
+PyObject *gated_grad(PyObject *const *a, Py_ssize_t n) {
+  Gated g;
+  Kept x, pre;
+  at::ScalarType type, wtype;
+  int code, act;
+  const at::Tensor *dh = n == 8 ? floats(a[2], &code) : nullptr;
+  if (!dh || code == UNIT_F32 || dh->dim() != 2 || !small(*dh) || !g.operands(a[1], dh->scalar_type(), a[3]) || dh->device() != g.w->device() || dh->size(1) != g.cols ||
+      !activation(a[4], &act) || !out_type(a[6], &type) || !out_type(a[7], &wtype))
+    Py_RETURN_NONE;
+  g.rows = (int32_t)dh->size(0);
+  if (!x.take(a[0], dh->scalar_type(), {g.rows, g.k}) || x.t->device() != g.w->device()) Py_RETURN_NONE;
+  if (a[5] != Py_None && (!pre.take(a[5], dh->scalar_type(), {g.rows, 2, g.cols}) || pre.t->device() != g.w->device())) Py_RETURN_NONE;
+  size_t need;
+  if (tlib.grad_workspace(x.code, code, g.rows, g.groups, g.cols, g.k, &need) != UNIT_OK) Py_RETURN_NONE;
+  at::Tensor ws = result(*dh, {(int64_t)need}, at::kByte), dx = result(*dh, {g.rows, g.k}, type), dw = result(*dh, g.w->sizes(), wtype);
+  void *s = stream(), *wp = g.w->data_ptr(), *hp = dh->data_ptr(), *dxp = dx.data_ptr(), *dwp = dw.data_ptr(), *wsp = ws.data_ptr();
+  const int rc = without_gil([&] {
+    return tlib.grad(x.at, x.scales, x.code, wp, hp, pre.at, pre.scales, pre.code, g.groups_at, g.width, dxp, float_code(type), dwp, float_code(wtype), code, act, g.rows,
+                     g.groups, g.cols, g.k, wsp, need, s);
+  });
+  if (rc != UNIT_OK) Py_RETURN_NONE;
+  PyObject *first = THPVariable_Wrap(std::move(dx));
+  return pair_of(first, THPVariable_Wrap(std::move(dw)));
+}
+
 // `addresses`, a tuple of `count` of them
 bool take_addresses(PyObject *addresses, int count, void **f) {
   if (!PyTuple_CheckExact(addresses) || PyTuple_GET_SIZE(addresses) != count) {
@@ -597,6 +833,24 @@ PyObject *bind_grouped(PyObject *, PyObject *const *a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// (addresses in GatedLibrary's order, Mxfp4Tensor, Mxfp8Tensor)
+PyObject *bind_gated(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  void *f[kGatedFunctions];
+  if (n != 3) {
+    PyErr_SetString(PyExc_ValueError, "bind: unexpected arguments");
+    return nullptr;
+  }
+  if (!take_addresses(a[0], kGatedFunctions, f)) return nullptr;
+  memcpy(&tlib, f, sizeof tlib);
+  PyObject **const kept[] = {&mx_type, &mx8_type};
+  for (int i = 0; i < 2; ++i) {
+    Py_INCREF(a[i + 1]);
+    Py_XDECREF(*kept[i]);
+    *kept[i] = a[i + 1];
+  }
+  Py_RETURN_NONE;
+}
+
 // (addresses in Library's order, the three prepared classes, torch.int8, torch.float16)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   void *f[kFunctions];
@@ -625,6 +879,8 @@ PyMethodDef methods[] = {
     method<conv_f16>("conv_f16"), method<dense>("dense"),           method<gemm>("gemm"),
     method<quantize>("quantize"), method<dequantize>("dequantize"), method<product_mx>("product_mx"),     method<grouped>("grouped"),
     method<grouped_grad>("grouped_grad"),
+    method<quantize8>("quantize8"), method<dequantize8>("dequantize8"), method<gated>("gated"), method<gated_mx>("gated_mx"), method<gated_grad>("gated_grad"),
+    {"bind_gated", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind_gated)), METH_FASTCALL, nullptr},
     {"bind_grouped", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind_grouped)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -116,7 +116,7 @@ extern "C" int unit_gated_dense(const void *x, const void *w, const void *sizes,
   if (int rc = check_device()) return rc;
   if (!rows) return UNIT_OK;
   GatedParams p{{static_cast<const char *>(x), static_cast<const char *>(w), nullptr, nullptr, static_cast<char *>(out), sizes, size_bytes, groups, rows, N, K},
-                act, static_cast<char *>(pre), static_cast<char *>(pre_scales)};
+                act, static_cast<char *>(pre), static_cast<char *>(pre_scales), nullptr};
   return (dtype == UNIT_F16 ? run_gated_f16 : run_gated_bf16)(what, gate, p, out_dtype, static_cast<hipStream_t>(stream));
 }
 
@@ -128,29 +128,78 @@ extern "C" int unit_gated_dense_mxfp4(const void *x, const void *xscales, int32_
   if (int rc = check_activation(what, activation, &act)) return rc;
   if (int rc = check_gated(what, sizes, size_bytes, rows, groups, N, K, N > 0 && K > 0 ? mx_code_bytes(2l * N, K) : 0)) return rc;
   GatedParams p{{static_cast<const char *>(x), static_cast<const char *>(wcodes), static_cast<const u32 *>(xscales), static_cast<const u32 *>(wscales),
-                 static_cast<char *>(out), sizes, size_bytes, groups, rows, N, K, x_dtype}, act, nullptr, nullptr};
+                 static_cast<char *>(out), sizes, size_bytes, groups, rows, N, K, x_dtype}, act, nullptr, nullptr, nullptr};
   bool run;
   if (int rc = mxfp4_rows(what, &p, out_dtype, ws, ws_bytes, static_cast<hipStream_t>(stream), [](const GroupedParams &) { return false; }, &run)) return rc;
   return run ? run_gated_mx(what, p, out_dtype, static_cast<hipStream_t>(stream)) : UNIT_OK;
 }
 
-extern "C" int unit_gate_grad(const void *pre, const void *pre_scales, int32_t pre_dtype, const void *dh, void *dpre, int32_t dtype, int32_t activation, int32_t rows,
-                              int32_t N, unit_stream_t stream) {
-  const char *what = "unit_gate_grad";
+namespace {
+
+// The parts of the workspace of a gradient: dpre, the rows restored from MXFP8
+struct GradParts {
+  size_t dpre, x;
+  GradParts(int x_dtype, int rows, int N, int K) : dpre(((size_t)rows * N * 4 + 255) / 256 * 256), x(x_dtype == UNIT_MXFP8 ? (size_t)rows * K * 2 : 0) {}
+};
+
+int check_grad_shape(const char *what, int x_dtype, int dtype, int rows, int groups, int N, int K) {
+  if (dtype != UNIT_F16 && dtype != UNIT_BF16) return fail(UNIT_E_ARG, "%s: dtype must be UNIT_F16 or UNIT_BF16, got %d", what, dtype);
+  if (x_dtype != dtype && x_dtype != UNIT_MXFP8) return fail(UNIT_E_ARG, "%s: x_dtype must be dtype or UNIT_MXFP8, got %d", what, x_dtype);
+  const int unused = 0;
+  if (int rc = check_gated(what, &unused, 4, rows, groups, N, K, N > 0 && K > 0 ? (size_t)N * K * 4 : 0)) return rc;
+  return check_f16(what, N, K);
+}
+
+}  // namespace
+
+extern "C" int unit_gated_dense_grad_ws_bytes(int32_t x_dtype, int32_t dtype, int32_t rows, int32_t groups, int32_t N, int32_t K, size_t *bytes) {
+  const char *what = "unit_gated_dense_grad_ws_bytes";
+  if (int rc = check_grad_shape(what, x_dtype, dtype, rows, groups, N, K)) return rc;
+  if (!bytes) return fail(UNIT_E_ARG, "%s: null pointer", what);
+  const GradParts parts(x_dtype, rows, N, K);
+  *bytes = parts.dpre + parts.x;
+  return UNIT_OK;
+}
+
+extern "C" int unit_gated_dense_grad(const void *x, const void *x_scales, int32_t x_dtype, const void *w, const void *dh, const void *pre, const void *pre_scales,
+                                     int32_t pre_dtype, const void *sizes, int32_t size_bytes, void *dx, int32_t dx_dtype, void *dw, int32_t dw_dtype, int32_t dtype,
+                                     int32_t activation, int32_t rows, int32_t groups, int32_t N, int32_t K, void *ws, size_t ws_bytes, unit_stream_t stream) {
+  const char *what = "unit_gated_dense_grad";
   Activation act;
-  if (int rc = check_types(what, dtype, dtype)) return rc;
+  if (int rc = check_grad_shape(what, x_dtype, dtype, rows, groups, N, K)) return rc;
+  if (int rc = check_groups(what, sizes, size_bytes, rows, groups, N, K, 0)) return rc;
   if (int rc = check_activation(what, activation, &act)) return rc;
-  if (pre_dtype != dtype && pre_dtype != UNIT_MXFP8) return fail(UNIT_E_ARG, "%s: pre_dtype must be dtype or UNIT_MXFP8, got %d", what, pre_dtype);
-  if (rows < 0 || N <= 0 || N % 8) return fail(UNIT_E_ARG, "%s: rows must not be negative and N a positive multiple of 8", what);
-  if (rows > 1 << 30 || N > 1 << 21) return fail(UNIT_E_ARG, "%s: sizes beyond 2^30 rows or 2^21 columns", what);
-  if (int rc = check_ptrs(what, rows, {pre, dh, dpre})) return rc;
-  if (pre_dtype == UNIT_MXFP8 && rows && !pre_scales) return fail(UNIT_E_ARG, "%s: null pointer", what);
+  if (dx && dx_dtype != UNIT_F32 && dx_dtype != dtype) return fail(UNIT_E_ARG, "%s: out_dtype of dx must be UNIT_F32 or dtype, got %d", what, dx_dtype);
+  if (dw && dw_dtype != UNIT_F32 && dw_dtype != dtype) return fail(UNIT_E_ARG, "%s: out_dtype of dw must be UNIT_F32 or dtype, got %d", what, dw_dtype);
+  if (pre && pre_dtype != dtype && pre_dtype != UNIT_MXFP8) return fail(UNIT_E_ARG, "%s: pre_dtype must be dtype or UNIT_MXFP8, got %d", what, pre_dtype);
+  const bool needs_x = dw || !pre, x8 = x_dtype == UNIT_MXFP8;
+  const GradParts parts(x_dtype, rows, N, K);
+  if (int rc = check_ptrs(what, rows, {w, dh, ws})) return rc;
+  if (int rc = check_ptrs(what, rows && needs_x, {x})) return rc;
+  if (int rc = check_aligned(what, {pre, dx, dw})) return rc;
+  if (rows && ((x8 && needs_x && !x_scales) || (pre && pre_dtype == UNIT_MXFP8 && !pre_scales))) return fail(UNIT_E_ARG, "%s: null pointer", what);
+  if (ws_bytes < parts.dpre + parts.x) return fail(UNIT_E_ARG, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, parts.dpre + parts.x);
   if (int rc = check_device()) return rc;
-  if (!rows) return UNIT_OK;
+  if (!dx && !dw) return UNIT_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == UNIT_F16)
-    return pre_dtype == UNIT_MXFP8 ? run_gate_grad<_Float16, true>(what, pre, pre_scales, dh, dpre, rows, N, act, s)
-                                   : run_gate_grad<_Float16, false>(what, pre, pre_scales, dh, dpre, rows, N, act, s);
-  return pre_dtype == UNIT_MXFP8 ? run_gate_grad<__bf16, true>(what, pre, pre_scales, dh, dpre, rows, N, act, s)
-                                 : run_gate_grad<__bf16, false>(what, pre, pre_scales, dh, dpre, rows, N, act, s);
+  char *const dpre = static_cast<char *>(ws);
+  if (x8 && needs_x && rows) {
+    if (int rc = unit_dequantize_mxfp8(x, x_scales, rows, K, dpre + parts.dpre, dtype, stream)) return rc;
+    x = dpre + parts.dpre;
+  }
+  if (rows && pre) {
+    const bool pre8 = pre_dtype == UNIT_MXFP8;
+    const int rc = dtype == UNIT_F16 ? (pre8 ? run_gate_grad<_Float16, true> : run_gate_grad<_Float16, false>)(what, pre, pre_scales, dh, dpre, rows, N, act, s)
+                                     : (pre8 ? run_gate_grad<__bf16, true> : run_gate_grad<__bf16, false>)(what, pre, pre_scales, dh, dpre, rows, N, act, s);
+    if (rc) return rc;
+  } else if (rows) {
+    GatedParams p{{static_cast<const char *>(x), static_cast<const char *>(w), nullptr, nullptr, dpre, sizes, size_bytes, groups, rows, N, K},
+                  act, nullptr, nullptr, static_cast<const char *>(dh)};
+    if (int rc = (dtype == UNIT_F16 ? run_gated_f16 : run_gated_bf16)(what, GATE_GRAD, p, dtype, s)) return rc;
+  }
+  if (dx)
+    if (int rc = unit_grouped_dense_grad_data(dpre, w, sizes, size_bytes, dx, dtype, dx_dtype, rows, groups, 2 * N, K, stream)) return rc;
+  if (dw)
+    if (int rc = unit_grouped_dense_grad_weight(x, dpre, sizes, size_bytes, dw, dtype, dw_dtype, rows, groups, 2 * N, K, stream)) return rc;
+  return UNIT_OK;
 }

@@ -41,10 +41,12 @@ struct GatedParams : GroupedParams {
   Activation act;
   char *pre;         // kept pre-activations (rows, 2, N): the operands' type, or MXFP8 codes
   char *pre_scales;  // MXFP8
+  const char *dh;    // GATE_GRAD: h's gradient (rows, N), of the operands' type
 };
 
-// What a kernel of the gated product writes besides h: nothing, the pre-activations in the operands' type, or in MXFP8
-enum Gate { GATE_NONE, GATE_ONLY, GATE_KEEP, GATE_KEEP8 };
+// What a kernel of the gated product writes: h, h and the pre-activations in the operands' type, h and them in MXFP8, or the gate's gradients
+// dpre (rows, 2, N) in the place of h
+enum Gate { GATE_NONE, GATE_ONLY, GATE_KEEP, GATE_KEEP8, GATE_GRAD };
 
 // what a kernel of the product takes.  (The enumeration has a name and the condition none of it: in a kernel's mangled name an unnamed type is
 // counted, and the host's count differs from the device's.)

@@ -4,7 +4,7 @@
 namespace unit {
 
 int run_gated_f16(const char *what, int gate, const GatedParams &p, int out_dtype, hipStream_t s) {
-  return out_dtype == UNIT_F32 ? run_gated_gate<OpHalf, float>(what, gate, "f16gated", p, s) : run_gated_gate<OpHalf, _Float16>(what, gate, "f16gated", p, s);
+  return out_dtype == UNIT_F32 && gate != GATE_GRAD ? run_gated_gate<OpHalf, float>(what, gate, "f16gated", p, s) : run_gated_gate<OpHalf, _Float16>(what, gate, "f16gated", p, s);
 }
 
 }  // namespace unit

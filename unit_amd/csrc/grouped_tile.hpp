@@ -279,6 +279,49 @@ __device__ __forceinline__ void put_mx8(char *rows, char *codes, char *scales, i
   }
 }
 
+// The gate's gradients of a wave: dg = dh u act'(g), du = dh act(g), of the same sums that h is made of.  dh comes in runs of 16 bytes a lane,
+// all of them asked for at once, and goes through the wave's LDS into the accumulators' order.
+template <class T, class Half, class Acc>
+__device__ __forceinline__ void gated_gradients(const GatedParams &p, char *rows, const Acc &acc, int blocks, long row0, int x0, int high, int y) {
+  constexpr int CB = T::TY / 2, PITCH = CB * 64 + 16, RUNS = CB * 4, LOADS = 32 * RUNS / 64;
+  typedef Half v4e __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
+  v4u d[T::TX][LOADS];
+#pragma unroll
+  for (int i = 0; i < T::TX; ++i)
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+      const int row = (k * 64 + lane) / RUNS, c = (k * 64 + lane) % RUNS * 8;
+      d[i][k] = v4u{0, 0, 0, 0};
+      if (i < blocks && row < high - x0 - i * 32 && y + c < p.n)  // N is a multiple of 8: eight columns are there or not
+        d[i][k] = *reinterpret_cast<const v4u *>(p.dh + ((row0 + x0 + i * 32 + row) * p.n + y + c) * 2);
+    }
+#pragma unroll
+  for (int i = 0; i < T::TX; ++i) {
+    if (i >= blocks) break;
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) *reinterpret_cast<v4u *>(rows + (k * 64 + lane) / RUNS * PITCH + (k * 64 + lane) % RUNS * 16) = d[i][k];
+    v4f dg[CB][4], du[CB][4];
+#pragma unroll
+    for (int j = 0; j < CB; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const v4e dh = *reinterpret_cast<const v4e *>(rows + l32 * PITCH + (j * 32 + 8 * r + 4 * half) * 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float slope;
+          const float a = act_both(p.act, acc[i][j][4 * r + e], &slope), f = (float)dh[e];
+          dg[j][r][e] = f * acc[i][j + CB][4 * r + e] * slope;
+          du[j][r][e] = f * a;
+        }
+      }
+    char *dst = p.out + (row0 + x0 + i * 32) * 2 * p.n * 2;
+    const int left = high - x0 - i * 32;
+    RowsOut<Half, CB>::put(rows, dst, 2l * p.n, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) { return dg[j][r]; });
+    RowsOut<Half, CB>::put(rows, dst + 2l * p.n, 2l * p.n, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) { return du[j][r]; });
+  }
+}
+
 // A wave's results of a gated product: acc[i][j] holds gate x, acc[i][j + TY / 2] up x.  The activation is of the sums in fp32; h and what
 // is kept are rounded from them once each.
 template <class T, int GATE, class Half, class Out, class Acc>
@@ -583,7 +626,11 @@ __device__ __forceinline__ void compute_tile(const GateParams<GATE> &p, char *ld
     constexpr int PITCH = RowsOut<float, T::TY / 2>::PITCH;  // of the widest
     static_assert(NW * 32 * PITCH <= NSTAGE * STAGE, "the waves' rows fit the ring");
     __syncthreads();  // the ring is read out
-    gated_results<T, GATE, typename Op::half_t, Out>(p, lds + wave * (32 * PITCH), acc, blocks_x, (long)first + x0, block0 * 32, high, y0 + wy * WCOLS);
+    char *const rows = lds + wave * (32 * PITCH);
+    if constexpr (GATE == GATE_GRAD)
+      gated_gradients<T, Out>(p, rows, acc, blocks_x, (long)first + x0, block0 * 32, high, y0 + wy * WCOLS);
+    else
+      gated_results<T, GATE, typename Op::half_t, Out>(p, rows, acc, blocks_x, (long)first + x0, block0 * 32, high, y0 + wy * WCOLS);
     return;
   }
   constexpr int ES_OUT = (int)sizeof(Out), PITCH = T::TY * 32 * ES_OUT + 16, PER = 16 / ES_OUT, RUNS = T::TY * 32 / PER;  // elements per run, runs per row

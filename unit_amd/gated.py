@@ -13,9 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .grouped import (_CODE, _HALVES, _MXFP4, _MXFP8, _NAME, Mxfp8Tensor, _floats, _mxfp4, _mxfp8_empty, _on, _out_dtype, _product_grads, _same_device, _sizes,
-                      dequantize_mxfp8)
-from .grouped import Mxfp4Tensor
+from .grouped import _CODE, _HALVES, _MXFP4, _MXFP8, Mxfp4Tensor, Mxfp8Tensor, _floats, _mxfp4, _mxfp8_empty, _native_gated, _on, _out_dtype, _same_device, _sizes
 from .ops import _dev, _stream
 
 __all__ = ["gated_dense", "gated_dense_mxfp4", "gated_dense_grad"]
@@ -68,6 +66,9 @@ def gated_dense(data, weight, group_sizes=None, activation="silu", out_dtype="fl
     activation "silu", z / (1 + exp(-z)), or "gelu_tanh", z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2.
     keep: what comes back beside out for gated_dense_grad's `pre`, gate . data[r] and up . data[r] as (rows, 2, N): "pre" a tensor of
     data's type, "mxfp8" an Mxfp8Tensor, a quarter of a float32's size; None nothing, and out alone is returned."""
+    done = _native_gated.gated(data, weight, group_sizes, activation, out_dtype, keep)
+    if done is not None:
+        return done
     act, dt = _activation(activation), _out_dtype(out_dtype)
     if keep not in (None, "pre", "mxfp8"):
         raise ValueError(f"keep: expected None, 'pre' or 'mxfp8', got {keep!r}")
@@ -101,6 +102,9 @@ def _forward(data, weight, sizes, act, shape, out, keep):
 def gated_dense_mxfp4(data, weight, group_sizes=None, activation="silu", out_dtype="float32"):
     """gated_dense with MXFP4 operands: data (rows, K) float32, float16 or bfloat16, quantised on the way as quantize_mxfp4 does, or an
     Mxfp4Tensor; weight an Mxfp4Tensor (2 N, K), with group_sizes (E, 2 N, K); N and K of any size."""
+    out = _native_gated.gated_mx(data, weight, group_sizes, activation, out_dtype)
+    if out is not None:
+        return out
     act, dt = _activation(activation), _out_dtype(out_dtype)
     ndim = 2 if group_sizes is None else 3
     if len(_mxfp4(weight, "weight").shape) != ndim:
@@ -137,7 +141,8 @@ def gated_dense_grad(data, weight, grad, group_sizes=None, activation="silu", pr
     data as in gated_dense, or an Mxfp8Tensor of it; pre what gated_dense kept (either form), or None: the pre-activations are then
     computed from data again.  The gate's own gradients, grad * up * act'(gate) and grad * act(gate), are computed in float32 and
     rounded to weight's type, which the products after them take; those sum in float32 and round once."""
-    return _gated_grad(data, weight, grad, group_sizes, activation, pre, out_dtype, weight_out_dtype)
+    both = _native_gated.gated_grad(data, weight, grad, group_sizes, activation, pre, out_dtype, weight_out_dtype)
+    return _gated_grad(data, weight, grad, group_sizes, activation, pre, out_dtype, weight_out_dtype) if both is None else both
 
 
 def _gated_grad(data, weight, grad, group_sizes, activation, pre, out_dtype, weight_out_dtype, wanted=(True, True)):
@@ -154,12 +159,16 @@ def _gated_grad(data, weight, grad, group_sizes, activation, pre, out_dtype, wei
         if tuple(pre.shape) != (rows, 2, n):
             raise ValueError(f"pre: expected ({rows}, 2, {n}), got {tuple(pre.shape)}")
         _same_device(pre, "pre", weight)
+    L, code = _lib.load(), _CODE[weight.dtype]
+    x = (*data._pointers()[:2], _MXFP8) if isinstance(data, Mxfp8Tensor) else (data.data_ptr(), None, code)
+    kept = (None, None, 0) if pre is None else (*pre._pointers()[:2], _MXFP8) if isinstance(pre, Mxfp8Tensor) else (pre.data_ptr(), None, code)
+    need = ctypes.c_size_t()
+    check(L.unit_gated_dense_grad_ws_bytes(x[2], code, rows, e, n, k, ctypes.byref(need)))
     with _on(weight):
-        if isinstance(data, Mxfp8Tensor) and (wanted[1] or pre is None):
-            data = dequantize_mxfp8(data, _NAME[weight.dtype])
-        if pre is None:
-            pre = _forward(data, weight, sizes, act, (rows, e, n, k), torch.empty((rows, n), dtype=weight.dtype, device=weight.device), "pre")
-        kept = (*pre._pointers()[:2], _MXFP8) if isinstance(pre, Mxfp8Tensor) else (pre.data_ptr(), None, _CODE[pre.dtype])
-        dpre = torch.empty((rows, 2 * n), dtype=weight.dtype, device=weight.device)
-        check(_lib.load().unit_gate_grad(*kept, grad.data_ptr(), dpre.data_ptr(), _CODE[weight.dtype], act, rows, n, _stream()))
-        return _product_grads(data, weight, dpre, sizes, (rows, e, 2 * n, k), dt, wdt, wanted)
+        ws = torch.empty((need.value,), dtype=torch.uint8, device=weight.device)
+        ddata = torch.empty((rows, k), dtype=dt, device=weight.device) if wanted[0] else None
+        dweight = torch.empty(weight.shape, dtype=wdt, device=weight.device) if wanted[1] else None
+        result = lambda t, d: (None, 0) if t is None else (t.data_ptr(), _CODE[d])  # noqa: E731
+        check(L.unit_gated_dense_grad(*x, weight.data_ptr(), grad.data_ptr(), *kept, *_group_args(sizes), *result(ddata, dt), *result(dweight, wdt), code, act,
+                                      rows, e, n, k, ws.data_ptr(), ws.numel(), _stream()))
+    return ddata, dweight

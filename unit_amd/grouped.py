@@ -250,6 +250,20 @@ class Mxfp8Tensor:
         return f"Mxfp8Tensor(shape={self.shape}, device='{self.device}')"
 
 
+class _GatedCalls(_Calls):
+    """The common case of MXFP8 and of the gated products (gated.py) as native functions, like ops._Calls."""
+
+    _NAMES = ("quantize8", "dequantize8", "gated", "gated_mx", "gated_grad")
+    _LIBRARY = ("unit_mxfp4_bytes", "unit_mxfp4_workspace_bytes", "unit_mxfp8_bytes", "unit_quantize_mxfp8", "unit_dequantize_mxfp8", "unit_gated_dense",
+                "unit_gated_dense_mxfp4", "unit_gated_dense_grad_ws_bytes", "unit_gated_dense_grad")
+
+    def _bind(self, calls, addresses):
+        calls.bind_gated(addresses, Mxfp4Tensor, Mxfp8Tensor)
+
+
+_native_gated = _GatedCalls()
+
+
 def _mxfp8_empty(shape, device):
     return Mxfp8Tensor(torch.empty((sum(_mxfp8_bytes(math.prod(shape[:-1]), shape[-1])),), dtype=torch.uint8, device=device), tuple(shape))
 
@@ -260,6 +274,9 @@ def quantize_mxfp8(x):
     The scale of a block is the smallest power of two, 2^-127 at least, for which its largest magnitude is at most 448; elements are
     x / scale rounded to the nearest 8-bit float, ties to the even mantissa, so nothing saturates.  A block that holds an infinity or
     a NaN becomes NaN throughout."""
+    q = _native_gated.quantize8(x)
+    if q is not None:
+        return q
     x = _floats(x, "x", tuple(_CODE))
     if x.dim() not in (2, 3):
         raise ValueError(f"x: expected two axes or three, got shape {tuple(x.shape)}")
@@ -273,6 +290,9 @@ def quantize_mxfp8(x):
 def dequantize_mxfp8(q, out_dtype="float32"):
     """The values that an Mxfp8Tensor stands for, rounded once where out_dtype does not hold them.  The type that was quantised holds them all
     but for the power of two above its largest value, which magnitudes within a thirty-second of it become: infinite."""
+    out = _native_gated.dequantize8(q, out_dtype)
+    if out is not None:
+        return out
     dt = _out_dtype(out_dtype)
     if not isinstance(q, Mxfp8Tensor):
         raise TypeError(f"q: expected an Mxfp8Tensor, got {type(q).__name__}")
@@ -340,22 +360,16 @@ def _grouped_grad(data, weight, grad, group_sizes, out_dtype, weight_out_dtype, 
     rows = data.shape[0]
     if tuple(grad.shape) != (rows, n):
         raise ValueError(f"grad: expected ({rows}, {n}), got {tuple(grad.shape)}")
-    with _on(weight) if isinstance(data, Mxfp8Tensor) else contextlib.nullcontext():
-        return _product_grads(data, weight, grad, sizes, (rows, e, n, k), dt, wdt, wanted)
-
-
-def _product_grads(data, weight, grad, sizes, shape, dt, wdt, wanted):
-    """the gradients' two products; sizes None: one group, whose weight may have two axes"""
-    rows, e, n, k = shape
-    L, tail, code = _lib.load(), (*shape, _stream()), _CODE[weight.dtype]
-    groups = (None, 4) if sizes is None else (sizes.data_ptr(), sizes.element_size())
+    L, tail = _lib.load(), (rows, e, n, k, _stream())
     ddata = dweight = None
     if wanted[0]:
         ddata = torch.empty((rows, k), dtype=dt, device=weight.device)
-        check(L.unit_grouped_dense_grad_data(grad.data_ptr(), weight.data_ptr(), *groups, ddata.data_ptr(), code, _CODE[dt], *tail))
+        check(L.unit_grouped_dense_grad_data(grad.data_ptr(), weight.data_ptr(), sizes.data_ptr(), sizes.element_size(), ddata.data_ptr(),
+                                             _CODE[weight.dtype], _CODE[dt], *tail))
     if wanted[1]:
         if isinstance(data, Mxfp8Tensor):
             data = dequantize_mxfp8(data, _NAME[weight.dtype])
-        dweight = torch.empty(weight.shape, dtype=wdt, device=weight.device)
-        check(L.unit_grouped_dense_grad_weight(data.data_ptr(), grad.data_ptr(), *groups, dweight.data_ptr(), code, _CODE[wdt], *tail))
+        dweight = torch.empty((e, n, k), dtype=wdt, device=weight.device)
+        check(L.unit_grouped_dense_grad_weight(data.data_ptr(), grad.data_ptr(), sizes.data_ptr(), sizes.element_size(), dweight.data_ptr(),
+                                               _CODE[weight.dtype], _CODE[wdt], *tail))
     return ddata, dweight
