@@ -211,11 +211,11 @@ def test_large_tiles(dev):
         near(kept, pre, pre_off, "bfloat16")
 
 
-@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5, 6, 7])
 @pytest.mark.parametrize("keep", [None, "pre", "mxfp8"])
 def test_every_tile(dev, tile, keep, monkeypatch):
     """Each tile on problems that end inside it, whichever the rule would take."""
-    monkeypatch.setenv("UNIT_AMD_GROUPED_TILE", str(tile))
+    monkeypatch.setenv("UNIT_AMD_GATED_TILE", str(tile))
     for sizes, rows, n, k in ((None, 40, 72, 136), ([70, 0, 300, 33], 410, 328, 200)):
         x, w = randn((rows, k), "float16", 9, dev), randn((() if sizes is None else (len(sizes),)) + (2 * n, k), "float16", 10, dev, k ** -0.5)
         s = None if sizes is None else torch.tensor(sizes, device=dev)
@@ -250,6 +250,16 @@ def test_nonfinite_values_stay_in_their_rows_and_groups(dev, sizes):
         assert bool(torch.isfinite(dx[good]).all()) and bool(torch.isnan(dx[bad]).all())
         if sizes:
             assert not bool(dx[-6:].any()) and bool(torch.isfinite(dw[:2]).all()) and bool(torch.isnan(dw[2]).any())
+
+
+@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+def test_every_mxfp4_tile(dev, tile, monkeypatch):
+    monkeypatch.setenv("UNIT_AMD_GROUPED_TILE", str(tile))
+    for sizes, rows, n, k in ((None, 40, 72, 136), ([70, 0, 300, 33], 410, 333, 600)):
+        x, w = randn((rows, k), "float16", 9, dev), U.quantize_mxfp4(randn((() if sizes is None else (len(sizes),)) + (2 * n, k), "float16", 10, dev, k ** -0.5))
+        s = None if sizes is None else torch.tensor(sizes, device=dev)
+        h, off, _, _ = forward(U.dequantize_mxfp4(U.quantize_mxfp4(x)), U.dequantize_mxfp4(w), sizes, "gelu_tanh")
+        near(U.gated_dense_mxfp4(x, w, s, "gelu_tanh"), h, off, "float32")
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
@@ -341,9 +351,10 @@ def test_refusals(dev):
             call()
 
 
-@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5, 6, 7])
 def test_gradients_on_every_tile(dev, tile, monkeypatch):
-    monkeypatch.setenv("UNIT_AMD_GROUPED_TILE", str(tile))
+    monkeypatch.setenv("UNIT_AMD_GATED_TILE", str(tile))
+    monkeypatch.setenv("UNIT_AMD_GROUPED_TILE", str(min(tile, 5)))
     for case in ((None, 40, 72, 136), ([70, 0, 300, 33], 7, 328, 200)):
         x, w, dy, s = operands(case, "float16", dev)
         _, _, exact, off = forward(x, w, case[0], "silu")

@@ -4,10 +4,17 @@
 namespace unit {
 namespace {
 
+// the tile that the product with both halves of the weight would take
+inline int gated_tile_size_mx(const GatedParams &p) {
+  GroupedParams both = p;
+  both.n = 2 * p.n;
+  return grouped_tile_size(both, FORWARD, true);
+}
+
 template <class Out>
 int run(const char *what, const GatedParams &p, hipStream_t s) {
   const char *tag = "mxgated";
-  switch (gated_tile_size(p, true)) {
+  switch (gated_tile_size_mx(p)) {
     case TILE_FEW: return run_grouped_tile<OpMx, FORWARD, Tile<32, 128, 128, 1, 2>, 2, Out, GATE_ONLY>(what, tag, p, s);
     case TILE_SMALL: return run_grouped_tile<OpMx, FORWARD, Tile<64, 128, 128, 2, 2>, 3, Out, GATE_ONLY>(what, tag, p, s);
     case TILE_MIDDLE: return run_grouped_tile<OpMx, FORWARD, Tile<128, 128, 128, 2, 2>, 2, Out, GATE_ONLY>(what, tag, p, s);

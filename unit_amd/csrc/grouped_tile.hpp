@@ -245,21 +245,25 @@ struct RowsOut {
   }
 };
 
-// The same for MXFP8, which keeps whole blocks: each of a row's BLOCKS blocks is in two lanes, 16 columns each.
-template <int BLOCKS, class F>
-__device__ __forceinline__ void put_mx8(char *rows, char *codes, char *scales, int blocks, int high, int width, int y, F value) {
-  constexpr int PITCH = BLOCKS * 32 + 16, RUNS = BLOCKS * 2;
-  const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
-#pragma unroll
-  for (int j = 0; j < BLOCKS; ++j) {
+// Pre-activations of a tile in MXFP8.  Each of a row's blocks of 32 columns is in two lanes, 16 columns each; codes and scales are gathered in LDS,
+// [row][gate, up][column], from where the whole workgroup writes them in pieces of 16 bytes, a row's 128 columns a line.  (By each wave
+// for itself, 32 bytes and a single scale at a time: 8192 x 1024 -> 1024 dense KEEP8_OLD us, KEEP8_NEW like this.)
+template <class T>
+struct Mx8Tile {
+  static constexpr int COLS = T::BY / 2, PITCH = T::BY + 16, BLOCKS = COLS / 32, SCALES = T::BX * PITCH, BYTES = SCALES + T::BX * 2 * BLOCKS;
+
+  // half: 0 gate, 1 up; row: of the tile; col: the block's first column in the tile; left: columns of the result from there on
+  template <class F>
+  static __device__ __forceinline__ void block(char *lds, int half, int row, int col, int left, F value) {
+    const int hi = (threadIdx.x & 63) >> 5;
     v4f f[4];
     u32 top = 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      f[r] = value(j, r);
+      f[r] = value(r);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (y + j * 32 + 8 * r + 4 * half + e >= width) f[r][e] = 0;  // zeros behind the row's end
+        if (8 * r + 4 * hi + e >= left) f[r][e] = 0;  // zeros behind the row's end
       const v4u bits = __builtin_bit_cast(v4u, f[r]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = max(top, bits[e] & 0x7fffffffu);
@@ -267,17 +271,37 @@ __device__ __forceinline__ void put_mx8(char *rows, char *codes, char *scales, i
     top = max(top, (u32)__shfl_xor((int)top, 32));
     const u32 s = mx8_scale(top);
     const float p = mx_power(s == 255 ? 127 : s);
+    char *const codes = lds + row * PITCH + half * COLS + col;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) *reinterpret_cast<u32 *>(rows + l32 * PITCH + j * 32 + 8 * r + 4 * half) = four_codes8(f[r], p);
-    if (half == 0 && l32 < high && y + j * 32 < width) scales[(long)l32 * 2 * blocks + (y >> 5) + j] = (char)s;
+    for (int r = 0; r < 4; ++r) *reinterpret_cast<u32 *>(codes + 8 * r + 4 * hi) = four_codes8(f[r], p);
+    if (!hi) lds[SCALES + (row * 2 + half) * BLOCKS + col / 32] = (char)s;
   }
+
+  // row0: of the whole matrix; y0: the tile's first column
+  static __device__ __forceinline__ void write(const GatedParams &p, const char *lds, long row0, int high, int y0) {
+    constexpr int PIECES = T::BY / 16;  // of a row, both halves
+    const int nb = mx8_blocks(p.n);
+    for (int i = threadIdx.x; i < high * PIECES; i += T::NT) {
+      const int row = i / PIECES, piece = i % PIECES, half = piece / (PIECES / 2), c = piece % (PIECES / 2) * 16;
+      if (y0 + c < nb * 32)
+        *reinterpret_cast<v4u *>(p.pre + ((row0 + row) * 2 + half) * nb * 32l + y0 + c) = *reinterpret_cast<const v4u *>(lds + row * PITCH + half * COLS + c);
+    }
+    const int b0 = y0 / 32;
+    using word = std::conditional_t<BLOCKS == 4, u32, std::conditional_t<BLOCKS == 2, unsigned short, unsigned char>>;
+    const bool whole = nb % BLOCKS == 0 && (uintptr_t)p.pre_scales % BLOCKS == 0;
+    for (int i = threadIdx.x; i < high * 2; i += T::NT) {
+      char *dst = p.pre_scales + (row0 * 2 + i) * nb + b0;
+      const char *src = lds + SCALES + i * BLOCKS;
+      if (whole) {
+        *reinterpret_cast<word *>(dst) = *reinterpret_cast<const word *>(src);
+      } else {
 #pragma unroll
-  for (int k = 0; k < (32 * RUNS + 63) / 64; ++k) {
-    const int row = (k * 64 + lane) / RUNS, c = (k * 64 + lane) % RUNS * 16;
-    const v4u v = *reinterpret_cast<const v4u *>(rows + row * PITCH + c);
-    if (row < high && y + c < blocks * 32) *reinterpret_cast<v4u *>(codes + (long)row * 2 * blocks * 32 + y + c) = v;
+        for (int b = 0; b < BLOCKS; ++b)
+          if (b0 + b < nb) dst[b] = src[b];
+      }
+    }
   }
-}
+};
 
 // The gate's gradients of a wave: dg = dh u act'(g), du = dh act(g), of the same sums that h is made of.  dh comes in runs of 16 bytes a lane,
 // all of them asked for at once, and goes through the wave's LDS into the accumulators' order.
@@ -338,12 +362,6 @@ __device__ __forceinline__ void gated_results(const GatedParams &p, char *rows, 
       RowsOut<Half, CB>::put(rows, pre, 2l * p.n, left, p.n, y, part);
       RowsOut<Half, CB>::put(rows, pre + 2l * p.n, 2l * p.n, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) { return part(j + CB, r); });
     }
-    if constexpr (GATE == GATE_KEEP8) {
-      const int nb = mx8_blocks(p.n);
-      char *codes = p.pre + row * 2 * nb * 32, *scales = p.pre_scales + row * 2 * nb;
-      put_mx8<CB>(rows, codes, scales, nb, left, p.n, y, part);
-      put_mx8<CB>(rows, codes + nb * 32l, scales + nb, nb, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) { return part(j + CB, r); });
-    }
     RowsOut<Out, CB>::put(rows, p.out + row * p.n * (long)sizeof(Out), p.n, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) {
       const v4f g = part(j, r), u = part(j + CB, r);
       v4f h;
@@ -358,18 +376,20 @@ __device__ __forceinline__ void gated_results(const GatedParams &p, char *rows, 
 template <class Op, int DIR, class T, int NSTAGE, class Out, int GATE = GATE_NONE>
 __device__ __forceinline__ void compute_tile(const GateParams<GATE> &p, char *lds, int group, int first, int count, int x0, int high, int y0) {
   constexpr bool MX = Op::kMx, XT = DIR == GRAD_WEIGHT, YT = DIR != FORWARD;
-  constexpr int KK = T::BKB / 32, CPR = T::CPR, NW = T::NT / 64, RPL = 64 / CPR;
+  constexpr int KK = T::BKB / 32 / T::KG, CPR = T::CPR, NW = T::NT / 64, NWG = NW / T::KG, RPL = 64 / CPR;  // KK: k-steps of a stage and wave
   constexpr int KS = T::BKB / 2;                     // cols: reduction elements of a stage
   constexpr int XL = T::XBYTES / 1024 / NW, YL = T::YBYTES / 1024 / NW;
   constexpr int SCALES = MX ? (T::BX + T::BY) * 8 : 0, PIECES = MX ? (SCALES + 1023) / 1024 : 0, PIECE = PIECES ? PIECES : 1;
   constexpr int LPS = XL + YL + (MX ? 1 : 0);        // direct loads per wave and stage
   constexpr int STAGE = T::STAGE + PIECES * 1024;
   static_assert(XL * 1024 * NW == T::XBYTES && YL * 1024 * NW == T::YBYTES && KK % 2 == 0, "loads split evenly over the waves");
-  static_assert(!MX || (T::BKB == 128 && PIECES <= NW && DIR == FORWARD), "a stage of MXFP4 is one dword of scales per row and half");
+  static_assert(!MX || (T::BKB == 128 && PIECES <= NW && DIR == FORWARD && T::KG == 1), "a stage of MXFP4 is one dword of scales per row and half");
 
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int wx = wave / T::WY, wy = wave % T::WY, l32 = lane & 31, half = lane >> 5;  // waves of different rows share a SIMD
+  // KG sets of waves have the same tile and each its share of a stage's k-steps
+  const int kg = T::KG == 1 ? 0 : wave / NWG, kk0 = kg * KK, in_kg = T::KG == 1 ? wave : wave % NWG;
+  const int wx = in_kg / T::WY, wy = in_kg % T::WY, l32 = lane & 31, half = lane >> 5;  // waves of different rows share a SIMD
   // the row blocks there are, shared out evenly: this wave's first and how many
   const int high32 = (high + 31) / 32, block0 = (high32 * wx + T::WX - 1) / T::WX, blocks_x = (high32 * (wx + 1) + T::WX - 1) / T::WX - block0;
   const u32 ring = (u32)(uintptr_t)(lptr_t)lds;
@@ -498,21 +518,22 @@ __device__ __forceinline__ void compute_tile(const GateParams<GATE> &p, char *ld
   v4i xf[2][T::TX], yf[2][T::TY];
   int sx[2][T::TX], sy[2][T::TY];  // MXFP4: scale dwords of this stage and of the next
   // fragment idx of a step's list: X0, Y0 .. Y(TY-1), X1 .. X(TX-1)
-  auto load_one = [&](const char *stage, int kk, int s, int idx) __attribute__((always_inline)) {
+  auto load_one = [&](const char *stage, int kstep, int s, int idx) __attribute__((always_inline)) {
+    const int kk = kk0 + kstep;
     if (idx >= 1 && idx <= T::TY) {
       const int j = idx - 1;
       if constexpr (YT)
         yf[s][j] = transposed(stage + ytr[j] + kk * 16 * (T::BY * 2), T::BY * 2);
       else
         yf[s][j] = *reinterpret_cast<const v4i *>(stage + T::XBYTES + (yrow + j * 32) * T::BKB + (((2 * kk + half) ^ ysw) << 4));
-      if (MX && kk == 0) sy[1][j] = *reinterpret_cast<const int *>(stage + T::STAGE + T::BX * 8 + half * (T::BY * 4) + (yrow + j * 32) * 4);
+      if (MX && kstep == 0) sy[1][j] = *reinterpret_cast<const int *>(stage + T::STAGE + T::BX * 8 + half * (T::BY * 4) + (yrow + j * 32) * 4);
     } else {
       const int i = idx == 0 ? 0 : idx - T::TY;
       if constexpr (XT)
         xf[s][i] = transposed(stage + xtr[i] + kk * 16 * (T::BX * 2), T::BX * 2);
       else
         xf[s][i] = *reinterpret_cast<const v4i *>(stage + (xrow + i * 32) * T::BKB + (((2 * kk + half) ^ xsw) << 4));
-      if (MX && kk == 0) sx[1][i] = *reinterpret_cast<const int *>(stage + T::STAGE + half * (T::BX * 4) + (xrow + i * 32) * 4);
+      if (MX && kstep == 0) sx[1][i] = *reinterpret_cast<const int *>(stage + T::STAGE + half * (T::BX * 4) + (xrow + i * 32) * 4);
     }
   };
   auto next_scales = [&]() __attribute__((always_inline)) {
@@ -621,12 +642,61 @@ __device__ __forceinline__ void compute_tile(const GateParams<GATE> &p, char *ld
 
   // Results, rounded once, here: each wave puts 32 rows of its columns in order in LDS of its own and writes them in runs of 16 bytes a lane.
   // (Straight from the registers, 2 bytes a lane: experts of 16384 x 1024 -> 2048 102.7 us, 96.2 like this.)
+  if constexpr (T::KG > 1) {  // the sets' sums, added in their order
+    constexpr int BYTES = T::TX * T::TY * 4096;
+    static_assert((T::KG - 1) * NWG * BYTES <= NSTAGE * STAGE, "the other sets' sums fit the ring");
+    __syncthreads();  // the ring is read out
+    char *const mine = lds + in_kg * BYTES + lane * 16;
+    if (kg) {
+#pragma unroll
+      for (int i = 0; i < T::TX; ++i)
+#pragma unroll
+        for (int j = 0; j < T::TY; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            *reinterpret_cast<v4f *>(mine + (kg - 1) * (NWG * BYTES) + ((i * T::TY + j) * 4 + r) * 1024) =
+                v4f{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+    }
+    __syncthreads();
+    if (!kg) {
+#pragma unroll
+      for (int g = 1; g < T::KG; ++g)
+#pragma unroll
+        for (int i = 0; i < T::TX; ++i)
+#pragma unroll
+          for (int j = 0; j < T::TY; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const v4f v = *reinterpret_cast<const v4f *>(mine + (g - 1) * (NWG * BYTES) + ((i * T::TY + j) * 4 + r) * 1024);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[i][j][4 * r + e] += v[e];
+            }
+    }
+  }
   if constexpr (GATE) {
     static_assert(T::TY % 2 == 0 && DIR == FORWARD, "a wave has the gate's columns and the up projection's");
     constexpr int PITCH = RowsOut<float, T::TY / 2>::PITCH;  // of the widest
-    static_assert(NW * 32 * PITCH <= NSTAGE * STAGE, "the waves' rows fit the ring");
+    constexpr int KEPT = GATE == GATE_KEEP8 ? Mx8Tile<T>::BYTES : 0;
+    static_assert(KEPT + NWG * 32 * PITCH <= NSTAGE * STAGE && KEPT % 16 == 0, "codes, scales and the waves' rows fit the ring");
     __syncthreads();  // the ring is read out
-    char *const rows = lds + wave * (32 * PITCH);
+    char *const rows = lds + KEPT + in_kg * (32 * PITCH);
+    if constexpr (GATE == GATE_KEEP8) {
+      if (!kg)
+#pragma unroll
+        for (int i = 0; i < T::TX; ++i) {
+          if (i >= blocks_x) break;
+#pragma unroll
+          for (int j = 0; j < T::TY; ++j) {
+            const int col = wy * WCOLS + j % (T::TY / 2) * 32;
+            Mx8Tile<T>::block(lds, j / (T::TY / 2), (block0 + i) * 32 + l32, col, p.n - y0 - col, [&](int r) __attribute__((always_inline)) {
+              return v4f{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+            });
+          }
+        }
+      __syncthreads();
+      Mx8Tile<T>::write(p, lds, (long)first + x0, high, y0);
+    }
+    if (kg) return;
     if constexpr (GATE == GATE_GRAD)
       gated_gradients<T, Out>(p, rows, acc, blocks_x, (long)first + x0, block0 * 32, high, y0 + wy * WCOLS);
     else
@@ -634,8 +704,9 @@ __device__ __forceinline__ void compute_tile(const GateParams<GATE> &p, char *ld
     return;
   }
   constexpr int ES_OUT = (int)sizeof(Out), PITCH = T::TY * 32 * ES_OUT + 16, PER = 16 / ES_OUT, RUNS = T::TY * 32 / PER;  // elements per run, runs per row
-  static_assert(NW * 32 * PITCH <= NSTAGE * STAGE, "the waves' rows fit the ring");
+  static_assert(GATE || NW * 32 * PITCH <= NSTAGE * STAGE, "the waves' rows fit the ring");
   __syncthreads();  // the ring is read out
+  if (T::KG > 1 && kg) return;
   char *const rows = lds + wave * (32 * PITCH);
   const long out_row = (DIR == GRAD_WEIGHT ? (long)group * p.n : (long)first) + x0;
   const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(p.out + out_row * ys * (long)sizeof(Out), 0, -1, 0x00020000);
@@ -695,7 +766,7 @@ __global__ __launch_bounds__(T::NT, 2) void grouped_tile(GateParams<GATE> p, int
     find_rows(p, turn, lane, group, first, count);
     compute_tile<Op, DIR, T, NSTAGE, Out>(p, lds, group, first, count, x0, min(p.n - x0, T::BX), in / xts * T::BY);
   } else {
-    const GroupTileOf g = find_tile<T::BX, 4>(p, nts, (int)blockIdx.x, lane);
+    const GroupTileOf g = find_tile<T::BX, GATE ? 8 : 4>(p, nts, (int)blockIdx.x, lane);
     if (!g.any) return;
     compute_tile<Op, DIR, T, NSTAGE, Out, GATE>(p, lds, g.group, g.first, g.count, g.x0, g.high, g.nt * (GATE ? T::BY / 2 : T::BY));
   }
