@@ -407,3 +407,39 @@ def test_the_common_case_is_native(dev):
     for data, pre in ((x, None), (x8, None), (x, pre8), (x8, pre8)):
         assert native.gated_grad(data, w, dy, None, "silu", pre, "float16", "float32") is not None
     assert native.gated(x, w, None, "relu", "float16", None) is None and native.gated(x.float(), w, None, "silu", "float16", None) is None
+
+
+@pytest.mark.parametrize("tiles", [1, 2, 3, 4])
+@pytest.mark.parametrize("splits", [1, 2, 4, 16])
+def test_gradients_in_one_launch(dev, tiles, splits, monkeypatch):
+    """Each form of the launch, rows shared out or not, either product first, ragged on every side; with the tiles of groups beside it."""
+    monkeypatch.setenv("UNIT_AMD_GATED_PAIR", str(tiles))
+    monkeypatch.setenv("UNIT_AMD_GATED_SPLITS", str(splits))
+    cases = [(None, 1100, 72, 136), (None, 130, 264, 328), (None, 2087, 24, 72)]
+    for case in cases + ([([70, 0, 300, 33], 7, 136, 200), ([900, 0, 1], 0, 40, 264)] if splits == 1 else []):
+        for dtype, out in (("bfloat16", "bfloat16"), ("float16", "float32")):
+            x, w, dy, s = operands(case, dtype, dev)
+            _, kept = U.gated_dense(x, w, s, "silu", keep="pre")
+            got = U.gated_dense_grad(x, w, dy, s, "silu", kept, out, out)
+            dx, dxo, dw, dwo = gradients(x, w, dy, case[0], "silu", kept.double(), torch.zeros_like(kept, dtype=torch.float64), dtype)
+            near(got[0], dx, dxo, out)
+            near(got[1], dw, dwo, out)
+            for a, b in zip(got, U.gated_dense_grad(x, w, dy, s, "silu", kept, out, out)):
+                assert torch.equal(a, b)
+
+
+def test_gradients_of_many_rows_and_a_small_weight(dev):
+    """Where the rows are shared out by the rule itself, with the other operand frozen too."""
+    from unit_amd.gated import _gated_grad
+    x, w, dy, _ = operands((None, 9001, 136, 72), "bfloat16", dev)
+    _, kept = U.gated_dense(x, w, keep="pre")
+    dx, dxo, dw, dwo = gradients(x, w, dy, None, "silu", kept.double(), torch.zeros_like(kept, dtype=torch.float64), "bfloat16")
+    got = U.gated_dense_grad(x, w, dy, pre=kept)
+    near(got[0], dx, dxo, "float32")
+    near(got[1], dw, dwo, "float32")
+    for wanted in ((True, False), (False, True)):
+        one = _gated_grad(x, w, dy, None, "silu", kept, "float32", "float32", wanted)
+        for have, t, want, off in zip(wanted, one, (dx, dw), (dxo, dwo)):
+            assert (t is not None) == have
+            if have:
+                near(t, want, off, "float32")

@@ -15,6 +15,35 @@ int check_gated(const char *what, const void *sizes, int size_bytes, int rows, i
   return check_groups(what, sizes, size_bytes, rows, groups, N, K, w_bytes);
 }
 
+// dw from the float32 sums of the splits, added in their order, four elements a lane
+template <class Out>
+__global__ __launch_bounds__(256) void add_splits_kernel(const v4f *parts, Out *out, long quads, int splits) {
+  typedef Out v4o __attribute__((ext_vector_type(4)));
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= quads) return;
+  v4f sum = parts[i];
+#pragma unroll 4
+  for (int s = 1; s < splits; ++s) sum += parts[s * quads + i];
+  v4o v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (Out)sum[e];  // the one rounding
+  reinterpret_cast<v4o *>(out)[i] = v;
+}
+
+int add_splits(const char *what, const void *parts, void *out, int out_dtype, long elements, int splits, hipStream_t s) {
+  const long quads = elements / 4;  // N and K are multiples of 8
+  const dim3 grid((unsigned)((quads + 255) / 256));
+  const v4f *p = static_cast<const v4f *>(parts);
+  if (out_dtype == UNIT_F32)
+    hipLaunchKernelGGL(add_splits_kernel<float>, grid, dim3(256), 0, s, p, static_cast<float *>(out), quads, splits);
+  else if (out_dtype == UNIT_F16)
+    hipLaunchKernelGGL(add_splits_kernel<_Float16>, grid, dim3(256), 0, s, p, static_cast<_Float16 *>(out), quads, splits);
+  else
+    hipLaunchKernelGGL(add_splits_kernel<__bf16>, grid, dim3(256), 0, s, p, static_cast<__bf16 *>(out), quads, splits);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? UNIT_OK : fail(UNIT_E_LAUNCH, "%s: launch: %s", what, hipGetErrorString(e));
+}
+
 // dpre from dh and the pre-activations, eight columns a lane: 16 bytes of each of three operands in, of each of two results out (six,
 // eight and two in MXFP8), which is what it is bound by.
 template <class Half, bool MX8, int ROUNDS>
@@ -96,6 +125,46 @@ int run_gate_grad(const char *what, const void *pre, const void *scales, const v
 }
 
 }  // namespace
+
+PairPlan gated_pair_plan(int rows, int groups, bool one_group, int both, int k) {
+  struct Cost {
+    int x, y;
+    double a, b;
+  };
+  struct Form {
+    Cost dx, dw;
+    int slots;
+  };
+  static const Form forms[] = {{{64, 64, 3.5, 0.3}, {128, 128, 7, 0.5}, 512},
+                               {{128, 128, 6, 0.34}, {128, 128, 6, 0.34}, 256},
+                               {{192, 256, 6, 0.95}, {256, 256, 10, 0.95}, 256},
+                               {{256, 256, 10, 0.95}, {256, 256, 10, 0.95}, 256}};
+  const double r = rows > 0 ? rows : 1, busy = groups < r ? groups : r;
+  const auto up = [](double v, int d) { return (double)(long)((v + d - 1) / d); };
+  const int pinned = tuning_override("UNIT_AMD_GATED_PAIR"), pinned_splits = tuning_override("UNIT_AMD_GATED_SPLITS");
+  PairPlan best{PAIR_SMALL, 1, 0};
+  double least = 1e300;
+  for (int f = 0; f < 4; ++f)
+    for (int splits = 1; splits <= 16; splits *= 2) {
+      if (pinned > 0 && f != pinned - 1) continue;
+      // a split has 512 rows at least
+      if (pinned_splits > 0 && one_group ? splits != pinned_splits : splits > 1 && (!one_group || r < 512.0 * splits)) continue;
+      const Form &m = forms[f];
+      const double dx_tiles = (one_group ? up(r, m.dx.x) : r / m.dx.x + busy / 2) * up(k, m.dx.y), dw_tiles = (double)groups * splits * up(both, m.dw.x) * up(k, m.dw.y);
+      const double rows_w = r / groups / splits, tx = m.dx.a + m.dx.b * both / 64, tw = m.dw.a + m.dw.b * rows_w / 64;
+      const double longest_w = m.dw.a + m.dw.b * (one_group ? 1 : 2) * rows_w / 64, longest = tx > longest_w ? tx : longest_w;
+      const double total = (dx_tiles * tx + dw_tiles * tw) / m.slots;
+      double us = (total > longest ? total : longest) + 0.25 * (total > longest ? longest : total);
+      if (splits > 1) us += 4 + (splits + 0.5) * 2.0 * both * k * 4 / 5e6;  // the sums written and read, and a launch
+      if (us < least) {
+        least = us;
+        best = {static_cast<PairTiles>(f), splits, (int)(up(up(r, splits), 64) * 64)};
+      }
+    }
+  while (best.splits > 1 && (long)(best.splits - 1) * best.split_rows >= rows) --best.splits;  // none without rows
+  return best;
+}
+
 }  // namespace unit
 
 using namespace unit;
@@ -136,10 +205,17 @@ extern "C" int unit_gated_dense_mxfp4(const void *x, const void *xscales, int32_
 
 namespace {
 
-// The parts of the workspace of a gradient: dpre, the rows restored from MXFP8
+// The parts of the workspace of a gradient: dpre, the rows restored from MXFP8, float32 sums of dw's splits
 struct GradParts {
-  size_t dpre, x;
-  GradParts(int x_dtype, int rows, int N, int K) : dpre(((size_t)rows * N * 4 + 255) / 256 * 256), x(x_dtype == UNIT_MXFP8 ? (size_t)rows * K * 2 : 0) {}
+  size_t dpre, x, sums;
+  GradParts(int x_dtype, int rows, int groups, int N, int K) {
+    const auto lines = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+    const int splits = groups == 1 && rows ? gated_pair_plan(rows, 1, true, 2 * N, K).splits : 1;
+    dpre = lines((size_t)rows * N * 4);
+    x = x_dtype == UNIT_MXFP8 ? lines((size_t)rows * K * 2) : 0;
+    sums = splits > 1 ? (size_t)splits * N * K * 8 : 0;
+  }
+  size_t bytes() const { return dpre + x + sums; }
 };
 
 int check_grad_shape(const char *what, int x_dtype, int dtype, int rows, int groups, int N, int K) {
@@ -156,8 +232,7 @@ extern "C" int unit_gated_dense_grad_ws_bytes(int32_t x_dtype, int32_t dtype, in
   const char *what = "unit_gated_dense_grad_ws_bytes";
   if (int rc = check_grad_shape(what, x_dtype, dtype, rows, groups, N, K)) return rc;
   if (!bytes) return fail(UNIT_E_ARG, "%s: null pointer", what);
-  const GradParts parts(x_dtype, rows, N, K);
-  *bytes = parts.dpre + parts.x;
+  *bytes = GradParts(x_dtype, rows, groups, N, K).bytes();
   return UNIT_OK;
 }
 
@@ -173,12 +248,12 @@ extern "C" int unit_gated_dense_grad(const void *x, const void *x_scales, int32_
   if (dw && dw_dtype != UNIT_F32 && dw_dtype != dtype) return fail(UNIT_E_ARG, "%s: out_dtype of dw must be UNIT_F32 or dtype, got %d", what, dw_dtype);
   if (pre && pre_dtype != dtype && pre_dtype != UNIT_MXFP8) return fail(UNIT_E_ARG, "%s: pre_dtype must be dtype or UNIT_MXFP8, got %d", what, pre_dtype);
   const bool needs_x = dw || !pre, x8 = x_dtype == UNIT_MXFP8;
-  const GradParts parts(x_dtype, rows, N, K);
+  const GradParts parts(x_dtype, rows, groups, N, K);
   if (int rc = check_ptrs(what, rows, {w, dh, ws})) return rc;
   if (int rc = check_ptrs(what, rows && needs_x, {x})) return rc;
   if (int rc = check_aligned(what, {pre, dx, dw})) return rc;
   if (rows && ((x8 && needs_x && !x_scales) || (pre && pre_dtype == UNIT_MXFP8 && !pre_scales))) return fail(UNIT_E_ARG, "%s: null pointer", what);
-  if (ws_bytes < parts.dpre + parts.x) return fail(UNIT_E_ARG, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, parts.dpre + parts.x);
+  if (ws_bytes < parts.bytes()) return fail(UNIT_E_ARG, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, parts.bytes());
   if (int rc = check_device()) return rc;
   if (!dx && !dw) return UNIT_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -196,6 +271,17 @@ extern "C" int unit_gated_dense_grad(const void *x, const void *x_scales, int32_
     GatedParams p{{static_cast<const char *>(x), static_cast<const char *>(w), nullptr, nullptr, dpre, sizes, size_bytes, groups, rows, N, K},
                   act, nullptr, nullptr, static_cast<const char *>(dh)};
     if (int rc = (dtype == UNIT_F16 ? run_gated_f16 : run_gated_bf16)(what, GATE_GRAD, p, dtype, s)) return rc;
+  }
+  if (dx && dw && rows) {
+    PairPlan plan = gated_pair_plan(rows, groups, !sizes, 2 * N, K);
+    const bool split = plan.splits > 1;
+    char *const sums = dpre + parts.dpre + parts.x;
+    const auto product = [&](const void *y, void *out) {
+      return GroupedParams{dpre, static_cast<const char *>(y), nullptr, nullptr, static_cast<char *>(out), sizes, size_bytes, groups, rows, 2 * N, K};
+    };
+    const auto run = dtype == UNIT_F16 ? run_gated_pair_f16 : run_gated_pair_bf16;
+    if (int rc = run(what, product(w, dx), dx_dtype, product(x, split ? sums : dw), split ? (int)UNIT_F32 : dw_dtype, plan, s)) return rc;
+    return split ? add_splits(what, sums, dw, dw_dtype, 2l * N * K, plan.splits, s) : UNIT_OK;
   }
   if (dx)
     if (int rc = unit_grouped_dense_grad_data(dpre, w, sizes, size_bytes, dx, dtype, dx_dtype, rows, groups, 2 * N, K, stream)) return rc;

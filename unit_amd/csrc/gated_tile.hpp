@@ -16,9 +16,10 @@ namespace unit {
 //   ROUND   192 x 128: where its rounds are less work than LARGE's, a group ending in the middle of a tile on average
 //             2200 x 2048 -> 4096:         LARGE 96.1, ROUND *80.9    8192 x 1024 -> 1024 over 16: LARGE 52.5, ROUND *46.3
 //             16384 x 1024 -> 1024 over 32: LARGE *92.5, ROUND 105.7  4096 x 2048 -> 4096: LARGE *114.5, ROUND 129.1
-//   WIDE    128 x 64, two sets, one a CU: most of one round of it, and 2 KiB of reduction
+//   WIDE    128 x 64, two sets, one a CU: most of one round of it, 128 rows a group, and 2 KiB of reduction
 //             1500 x 1024 -> 1024 (192 tiles): WIDE *11.8, MIDDLE 12.4, SMALL 13.0   500 x 2048 -> 4096 (256): WIDE *22.2, MIDDLE 22.6
 //             1000 x 512 -> 2048 (256):    WIDE 11.5, MIDDLE *8.9     1000 x 1024 -> 1024 (128): WIDE 11.1, SMALL *9.0
+//             2200 x 4096 -> 512 (144):    WIDE *27.5, SMALL 34.6     1000 x 1024 -> 1024 over 16: WIDE 22.3, SMALL *15.3
 //   MIDDLE  128 x 64, two a CU: 192 tiles and as many rows a group
 //             1000 x 512 -> 2048:          MIDDLE *8.9, SMALL 10.5    3000 x 1024 -> 1024 over 64: MIDDLE 63.9, SMALL *53.9
 //   SMALL   64 x 64, two a CU
@@ -36,7 +37,7 @@ inline GatedTile gated_tile_size(const GatedParams &p) {
     return 10 * rounds(192) < 9 * rounds(256) ? GATED_ROUND : GATED_LARGE;
   }
   const long middle = tiles(128, 64);
-  if (middle >= 160 && middle <= 256 && p.k >= 1024) return GATED_WIDE;
+  if (middle >= 140 && middle <= 256 && p.k >= 1024 && mean >= 128) return GATED_WIDE;
   return middle >= 192 && mean >= 192 ? GATED_MIDDLE : GATED_SMALL;
 }
 
