@@ -64,7 +64,9 @@ def test_gated_mxfp4_arguments(L):
 def test_gated_gradient_arguments(L):
     need = ctypes.c_size_t()
     assert L.unit_gated_dense_grad_ws_bytes(1, 1, 4, 2, 16, 16, ctypes.byref(need)) == 0 and need.value == 256
-    assert L.unit_gated_dense_grad_ws_bytes(4, 2, 1000, 2, 24, 40, ctypes.byref(need)) == 0 and need.value == 1000 * 96 + 1000 * 80
+    assert L.unit_gated_dense_grad_ws_bytes(4, 2, 1000, 2, 24, 40, ctypes.byref(need)) == 0 and need.value == 1000 * 96 + 80128  # parts begin on 256 bytes
+    # one group of many rows and a small weight: float32 sums of the parts that its rows are shared out to
+    assert L.unit_gated_dense_grad_ws_bytes(1, 1, 10000, 1, 64, 64, ctypes.byref(need)) == 0 and need.value > 10000 * 256 and (need.value - 10000 * 256) % (64 * 64 * 8) == 0
     assert L.unit_gated_dense_grad_ws_bytes(1, 1, 0, 2, 16, 16, ctypes.byref(need)) == 0 and need.value == 0
     said(L, L.unit_gated_dense_grad_ws_bytes(2, 1, 4, 2, 16, 16, ctypes.byref(need)), "x_dtype")
     said(L, L.unit_gated_dense_grad_ws_bytes(1, 1, 4, 2, 16, 16, None), "null")

@@ -1,17 +1,19 @@
 """A feed-forward layer of experts on the grouped products: tokens are routed to their `top_k` experts, sorted by expert, taken through
-an up and a down product, and put together again.  16-bit weights, trainable through torch.autograd (`expert_linear`), or MXFP4
-weights for serving.  No counterpart in the reference.
+an up and a down product, or a gated one and a down product, and put together again.  16-bit weights, trainable through torch.autograd
+(`expert_linear`, `gated_linear`), activations kept in 16 bits, in MXFP8 or not at all, or MXFP4 weights for serving.  No counterpart in
+the reference.
 
-  python -m unit_amd.experts [TOKENS EXPERTS TOP_K MODEL HIDDEN]     times both, forward and training step
+  python -m unit_amd.experts [TOKENS EXPERTS TOP_K MODEL HIDDEN [silu|gelu_tanh]]     times both, forward and training step; gated
 """
 import sys
 import time
 
 import torch
 
-from .grouped import Mxfp4Tensor, _grouped_grad, grouped_dense, grouped_dense_grad, grouped_dense_mxfp4, quantize_mxfp4
+from .gated import _activation, _gated_grad, gated_dense, gated_dense_grad, gated_dense_mxfp4
+from .grouped import Mxfp4Tensor, Mxfp8Tensor, _grouped_grad, grouped_dense, grouped_dense_grad, grouped_dense_mxfp4, quantize_mxfp4, quantize_mxfp8
 
-__all__ = ["ExpertLayer", "expert_linear", "route"]
+__all__ = ["ExpertLayer", "expert_linear", "gated_linear", "route"]
 
 _NAME = {torch.float32: "float32", torch.float16: "float16", torch.bfloat16: "bfloat16"}
 
@@ -23,28 +25,82 @@ def _name(x):
         raise TypeError(f"x: expected dtype {' or '.join(str(d) for d in _NAME)}, got {x.dtype}") from None
 
 
+def _aligned(grad):
+    grad = grad.contiguous()
+    if grad.data_ptr() % 16:  # a part of a larger gradient (torch.cat's, say): the kernels read 16 bytes at a time
+        grad = grad.clone()
+    return grad
+
+
+def _once(name):
+    if torch.is_grad_enabled():  # the products below leave no trace: a derivative of these gradients would lack its part
+        raise RuntimeError(f"{name}: its gradients have no derivative of their own (create_graph=True)")
+
+
+def _keep(ctx, *kept):
+    """what the backward pass needs: tensors as autograd keeps them, of an Mxfp8Tensor its buffer and shape"""
+    ctx.shapes = [t.shape if isinstance(t, Mxfp8Tensor) else None for t in kept]
+    ctx.save_for_backward(*(t.buf if isinstance(t, Mxfp8Tensor) else t for t in kept))
+
+
+def _kept(ctx):
+    return [t if shape is None else Mxfp8Tensor(t, shape) for t, shape in zip(ctx.saved_tensors, ctx.shapes)]
+
+
 class _ExpertLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, group_sizes):
-        ctx.save_for_backward(x, weight, group_sizes)
+    def forward(ctx, x, weight, group_sizes, keep):
+        ctx.name = _name(x)
+        _keep(ctx, quantize_mxfp8(x) if keep == "mxfp8" else x, weight, group_sizes)
         return grouped_dense(x, weight, group_sizes, _name(x))
 
     @staticmethod
     def backward(ctx, grad):
-        if torch.is_grad_enabled():  # the products below leave no trace: a derivative of these gradients would lack its part
-            raise RuntimeError("expert_linear: its gradients have no derivative of their own (create_graph=True)")
-        x, weight, group_sizes = ctx.saved_tensors
-        grad = grad.contiguous()
-        if grad.data_ptr() % 16:  # a part of a larger gradient (torch.cat's, say): the kernels read 16 bytes at a time
-            grad = grad.clone()
+        _once("expert_linear")
+        x, weight, group_sizes = _kept(ctx)
         wanted = ctx.needs_input_grad[:2]  # a frozen operand's gradient is not computed
-        args = x, weight, grad, group_sizes, _NAME[x.dtype], _NAME[weight.dtype]
-        return *(grouped_dense_grad(*args) if all(wanted) else _grouped_grad(*args, wanted)), None
+        args = x, weight, _aligned(grad), group_sizes, ctx.name, _NAME[weight.dtype]
+        return *(grouped_dense_grad(*args) if all(wanted) else _grouped_grad(*args, wanted)), None, None
 
 
-def expert_linear(x, weight, group_sizes):
-    """grouped_dense in x's type, differentiable in x and weight, once: a backward pass with create_graph=True is refused."""
-    return _ExpertLinear.apply(x, weight, group_sizes)
+def expert_linear(x, weight, group_sizes, keep=None):
+    """grouped_dense in x's type, differentiable in x and weight, once: a backward pass with create_graph=True is refused.
+    keep "mxfp8": x is kept for it in 8 bits."""
+    if keep not in (None, "mxfp8"):
+        raise ValueError(f"keep: expected None or 'mxfp8', got {keep!r}")
+    return _ExpertLinear.apply(x, weight, group_sizes, keep)
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, group_sizes, activation, keep):
+        ctx.name, ctx.activation = _name(x), activation
+        if keep == "rows":
+            h, pre = gated_dense(x, weight, group_sizes, activation, _name(x)), None
+        else:
+            h, pre = gated_dense(x, weight, group_sizes, activation, _name(x), keep=keep)
+        _keep(ctx, quantize_mxfp8(x) if keep == "mxfp8" else x, weight, group_sizes, pre)
+        return h
+
+    @staticmethod
+    def backward(ctx, grad):
+        _once("gated_linear")
+        x, weight, group_sizes, pre = _kept(ctx)
+        wanted = ctx.needs_input_grad[:2]
+        args = x, weight, _aligned(grad), group_sizes, ctx.activation, pre, ctx.name, _NAME[weight.dtype]
+        return *(gated_dense_grad(*args) if all(wanted) else _gated_grad(*args, wanted)), None, None, None
+
+
+def gated_linear(x, weight, group_sizes=None, activation="silu", keep="pre"):
+    """gated_dense in x's type, differentiable in x and weight, once.  keep: what it holds until then beside the weight, bytes per row of
+    16-bit operands: "pre" x and the pre-activations (2 K + 4 N), "mxfp8" both in 8 bits (K + 2 N and a thirty-second), "rows" x alone
+    (2 K): the pre-activations are computed again."""
+    if keep not in ("pre", "mxfp8", "rows"):
+        raise ValueError(f"keep: expected 'pre', 'mxfp8' or 'rows', got {keep!r}")
+    _activation(activation)
+    if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad):
+        return gated_dense(x, weight, group_sizes, activation, _name(x))
+    return _GatedLinear.apply(x, weight, group_sizes, activation, keep)
 
 
 def route(logits, top_k):
@@ -59,23 +115,39 @@ def route(logits, top_k):
 
 
 class ExpertLayer:
-    """y[t] = sum over t's experts e of share * down[e] . silu(up[e] . x[t]).
+    """y[t] = sum over t's experts e of share * down[e] . silu(up[e] . x[t]), or, with gate "silu" or "gelu_tanh", of
+    share * down[e] . (gate(g[e] . x[t]) * (u[e] . x[t])), g[e] the first half of up[e]'s rows and u[e] the second.
 
-    up (E, hidden, model) and down (E, model, hidden): float16 or bfloat16 tensors of x's type, or Mxfp4Tensors, for which
-    x has no gradient (an x that asks for one is refused) and the logits have theirs."""
+    up (E, hidden, model), gated (E, 2 * hidden, model), and down (E, model, hidden): float16 or bfloat16 tensors of x's type, or
+    Mxfp4Tensors, for which x has no gradient (an x that asks for one is refused) and the logits have theirs.
+    keep, of a gated layer: what it holds for the backward pass, as in gated_linear; with "mxfp8" down's rows are in 8 bits too."""
 
-    def __init__(self, up, down, top_k):
-        if not len(up.shape) == len(down.shape) == 3 or up.shape[0] != down.shape[0] or up.shape[1] != down.shape[2] or up.shape[2] != down.shape[1]:
-            raise ValueError(f"up {tuple(up.shape)}, down {tuple(down.shape)}: expected (E, hidden, model) and (E, model, hidden)")
+    def __init__(self, up, down, top_k, gate=None, keep="pre"):
+        if gate is not None:
+            _activation(gate)
+        if keep not in ("pre", "mxfp8", "rows"):
+            raise ValueError(f"keep: expected 'pre', 'mxfp8' or 'rows', got {keep!r}")
+        if gate is None and keep != "pre":
+            raise ValueError(f"keep: {keep!r} is of a layer with a gate")
+        times, width = (1, "hidden") if gate is None else (2, "2 * hidden")
+        if not len(up.shape) == len(down.shape) == 3 or up.shape[0] != down.shape[0] or up.shape[1] != times * down.shape[2] or up.shape[2] != down.shape[1]:
+            raise ValueError(f"up {tuple(up.shape)}, down {tuple(down.shape)}: expected (E, {width}, model) and (E, model, hidden)")
         if isinstance(up, Mxfp4Tensor) != isinstance(down, Mxfp4Tensor):
             raise TypeError("up, down: both or neither in MXFP4")
         if not 0 < top_k <= up.shape[0]:
             raise ValueError(f"top_k: {top_k} of {up.shape[0]} experts")
-        self.up, self.down, self.top_k = up, down, top_k
+        self.up, self.down, self.top_k, self.gate, self.keep = up, down, top_k, gate, keep
 
     def quantized(self):
         """The same layer with MXFP4 weights."""
-        return ExpertLayer(quantize_mxfp4(self.up.detach()), quantize_mxfp4(self.down.detach()), self.top_k)
+        return ExpertLayer(quantize_mxfp4(self.up.detach()), quantize_mxfp4(self.down.detach()), self.top_k, self.gate, self.keep)
+
+    def _hidden(self, x, sizes, product):
+        if self.gate is None:
+            return torch.nn.functional.silu(product(x, self.up))
+        if isinstance(self.up, Mxfp4Tensor):
+            return gated_dense_mxfp4(x, self.up, sizes, self.gate, _name(x))
+        return gated_linear(x, self.up, sizes, self.gate, self.keep)
 
     def __call__(self, x, logits):
         name = _name(x)
@@ -89,8 +161,9 @@ class ExpertLayer:
         if isinstance(self.up, Mxfp4Tensor):
             product = lambda a, w: grouped_dense_mxfp4(a, w, sizes, name)  # noqa: E731
         else:
-            product = lambda a, w: expert_linear(a, w, sizes)  # noqa: E731
-        y = product(torch.nn.functional.silu(product(x[token], self.up)), self.down)
+            kept = "mxfp8" if self.gate is not None and self.keep == "mxfp8" else None
+            product = lambda a, w: expert_linear(a, w, sizes, kept)  # noqa: E731
+        y = product(self._hidden(x[token], sizes, product), self.down)
         back = torch.empty_like(order).scatter_(0, order, torch.arange(len(order), device=order.device))
         # every token's pairs side by side again: added in one order, whatever runs beside it
         y = y[back].view(x.shape[0], self.top_k, self.down.shape[1])
@@ -109,24 +182,33 @@ def _time(f, reps=20):
 
 
 def main(argv):
-    tokens, experts, top_k, model, hidden = (int(a) for a in argv) if argv else (2048, 16, 2, 1024, 2048)
+    gate = argv[5] if len(argv) > 5 else None
+    tokens, experts, top_k, model, hidden = (int(a) for a in argv[:5]) if argv else (2048, 16, 2, 1024, 2048)
     g = torch.Generator(device="cuda").manual_seed(1)
     rand = lambda *s: torch.randn(s, device="cuda", generator=g)  # noqa: E731
-    up, down = ((rand(experts, a, b) / b ** 0.5).bfloat16().requires_grad_() for a, b in ((hidden, model), (model, hidden)))
+    wide = hidden if gate is None else 2 * hidden
+    up, down = ((rand(experts, a, b) / b ** 0.5).bfloat16().requires_grad_() for a, b in ((wide, model), (model, hidden)))
     x, logits = rand(tokens, model).bfloat16().requires_grad_(), rand(tokens, experts)
-    layer = ExpertLayer(up, down, top_k)
+    layer = ExpertLayer(up, down, top_k, gate)
     served = layer.quantized()
 
-    def step():
+    def step(layer):
         layer(x, logits).float().square().mean().backward()
         x.grad = up.grad = down.grad = None
 
     with torch.no_grad():
         y, q = layer(x, logits).float(), served(x, logits).float()
-        print(f"{tokens} tokens, {top_k} of {experts} experts, {model} -> {hidden} -> {model}")
+        print(f"{tokens} tokens, {top_k} of {experts} experts, {model} -> {hidden} -> {model}" + ("" if gate is None else f", gated by {gate}"))
         print(f"bf16 forward          {_time(lambda: layer(x, logits)):9.1f} us")
         print(f"MXFP4 forward         {_time(lambda: served(x, logits)):9.1f} us   relative difference {float((q - y).norm() / y.norm()):.3f}")
-    print(f"bf16 forward and back {_time(step):9.1f} us")
+    for keep in ("pre",) if gate is None else ("pre", "mxfp8", "rows"):
+        kept = ExpertLayer(up, down, top_k, gate, keep)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = kept(x, logits)
+        held = torch.cuda.memory_allocated() - before
+        del loss
+        print(f"bf16 forward and back {_time(lambda: step(kept)):9.1f} us" + ("" if gate is None else f"   keep {keep!r}: {held / 2 ** 20:.1f} MiB until the backward pass"))
 
 
 if __name__ == "__main__":
