@@ -79,6 +79,7 @@ PairPlan gated_pair_plan(int rows, int groups, bool one_group, int both, int k);
 // px: dpre, w, dx; pw: dpre, x, dw (splits > 1: float32 sums of each split, one behind the other)
 int run_gated_pair_f16(const char *what, const GroupedParams &px, int dx_dtype, const GroupedParams &pw, int dw_dtype, const PairPlan &plan, hipStream_t s);
 int run_gated_pair_bf16(const char *what, const GroupedParams &px, int dx_dtype, const GroupedParams &pw, int dw_dtype, const PairPlan &plan, hipStream_t s);
+bool gated_mx_takes_floats(const GroupedParams &p);
 int run_gated_mx(const char *what, const GatedParams &p, int out_dtype, hipStream_t s);
 
 }  // namespace unit

@@ -1,5 +1,5 @@
 // MXFP4 gated products.
-#include "gated_tile.hpp"
+#include "grouped_split.hpp"
 
 namespace unit {
 namespace {
@@ -13,6 +13,8 @@ inline int gated_tile_size_mx(const GatedParams &p) {
 
 template <class Out>
 int run(const char *what, const GatedParams &p, hipStream_t s) {
+  if (p.x_dtype == UNIT_F16) return run_grouped_split<_Float16, Out, GATE_ONLY>(what, p, s);
+  if (p.x_dtype == UNIT_BF16) return run_grouped_split<__bf16, Out, GATE_ONLY>(what, p, s);
   const char *tag = "mxgated";
   switch (gated_tile_size_mx(p)) {
     case TILE_FEW: return run_grouped_tile<OpMx, FORWARD, Tile<32, 128, 128, 1, 2>, 2, Out, GATE_ONLY>(what, tag, p, s);
@@ -23,6 +25,11 @@ int run(const char *what, const GatedParams &p, hipStream_t s) {
 }
 
 }  // namespace
+
+// as grouped_mx_takes_floats: one launch for everything, where the chip holds its workgroups at once
+bool gated_mx_takes_floats(const GroupedParams &p) {
+  return (p.x_dtype == UNIT_F16 || p.x_dtype == UNIT_BF16) && p.k % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && grouped_split_pays(p);
+}
 
 int run_gated_mx(const char *what, const GatedParams &p, int out_dtype, hipStream_t s) {
   if (out_dtype == UNIT_F32) return run<float>(what, p, s);

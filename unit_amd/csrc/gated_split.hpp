@@ -3,11 +3,11 @@
 //
 // Such a product reads its weight once and does next to nothing with it: what bounds it is the time from its start to its first bytes and how
 // many are on their way.  Nothing is staged, a wave asks for four units (128 bytes of each of its 32 weight rows) at once and there
-// is as little code as will do.  1 x 2048 -> 4096, bf16, weights from memory: 9.5 us, 12.5 by tiles.
+// is as little code as will do.  1 x 2048 -> 4096, bf16: 9.0 us, 12.5 by tiles.
 //
 // v_mfma_f32_16x16x32: lane l holds eight elements of row l % 16 at 8 * (l / 16), of the weight (first operand) and of the rows (second), and
-// receives columns 4 * (l / 16) .. + 3 of row l % 16.  Loads are bounded by descriptors: rows past the last, elements past a row's end and
-// units past the last read as zeros.
+// receives columns 4 * (l / 16) .. + 3 of row l % 16.  Loads are bounded by descriptors: rows past the last and elements past a row's end
+// read as zeros.
 #pragma once
 #include "grouped_tile.hpp"
 
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(KW * 64, 2) void gated_split(GatedParams p, int nts
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const u32 at = (u32)(u * 128 + h * 64);
-      const bool in = u < units && at + (u32)q * 16 < ld;  // K is a multiple of 8: eight elements are inside or outside together
+      const bool in = at + (u32)q * 16 < ld;  // K is a multiple of 8: eight elements are inside or outside together
       xf[S][h] = load(xsrc, in ? off0 + at : kOut);
 #pragma unroll
       for (int c = 0; c < CB; ++c) {
@@ -88,18 +88,46 @@ __global__ __launch_bounds__(KW * 64, 2) void gated_split(GatedParams p, int nts
         }
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto each_slot = [&](auto f) __attribute__((always_inline)) {
-    f(std::integral_constant<int, 0>{});
-    f(std::integral_constant<int, 1>{});
-    f(std::integral_constant<int, 2>{});
-    f(std::integral_constant<int, 3>{});
+  // f on slots FROM .. TO - 1
+  auto slots = [&](auto from, auto to, auto f) __attribute__((always_inline)) {
+    constexpr int FROM = decltype(from)::value, TO = decltype(to)::value;
+    if constexpr (FROM <= 0 && 0 < TO) f(std::integral_constant<int, 0>{});
+    if constexpr (FROM <= 1 && 1 < TO) f(std::integral_constant<int, 1>{});
+    if constexpr (FROM <= 2 && 2 < TO) f(std::integral_constant<int, 2>{});
+    if constexpr (FROM <= 3 && 3 < TO) f(std::integral_constant<int, 3>{});
   };
-  each_slot([&](auto s) __attribute__((always_inline)) { fetch(decltype(s)::value, s); });
-  for (int i = 0; i * KW < units; i += DEPTH)
-    each_slot([&](auto s) __attribute__((always_inline)) {
-      consume(s);
-      fetch(i + DEPTH + decltype(s)::value, s);
+  using none = std::integral_constant<int, 0>;
+  using all = std::integral_constant<int, DEPTH>;
+  // call(n) with n < DEPTH as a constant: no load is issued that brings nothing, and every path fills the slots in one order
+  auto counted = [&](int n, auto call) __attribute__((always_inline)) {
+    if (n == 0) call(none{});
+    else if (n == 1) call(std::integral_constant<int, 1>{});
+    else if (n == 2) call(std::integral_constant<int, 2>{});
+    else call(std::integral_constant<int, 3>{});
+  };
+  const int mine = units > wave ? (units - wave + KW - 1) / KW : 0;
+  if (mine < DEPTH) {
+    counted(mine, [&](auto n) __attribute__((always_inline)) {
+      slots(none{}, n, [&](auto s) __attribute__((always_inline)) { fetch(decltype(s)::value, s); });
+      slots(none{}, n, consume);
     });
+  } else {
+    slots(none{}, all{}, [&](auto s) __attribute__((always_inline)) { fetch(decltype(s)::value, s); });
+    int i = DEPTH;
+    for (; i + DEPTH <= mine; i += DEPTH)
+      slots(none{}, all{}, [&](auto s) __attribute__((always_inline)) {
+        consume(s);
+        fetch(i + decltype(s)::value, s);
+      });
+    counted(mine - i, [&](auto n) __attribute__((always_inline)) {
+      slots(none{}, n, [&](auto s) __attribute__((always_inline)) {
+        consume(s);
+        fetch(i + decltype(s)::value, s);
+      });
+      slots(n, all{}, consume);
+      slots(none{}, n, consume);
+    });
+  }
 
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -146,17 +174,24 @@ __global__ __launch_bounds__(KW * 64, 2) void gated_split(GatedParams p, int nts
   }
 }
 
-template <class Half, class Out, int GATE>
-int run_gated_split(const char *what, const char *tag, const GatedParams &p, hipStream_t s) {
-  constexpr int KW = 8;
+template <class Half, int KW, class Out, int GATE>
+int launch_gated_split(const char *what, const char *tag, const GatedParams &p, long parts, hipStream_t s) {
   const int nts = ceil_div(p.n, GATE == GATE_KEEP8 ? 32 : 16);
-  const long parts = p.sizes ? (p.groups + 1 < p.rows ? p.groups + 1 : p.rows) : 1;
   const long wgs = parts * nts + 7;  // rows are at most 16: a tile per part; + 7 as in run_grouped_tile
   hipLaunchKernelGGL((gated_split<Half, KW, Out, GATE>), dim3((unsigned)wgs), dim3(KW * 64), 0, s, p, nts);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: launch: %s", what, hipGetErrorString(e));
   set_variant("%s_split_x16_g%d", tag, KW);
   return UNIT_OK;
+}
+
+// Eight waves a workgroup while there is at most one of them a CU, else four.  us, four and eight, bf16: 1 x 2048 -> 4096 (256 of them) 10.4, 9.0;
+// 16 x 1024 -> 2048 over 16 (2048, nine in sixteen at work) 16.1, 21.2
+template <class Half, class Out, int GATE>
+int run_gated_split(const char *what, const char *tag, const GatedParams &p, hipStream_t s) {
+  const long parts = p.sizes ? (p.groups + 1 < p.rows ? p.groups + 1 : p.rows) : 1;
+  if (parts * ceil_div(p.n, 16) <= 256) return launch_gated_split<Half, 8, Out, GATE>(what, tag, p, parts, s);
+  return launch_gated_split<Half, 4, Out, GATE>(what, tag, p, parts, s);
 }
 
 }  // namespace unit

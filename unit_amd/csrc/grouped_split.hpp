@@ -18,10 +18,11 @@ namespace unit {
 
 constexpr u32 kOutsideSplit = 0x80000000u;  // past every descriptor here
 
-template <class X, int KW, class Out>
-__global__ __launch_bounds__(KW * 64, 2) void grouped_split(GroupedParams p, int nts) {
-  constexpr int BM = 16, BN = 16, PITCH = BN + 4, DEPTH = 4;
-  __shared__ __attribute__((aligned(16))) float part[KW * BM * PITCH];
+// GATE_ONLY: a gated product (gated.hpp), whose 16 columns are rows of the gate's weight and the same of the up projection's
+template <class X, int KW, class Out, int GATE = GATE_NONE>
+__global__ __launch_bounds__(KW * 64, 2) void grouped_split(GateParams<GATE> p, int nts) {
+  constexpr int BM = 16, BN = 16, PITCH = BN + 4, DEPTH = 4, M = GATE ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) float part[M * KW * BM * PITCH];
   const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
 
@@ -35,27 +36,34 @@ __global__ __launch_bounds__(KW * 64, 2) void grouped_split(GroupedParams p, int
   }
   const int x0 = t.x0, y0 = t.nt * BN, rows = min(t.count - x0, BM), cols = min(p.n - y0, BN);  // both positive
   const int stages = mx_stages(p.k), ld = stages * 128, units = t.group < p.groups ? stages : 0;
-  const long wrows = (long)p.groups * p.n, wrow = (long)t.group * p.n + y0;
+  const long wrows = (long)p.groups * M * p.n, wrow = (long)t.group * M * p.n + y0;
 
   auto buffer = [](const void *base, u32 bytes) {
     const unsigned long long b = (unsigned long long)base;
     const unsigned long long u = (unsigned long long)scalar((u32)b) | (unsigned long long)scalar((u32)(b >> 32)) << 32;
     return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(u), 0, (int)scalar(bytes), 0x00020000);
   };
-  const auto wsrc = buffer(p.y + wrow * ld, units ? (u32)cols * (u32)ld : 0);
+  __amdgpu_buffer_rsrc_t wsrc[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) wsrc[m] = buffer(p.y + (wrow + m * (long)p.n) * ld, units ? (u32)cols * (u32)ld : 0);
   const auto xsrc = buffer(reinterpret_cast<const X *>(p.x) + (long)(t.first + x0) * p.k, (u32)rows * (u32)p.k * 2);
   const u32 woff = (u32)r16 * (u32)ld + (u32)q * 16, xoff = (u32)r16 * (u32)p.k * 2 + (u32)q * 64;
 
-  v4f acc = {0, 0, 0, 0};
-  v4i w[DEPTH][2], x[DEPTH][2][4];
-  u32 ws[DEPTH];
+  v4f acc[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) acc[m] = v4f{0, 0, 0, 0};
+  v4i w[DEPTH][M][2], x[DEPTH][2][4];
+  u32 ws[DEPTH][M];
   // this wave's i-th unit; the waves of a workgroup read neighbouring lines at a time
   auto fetch = [&](int i, auto slot) __attribute__((always_inline)) {
     constexpr int S = decltype(slot)::value;
     const int u = wave + i * KW;
     const u32 out = u < units ? 0 : kOutsideSplit;
-    const auto ssrc = buffer(p.ys + wrow + (long)u * 2 * wrows, u < units ? 0x7fffffffu : 0);
-    ws[S] = (u32)__builtin_amdgcn_raw_buffer_load_b32(ssrc, (int)((u32)(q & 1) * (u32)wrows * 4 + (u32)r16 * 4), 0, 0);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const auto ssrc = buffer(p.ys + wrow + m * (long)p.n + (long)u * 2 * wrows, u < units ? 0x7fffffffu : 0);
+      ws[S][m] = (u32)__builtin_amdgcn_raw_buffer_load_b32(ssrc, (int)((u32)(q & 1) * (u32)wrows * 4 + (u32)r16 * 4), 0, 0);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -64,14 +72,18 @@ __global__ __launch_bounds__(KW * 64, 2) void grouped_split(GroupedParams p, int
         const u32 off = k < p.k ? (xoff + (u32)(u * 512 + h * 256 + v * 16)) | out : kOutsideSplit;
         x[S][h][v] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(xsrc, (int)off, 0, 0));
       }
-      w[S][h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(wsrc, (int)((woff + (u32)(u * 128 + h * 64)) | out), 0, 0));
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+        w[S][m][h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(wsrc[m], (int)((woff + (u32)(u * 128 + h * 64)) | out), 0, 0));
     }
     __builtin_amdgcn_sched_barrier(0);  // slots are filled in the same order on every path, or the waits become waits for everything
   };
   auto consume = [&](auto slot) __attribute__((always_inline)) {
     constexpr int S = decltype(slot)::value;
     typedef typename Eight<X>::b8 b8;
-    const int sw = (int)(ws[S] >> (q & 2) * 4);  // of a dword's four scales this lane's are bytes 0 and 2 now
+    int sw[M];  // of a dword's four scales this lane's are bytes 0 and 2 now
+#pragma unroll
+    for (int m = 0; m < M; ++m) sw[m] = (int)(ws[S][m] >> (q & 2) * 4);
     auto half_unit = [&](auto hc) __attribute__((always_inline)) {
       constexpr int H = decltype(hc)::value;
       u32 top = 0;
@@ -82,8 +94,11 @@ __global__ __launch_bounds__(KW * 64, 2) void grouped_split(GroupedParams p, int
       v8i xf = {};
 #pragma unroll
       for (int v = 0; v < 4; ++v) xf[v] = (int)eight_codes<X>(__builtin_bit_cast(b8, x[S][H][v]), scale);
-      const v8i wf = {w[S][H][0], w[S][H][1], w[S][H][2], w[S][H][3]};
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc, 4, 4, 2 * H, sw, 0, (int)e);
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const v8i wf = {w[S][m][H][0], w[S][m][H][1], w[S][m][H][2], w[S][m][H][3]};
+        acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[m], 4, 4, 2 * H, sw[m], 0, (int)e);
+      }
     };
     half_unit(std::integral_constant<int, 0>{});
     half_unit(std::integral_constant<int, 1>{});
@@ -102,16 +117,22 @@ __global__ __launch_bounds__(KW * 64, 2) void grouped_split(GroupedParams p, int
       fetch(i + DEPTH + decltype(s)::value, s);
     });
 
-  *reinterpret_cast<v4f *>(part + (wave * BM + r16) * PITCH + 4 * q) = acc;
+#pragma unroll
+  for (int m = 0; m < M; ++m) *reinterpret_cast<v4f *>(part + ((m * KW + wave) * BM + r16) * PITCH + 4 * q) = acc[m];
   __syncthreads();
   Out *out = reinterpret_cast<Out *>(p.out) + (long)(t.first + x0) * p.n + y0;
   for (int i = threadIdx.x; i < rows * BN; i += KW * 64) {
     const int row = i / BN, c = i % BN;
     if (c >= cols) continue;
-    float s = part[row * PITCH + c];
+    float s[M];
 #pragma unroll
-    for (int k = 1; k < KW; ++k) s += part[(k * BM + row) * PITCH + c];
-    out[(long)row * p.n + c] = (Out)s;  // the one rounding
+    for (int m = 0; m < M; ++m) {
+      s[m] = part[(m * KW * BM + row) * PITCH + c];
+#pragma unroll
+      for (int k = 1; k < KW; ++k) s[m] += part[((m * KW + k) * BM + row) * PITCH + c];
+    }
+    if constexpr (GATE) s[0] = act_value(p.act, s[0]) * s[M - 1];
+    out[(long)row * p.n + c] = (Out)s[0];  // the one rounding
   }
 }
 
@@ -121,17 +142,17 @@ inline bool grouped_split_pays(const GroupedParams &p) {
   return p.rows <= 16 && parts * ceil_div(p.n, 16) <= 512;
 }
 
-template <class X, class Out>
-int run_grouped_split(const char *what, const GroupedParams &p, hipStream_t s) {
+template <class X, class Out, int GATE = GATE_NONE>
+int run_grouped_split(const char *what, const GateParams<GATE> &p, hipStream_t s) {
   constexpr int KW = 4;
   const int nts = ceil_div(p.n, 16);
   const long parts = p.sizes ? (p.groups + 1 < p.rows ? p.groups + 1 : p.rows) : 1;
   const long wgs = parts * nts + 7;  // rows are at most 16: a tile per part; + 7 as in run_grouped_tile
-  auto kern = grouped_split<X, KW, Out>;
+  auto kern = grouped_split<X, KW, Out, GATE>;
   hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(KW * 64), 0, s, p, nts);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: launch: %s", what, hipGetErrorString(e));
-  set_variant("mxdense_split_x16_y16_g%d", KW);
+  set_variant(GATE ? "mxgated_split_x16_y16_g%d" : "mxdense_split_x16_y16_g%d", KW);
   return UNIT_OK;
 }
 

@@ -52,38 +52,8 @@ __global__ __launch_bounds__(256) void quantize8_kernel(const T *x, int pieces, 
 }
 
 template <class T, int ROUNDS>
-__global__ __launch_bounds__(256) void dequantize8_kernel(const v2u *codes, const unsigned char *scales, int pieces, int K, T *out, FastDiv by_row) {
-  typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  v2u c[ROUNDS];
-  u32 s[ROUNDS];
-  const int first = (int)blockIdx.x * (256 * ROUNDS) + (int)threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < ROUNDS; ++i) {
-    const int at = min(first + i * 256, pieces - 1);
-    c[i] = codes[at];
-    s[i] = scales[at >> 2];
-  }
-#pragma unroll
-  for (int i = 0; i < ROUNDS; ++i) {
-    const int at = first + i * 256;
-    int row, q;
-    by_row.divmod(min(at, pieces - 1), row, q);
-    const int k0 = q * 8;
-    if (at >= pieces || k0 >= K) continue;
-    const float p = mx8_power(s[i]);
-    const v4f lo = four_values8(c[i][0], p), hi = four_values8(c[i][1], p);
-    v8 v;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (T)(j < 4 ? lo[j] : hi[j - 4]);  // one rounding, where T does not hold the value
-    T *dst = out + (size_t)row * K + k0;
-    if (k0 + 8 <= K) {
-      *reinterpret_cast<v8 *>(dst) = v;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (k0 + j < K) dst[j] = v[j];
-    }
-  }
+__global__ __launch_bounds__(256) void dequantize8_kernel(Mx8Rows<T> r) {
+  restore_pieces<T, ROUNDS>(r, (int)blockIdx.x);
 }
 
 int check_mx8(const char *what, int64_t rows, int32_t K, std::initializer_list<const void *> ptrs) {
@@ -160,9 +130,9 @@ extern "C" int unit_dequantize_mxfp8(const void *codes, const void *scales, int6
   auto run = [&](auto *p) {
     return by_pieces(what, rows, K, [&](auto rounds, dim3 grid, int64_t row, int pieces) {
       using T = std::remove_pointer_t<decltype(p)>;
-      hipLaunchKernelGGL((dequantize8_kernel<T, decltype(rounds)::value>), grid, dim3(256), 0, static_cast<hipStream_t>(stream),
-                         reinterpret_cast<const v2u *>(static_cast<const char *>(codes) + mx8_code_bytes(row, K)),
-                         static_cast<const unsigned char *>(scales) + mx8_scale_bytes(row, K), pieces, K, p + row * K, by_row);
+      const Mx8Rows<T> r{reinterpret_cast<const v2u *>(static_cast<const char *>(codes) + mx8_code_bytes(row, K)),
+                         static_cast<const unsigned char *>(scales) + mx8_scale_bytes(row, K), pieces, K, p + row * K, by_row};
+      hipLaunchKernelGGL((dequantize8_kernel<T, decltype(rounds)::value>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), r);
     });
   };
   set_variant("mx8dequantize");

@@ -37,4 +37,49 @@ __device__ __forceinline__ v4f four_values8(u32 c, float p) {
 }
 __device__ __forceinline__ float mx8_power(u32 s) { return s == 255 ? __builtin_nanf("") : mx_power(s); }
 
+// Rows to be restored, in pieces of eight elements (4 * blocks a row).
+template <class T>
+struct Mx8Rows {
+  const v2u *codes;
+  const unsigned char *scales;
+  int pieces, K;
+  T *out;  // (rows, K)
+  FastDiv by_row;
+};
+// the pieces of workgroup `group` of 256 lanes, ROUNDS a lane
+template <class T, int ROUNDS>
+__device__ __forceinline__ void restore_pieces(const Mx8Rows<T> &r, int group) {
+  typedef T v8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  v2u c[ROUNDS];
+  u32 s[ROUNDS];
+  const int first = group * (256 * ROUNDS) + (int)threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int at = min(first + i * 256, r.pieces - 1);
+    c[i] = r.codes[at];
+    s[i] = r.scales[at >> 2];
+  }
+#pragma unroll
+  for (int i = 0; i < ROUNDS; ++i) {
+    const int at = first + i * 256;
+    int row, q;
+    r.by_row.divmod(min(at, r.pieces - 1), row, q);
+    const int k0 = q * 8;
+    if (at >= r.pieces || k0 >= r.K) continue;
+    const float p = mx8_power(s[i]);
+    const v4f lo = four_values8(c[i][0], p), hi = four_values8(c[i][1], p);
+    v8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (T)(j < 4 ? lo[j] : hi[j - 4]);  // one rounding, where T does not hold the value
+    T *dst = r.out + (size_t)row * r.K + k0;
+    if (k0 + 8 <= r.K) {
+      *reinterpret_cast<v8 *>(dst) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k0 + j < r.K) dst[j] = v[j];
+    }
+  }
+}
+
 }  // namespace unit
