@@ -211,12 +211,13 @@ def test_large_tiles(dev):
         near(kept, pre, pre_off, "bfloat16")
 
 
-@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5, 6, 7])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5, 6, 7, 8])
 @pytest.mark.parametrize("keep", [None, "pre", "mxfp8"])
 def test_every_tile(dev, tile, keep, monkeypatch):
     """Each tile on problems that end inside it, whichever the rule would take."""
     monkeypatch.setenv("UNIT_AMD_GATED_TILE", str(tile))
-    for sizes, rows, n, k in ((None, 40, 72, 136), ([70, 0, 300, 33], 410, 328, 200)):
+    monkeypatch.setenv("UNIT_AMD_GATED_MOST", "255" if keep == "pre" else "160" if keep else "0")
+    for sizes, rows, n, k in ((None, 40, 72, 136), ([70, 0, 300, 33], 410, 328, 200), ([256, 417, 160, 673, 161, 512, 0, 1], 2200, 136, 72), (None, 930, 200, 64)):
         x, w = randn((rows, k), "float16", 9, dev), randn((() if sizes is None else (len(sizes),)) + (2 * n, k), "float16", 10, dev, k ** -0.5)
         s = None if sizes is None else torch.tensor(sizes, device=dev)
         h, off, pre, pre_off = forward(x, w, sizes, "gelu_tanh")
@@ -351,7 +352,7 @@ def test_refusals(dev):
             call()
 
 
-@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5, 6, 7])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4, 5, 6, 7, 8])
 def test_gradients_on_every_tile(dev, tile, monkeypatch):
     monkeypatch.setenv("UNIT_AMD_GATED_TILE", str(tile))
     monkeypatch.setenv("UNIT_AMD_GROUPED_TILE", str(min(tile, 5)))

@@ -67,13 +67,24 @@ __device__ __forceinline__ u32 scan_upto(u32 v, u32 top) {
   return v;
 }
 
+// Which of a group's rows a tiling takes.  ALL_ROWS; or tiles of two heights share a group: FRONT_ROWS takes it in tiles of kFront rows, but for
+// a remainder of at most `most` rows, which is BACK_ROWS' (rows of no group are FRONT_ROWS').
+enum GroupRows { ALL_ROWS, FRONT_ROWS, BACK_ROWS };
+constexpr u32 kFront = 256;
+template <int ROWS>
+__device__ __forceinline__ u32 rows_taken(u32 count, u32 most) {
+  const u32 rest = count % kFront;
+  return ROWS == ALL_ROWS ? count : ROWS == FRONT_ROWS ? (rest > most ? count : count - rest) : (rest > most ? 0 : rest);
+}
+
 // Where the groups begin and end, in rows and in tiles of BM rows: sums of sizes over the lanes, lane l for group l of the chunk of 64
 // at hand.  Every wave does this by itself.
-template <int BM>
+template <int BM, int ROWS = ALL_ROWS>
 struct GroupScan {
   u32 rows0, tiles0;      // rows and tiles of the chunks before
   u32 start, end, tend;   // this lane's group: first row, end of rows, end of tiles
   u32 rows_in, tiles_in;  // rows and tiles of all groups
+  u32 most;               // of rows_taken
   int chunks;
 
   __device__ __forceinline__ void chunk(const GroupedParams &p, int c, int lane) {
@@ -81,7 +92,7 @@ struct GroupScan {
     const u32 size = g < p.groups ? (u32)group_size(p, g) : 0;
     end = min(rows0 + scan_upto(size, (u32)p.rows), (u32)p.rows);
     start = (u32)__builtin_amdgcn_update_dpp((int)rows0, (int)end, 0x138, 0xf, 0xf, false);  // the lane before's; lane 0: rows0
-    tend = tiles0 + scan_upto((end - start + BM - 1) / BM, 1u << 30);
+    tend = tiles0 + scan_upto((rows_taken<ROWS>(end - start, most) + BM - 1) / BM, 1u << 30);
   }
   __device__ __forceinline__ void run(const GroupedParams &p, int lane) {
     rows0 = tiles0 = 0;
@@ -93,7 +104,7 @@ struct GroupScan {
     rows_in = lane_value(end, 63), tiles_in = lane_value(tend, 63);
   }
   // tiles of all rows, those of no group included
-  __device__ __forceinline__ u32 total(const GroupedParams &p) const { return tiles_in + ((u32)p.rows - rows_in + BM - 1) / BM; }
+  __device__ __forceinline__ u32 total(const GroupedParams &p) const { return tiles_in + (ROWS == BACK_ROWS ? 0 : ((u32)p.rows - rows_in + BM - 1) / BM); }
   // the group of row tile m < total(): itself (p.groups: none), its rows, and how many tiles lie before them
   __device__ __forceinline__ void find(const GroupedParams &p, u32 m, int lane, int &group, int &first, int &count, u32 &before) {
     if (m >= tiles_in) {
@@ -129,10 +140,11 @@ struct GroupTileOf {
 // ends at once.  Workgroups are dealt round-robin to the eight XCDs: those of one XCD take consecutive tiles, which walk a group in
 // panels of PH row tiles, column tile after column tile, so that the XCD's L2 holds the panel's rows and sees each weight tile once
 // a panel.
-template <int BM, int PH>
-__device__ __forceinline__ GroupTileOf find_tile(const GroupedParams &p, int nts, int bid, int lane) {
+template <int BM, int PH, int ROWS = ALL_ROWS>
+__device__ __forceinline__ GroupTileOf find_tile(const GroupedParams &p, int nts, int bid, int lane, int most = 0) {
   GroupTileOf t;
-  GroupScan<BM> scan;
+  GroupScan<BM, ROWS> scan;
+  scan.most = (u32)most;
   scan.run(p, lane);
   const u32 total = scan.total(p) * (u32)nts;
   const u32 per = total / 8, rem = total % 8, xcd = (u32)bid % 8, idx = (u32)bid / 8;
@@ -141,15 +153,17 @@ __device__ __forceinline__ GroupTileOf find_tile(const GroupedParams &p, int nts
   if (!t.any) return t;
   u32 before;
   scan.find(p, scalar(logical / (u32)nts), lane, t.group, t.first, t.count, before);  // a group is nts * (its row tiles)
-  const u32 mts = ((u32)t.count + BM - 1) / BM, within = scalar(logical) - before * (u32)nts;
+  const u32 taken = ROWS == ALL_ROWS || t.group == p.groups ? (u32)t.count : rows_taken<ROWS>((u32)t.count, (u32)most);
+  const u32 mts = (taken + BM - 1) / BM, within = scalar(logical) - before * (u32)nts;
   const u32 panel = within / ((u32)nts * PH), in_panel = within - panel * ((u32)nts * PH);
   const u32 high = min(mts - panel * PH, (u32)PH);
   t.nt = (int)scalar(in_panel / high);
   const u32 mt = panel * PH + in_panel - (u32)t.nt * high;
   // as many tiles as BM asks for, of even heights in blocks of 32 rows; never beyond the end: (mts - 1) * BM < count
-  const u32 even = scalar(((u32)t.count + 32 * mts - 1) / (32 * mts)) * 32;
+  const u32 even = scalar((taken + 32 * mts - 1) / (32 * mts)) * 32;
   t.x0 = (int)scalar(mt * even);
-  t.high = min(t.count - t.x0, (int)even);
+  t.high = min((int)taken - t.x0, (int)even);
+  if constexpr (ROWS == BACK_ROWS) t.x0 += t.count - (int)taken;
   return t;
 }
 
