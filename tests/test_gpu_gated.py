@@ -115,6 +115,7 @@ CASES = [  # group sizes (None: one weight), rows beside them, N, K
     ([513, 3, 0, 700], 40, 520, 248),
     ([5, 0, 9] * 30, 11, 96, 192),     # more groups than a wave has lanes
     ([0] * 300 + [70] + [0] * 50 + [1], 0, 64, 72),
+    ([0] * 70 + [3] + [0] * 80 + [9, 1] + [0] * 20, 3, 72, 200),  # the same of at most 16 rows
 ]
 
 
@@ -247,10 +248,11 @@ def test_nonfinite_values_stay_in_their_rows_and_groups(dev, sizes):
         assert bool(torch.isfinite(values[good]).all()) and not bool(torch.isfinite(values[bad]).any())
         if sizes:
             assert not bool(y[-6:].any()) and not bool(values[-6:].any())
-        dx, dw = U.gated_dense_grad(x, w, dy, s, pre=pre)
-        assert bool(torch.isfinite(dx[good]).all()) and bool(torch.isnan(dx[bad]).all())
-        if sizes:
-            assert not bool(dx[-6:].any()) and bool(torch.isfinite(dw[:2]).all()) and bool(torch.isnan(dw[2]).any())
+        for kept in (pre, None):
+            dx, dw = U.gated_dense_grad(x, w, dy, s, pre=kept)
+            assert bool(torch.isfinite(dx[good]).all()) and bool(torch.isnan(dx[bad]).all())
+            if sizes:
+                assert not bool(dx[-6:].any()) and bool(torch.isfinite(dw[:2]).all()) and bool(torch.isnan(dw[2]).any())
 
 
 @pytest.mark.parametrize("tile", [1, 2, 3, 4])
@@ -350,6 +352,20 @@ def test_refusals(dev):
     ):
         with pytest.raises(error, match=text):
             call()
+
+
+@pytest.mark.parametrize("most", [1, 128, 255])
+def test_tiles_of_two_sizes_over_many_groups(dev, most, monkeypatch):
+    """More groups than a wave has lanes, with remainders of every kind: none, one row, the limit and one more, all but one row of a tile."""
+    monkeypatch.setenv("UNIT_AMD_GATED_TILE", "8")
+    monkeypatch.setenv("UNIT_AMD_GATED_MOST", str(most))
+    sizes = [256, 0, 257, most, most + 1, 255, 512 + most, 1, 0, 31] * 7 + [700]
+    rows, n, k = sum(sizes) + 9, 136, 72
+    x, w = randn((rows, k), "bfloat16", 11, dev), randn((len(sizes), 2 * n, k), "bfloat16", 12, dev, k ** -0.5)
+    h, off, pre, pre_off = forward(x, w, sizes, "silu")
+    got, kept = U.gated_dense(x, w, torch.tensor(sizes, device=dev), "silu", "bfloat16", keep="pre")
+    near(got, h, off, "bfloat16")
+    near(kept, pre, pre_off, "bfloat16")
 
 
 @pytest.mark.parametrize("tile", [1, 2, 3, 4, 5, 6, 7, 8])
