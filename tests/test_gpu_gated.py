@@ -426,7 +426,7 @@ def test_the_common_case_is_native(dev):
     assert native.gated(x, w, None, "relu", "float16", None) is None and native.gated(x.float(), w, None, "silu", "float16", None) is None
 
 
-@pytest.mark.parametrize("tiles", [1, 2, 3, 4])
+@pytest.mark.parametrize("tiles", [1, 2, 3, 4, 5])
 @pytest.mark.parametrize("splits", [1, 2, 4, 16])
 def test_gradients_in_one_launch(dev, tiles, splits, monkeypatch):
     """Each form of the launch, rows shared out or not, either product first, ragged on every side; with the tiles of groups beside it."""

@@ -156,15 +156,16 @@ PairPlan gated_pair_plan(int rows, int groups, bool one_group, int both, int k) 
   static const Form forms[] = {{{64, 64, 3.5, 0.3}, {128, 128, 7, 0.5}, 512},
                                {{128, 128, 6, 0.34}, {128, 128, 6, 0.34}, 256},
                                {{192, 256, 6, 0.95}, {256, 256, 10, 0.95}, 256},
-                               {{256, 256, 10, 0.95}, {256, 256, 10, 0.95}, 256}};
+                               {{256, 256, 10, 0.95}, {256, 256, 10, 0.95}, 256},
+                               {{128, 256, 8, 1.05}, {128, 256, 8, 1.05}, 512}};
   const double r = rows > 0 ? rows : 1, busy = groups < r ? groups : r;
   const auto up = [](double v, int d) { return (double)(long)((v + d - 1) / d); };
   const int pinned = tuning_override("UNIT_AMD_GATED_PAIR"), pinned_splits = tuning_override("UNIT_AMD_GATED_SPLITS");
   PairPlan best{PAIR_SMALL, 1, 0};
   double least = 1e300;
-  for (int f = 0; f < 4; ++f)
+  for (int f = 0; f < 5; ++f)
     for (int splits = 1; splits <= 16; splits *= 2) {
-      if (pinned > 0 && f != pinned - 1) continue;
+      if (pinned > 0 ? f != pinned - 1 : f == PAIR_TALL && one_group) continue;
       // a split has 512 rows at least
       if (pinned_splits > 0 && one_group ? splits != pinned_splits : splits > 1 && (!one_group || r < 512.0 * splits)) continue;
       const Form &m = forms[f];

@@ -58,17 +58,20 @@ int run_gated_bf16(const char *what, int gate, const GatedParams &p, int out_dty
 // How the two products of a gradient run (gated_pair.hpp): tiles of dx and of dw, and how many workgroups share the rows of a tile of dw.
 //   PAIR_SMALL 64 x 64 (two sets of waves) and 128 x 128, two workgroups a CU    PAIR_WIDE 128 x 128 (two sets), one a CU
 //   PAIR_ROUND 192 x 256 and 256 x 256                                           PAIR_LARGE 256 x 256
-// Chosen by an estimate: a tile costs a + b * (64-element stages), fitted to 16 forms of the launch on 23 problems; a launch takes its tiles over
+//   PAIR_TALL  128 x 256, two a CU, of several groups: the start and the results of one beside the stages of the other
+// Chosen by an estimate: a tile costs a + b * (64-element stages), fitted to 20 forms of the launch on 28 problems; a launch takes its tiles over
 // the workgroups that the chip holds, or its longest tile, whichever is more, and a quarter of the other.  Where the estimate is wrong it
 // costs 3.5 % on average over those problems.  us, rows x K -> N over groups (* the one taken):
-//   8192 x 1024 -> 2048 over 16: SMALL 244, WIDE 260, ROUND 186, LARGE *180     3000 x 2048 -> 4096: SMALL 285, WIDE 241, ROUND *193, LARGE 203
+//   8192 x 1024 -> 2048 over 16: SMALL 250, WIDE 267, ROUND 191, LARGE 186, TALL *184   1000 x 1024 -> 1024 over 64: ROUND 153, LARGE 152, TALL *132
+//   8192 x 1024 -> 1024 over 16: ROUND 102, LARGE 101, TALL *97                         200 x 512 -> 512 over 64: ROUND 32.5, LARGE 32.7, TALL *28.9
+//   16384 x 512 -> 512, one group: LARGE *60.6, TALL 71.4                               3000 x 2048 -> 4096: SMALL 285, WIDE 241, ROUND *193, LARGE 203
 //   1000 x 520 -> 776 over 12: SMALL *22.7, WIDE 30.2, ROUND 35.4, LARGE 35.7   2000 x 1024 -> 1024: SMALL 35.0, WIDE *28.0, ROUND 45.3
 //   5000 x 768 -> 1536 over 4: SMALL 77.4, WIDE *74.5, ROUND 67.6, LARGE 75.7   (one of those where it is wrong)
 // and of the splits, dense, at the best tiles for each:
 //   16384 x 512 -> 512 1: 107, 4: 64, 16: *58    10000 x 256 -> 256 1: 66, 8: 26.0, 16: *27.1 (others 30)    8192 x 2048 -> 512 1: 90, 4: *77, 8: 99
 //   8192 x 1024 -> 1024 1: 86, 4: *81, 8: 98     4096 x 1024 -> 2048 1: *79, 2: 93
-// Environment: UNIT_AMD_GATED_PAIR=1..4 pins the tiles, UNIT_AMD_GATED_SPLITS the splits.
-enum PairTiles { PAIR_SMALL, PAIR_WIDE, PAIR_ROUND, PAIR_LARGE };
+// Environment: UNIT_AMD_GATED_PAIR=1..5 pins the tiles, UNIT_AMD_GATED_SPLITS the splits.
+enum PairTiles { PAIR_SMALL, PAIR_WIDE, PAIR_ROUND, PAIR_LARGE, PAIR_TALL };
 struct PairPlan {
   PairTiles tiles;
   int splits, split_rows;  // rows of a split: whole stages of 64

@@ -79,6 +79,7 @@ int run_gated_pair_sizes(const char *what, const char *tag, const GroupedParams 
     case PAIR_SMALL: return run_gated_pair<Op, Tile<64, 64, 128, 2, 1, false, 2>, 4, Tile<128, 128, 64, 2, 2>, 4, OutX, OutW>(what, tag, px, pw, plan, s);
     case PAIR_WIDE: return run_gated_pair<Op, W, 3, W, 3, OutX, OutW>(what, tag, px, pw, plan, s);
     case PAIR_ROUND: return run_gated_pair<Op, Tile<192, 256, 128, 2, 4>, 2, L, 2, OutX, OutW>(what, tag, px, pw, plan, s);
+    case PAIR_TALL: return run_gated_pair<Op, Tile<128, 256, 64, 2, 2>, 3, Tile<128, 256, 64, 2, 2>, 3, OutX, OutW>(what, tag, px, pw, plan, s);
     default: return run_gated_pair<Op, L, 2, L, 2, OutX, OutW>(what, tag, px, pw, plan, s);
   }
 }
