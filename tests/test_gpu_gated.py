@@ -203,13 +203,14 @@ def test_gradients_are_the_differences_of_the_forward(dev, act):
 
 def test_large_tiles(dev):
     """Tiles of the largest sizes, ragged on every side, where the rules take them; against 64 bits as above."""
-    for sizes, rows, n, k in ((None, 4100, 1544, 776), ([1500, 0, 700, 1801], 4006, 1032, 520), ([256] * 12 + [9], 3081, 1280, 1032)):
+    for sizes, rows, n, k in ((None, 4100, 1544, 776), ([1500, 0, 700, 1801], 4006, 1032, 520), ([256] * 12 + [9], 3081, 1280, 1032), ([500, 700, 300] * 5, 7500, 1024, 1024)):
         x, w = randn((rows, k), "bfloat16", 7, dev), randn((() if sizes is None else (len(sizes),)) + (2 * n, k), "bfloat16", 8, dev, k ** -0.5)
         s = None if sizes is None else torch.tensor(sizes, device=dev)
         h, off, pre, pre_off = forward(x, w, sizes, "silu")
         got, kept = U.gated_dense(x, w, s, "silu", "bfloat16", keep="pre")
         near(got, h, off, "bfloat16")
         near(kept, pre, pre_off, "bfloat16")
+        assert torch.equal(got, U.gated_dense(x, w, s, "silu", "bfloat16")) and torch.equal(got, U.gated_dense(x, w, s, "silu", "bfloat16", keep="mxfp8")[0])
 
 
 @pytest.mark.parametrize("tile", [1, 2, 3, 4, 5, 6, 7, 8])

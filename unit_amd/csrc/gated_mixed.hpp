@@ -1,5 +1,5 @@
-// Gated products by tiles of two sizes in one launch: a group's rows by 256 x 128 columns, but for a remainder of 160 rows at most, which goes by
-// 128 x 64.  Groups that end inside a large tile cost a launch of few rounds a good part of one; small tiles come last and fill the
+// Gated products by tiles of two sizes in one launch: a group's rows by 256 x 128 columns, but for a remainder of `most` rows or fewer, which goes
+// by 128 x 64.  Groups that end inside a large tile cost a launch of few rounds a good part of one; small tiles come last and fill the
 // CUs that the large ones leave.
 #pragma once
 #include "grouped_tile.hpp"

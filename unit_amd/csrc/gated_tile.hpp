@@ -33,11 +33,12 @@ struct GatedTiling {
   int most = 128;  // MIXED: rows of a remainder that goes by small tiles
 };
 
-// LARGE, ROUND or MIXED: the least of their estimates.  A tile costs a start, its stages of 64 elements and its results (twice as much again where
-// pre-activations are kept); tiles are dealt to 256 CUs, large ones first.  A group ends anywhere in a large tile.  Of 42 problems of 2200 to
-// 16384 rows the one that it takes is 1.3 % slower than the best on average, 13 % at most (LARGE or ROUND alone: 7.7 and 30).
-inline GatedTiling large_tiles(const GatedParams &p, long groups, bool kept) {
-  const double stages = p.k / 64.0, large = 1 + 1.62 * stages + 6 * kept, wide = 1 + 0.45 * stages + 2 * kept;
+// LARGE, ROUND or MIXED: the least of their estimates.  A tile costs a start with its results, and its stages of 64 elements; tiles are dealt to
+// 256 CUs, large ones first.  A group ends anywhere in a large tile.  Of 42 problems of 2200 to 16384 rows the one that it takes is 1.3 % slower
+// than the best on average, 13 % at most (LARGE or ROUND alone: 7.7 and 30).  What is kept does not enter: it would change no choice of those,
+// and h has the same bits with it and without.
+inline GatedTiling large_tiles(const GatedParams &p, long groups) {
+  const double stages = p.k / 64.0, large = 4 + 1.62 * stages, wide = 2 + 0.45 * stages;
   const long cols = (p.n + 127) / 128, wide_cols = (p.n + 63) / 64;
   const auto dealt = [](double front, double tf, double back, double tb) {
     const double rounds = (double)(long)(front / 256), left = front - 256 * rounds;
@@ -60,7 +61,7 @@ inline GatedTiling large_tiles(const GatedParams &p, long groups, bool kept) {
   return best;
 }
 
-inline GatedTiling gated_tile_size(const GatedParams &p, bool kept) {
+inline GatedTiling gated_tile_size(const GatedParams &p) {
   if (const int pinned = tuning_override("UNIT_AMD_GATED_TILE")) {
     const int most = tuning_override("UNIT_AMD_GATED_MOST");
     return {static_cast<GatedTile>(pinned - 1), most > 0 && most < 256 ? most : 128};
@@ -69,7 +70,7 @@ inline GatedTiling gated_tile_size(const GatedParams &p, bool kept) {
   const auto tiles = [&](int x, int y) { return (mean + x - 1) / x * ((p.n + y - 1) / y) * busy; };
   if (tiles(64, 32) <= 256) return {GATED_NARROW};
   if (mean <= 16) return {GATED_FEW};
-  if (mean >= 128 && p.n >= 96 && p.k >= 256 && tiles(256, 128) >= 128 && mean * p.n * 2 * busy >= (1l << 32) / p.k) return large_tiles(p, busy, kept);
+  if (mean >= 128 && p.n >= 96 && p.k >= 256 && tiles(256, 128) >= 128 && mean * p.n * 2 * busy >= (1l << 32) / p.k) return large_tiles(p, busy);
   const long middle = tiles(128, 64);
   if (middle >= 140 && middle <= 256 && p.k >= 1024 && mean >= 128) return {GATED_WIDE};
   return {middle >= 192 && mean >= 192 ? GATED_MIDDLE : GATED_SMALL};
@@ -81,7 +82,7 @@ int run_gated_sizes(const char *what, const char *tag, const GatedParams &p, hip
     if (p.rows <= kSplitRows && !tuning_override("UNIT_AMD_GATED_TILE")) return run_gated_split<typename Op::half_t, Out, GATE>(what, tag, p, s);
   // LARGE keeps pre-activations of 16 bits in lines of 64 columns a wave: 16384 x 1024 -> 1024 over 32 107.4 us by 32 columns, 104.0 so
   constexpr int WX = GATE == GATE_KEEP ? 4 : 2;
-  const GatedTiling t = gated_tile_size(p, GATE != GATE_ONLY);
+  const GatedTiling t = gated_tile_size(p);
   switch (t.tile) {
     case GATED_NARROW: return run_grouped_tile<Op, FORWARD, Tile<64, 64, 128, 2, 1, false, 2>, 4, Out, GATE>(what, tag, p, s);
     case GATED_FEW: return run_grouped_tile<Op, FORWARD, Tile<32, 128, 128, 1, 2, false, 2>, 4, Out, GATE>(what, tag, p, s);

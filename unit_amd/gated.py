@@ -65,7 +65,7 @@ def gated_dense(data, weight, group_sizes=None, activation="silu", out_dtype="fl
     (E,), weight (E, 2 N, K) and rows sorted by expert as in grouped_dense (rows of no expert give zeros).
     activation "silu", z / (1 + exp(-z)), or "gelu_tanh", z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2.
     keep: what comes back beside out for gated_dense_grad's `pre`, gate . data[r] and up . data[r] as (rows, 2, N): "pre" a tensor of
-    data's type, "mxfp8" an Mxfp8Tensor, a quarter of a float32's size; None nothing, and out alone is returned."""
+    data's type, "mxfp8" an Mxfp8Tensor, a quarter of a float32's size; None nothing, and out alone is returned.  out is the same to the bit."""
     done = _native_gated.gated(data, weight, group_sizes, activation, out_dtype, keep)
     if done is not None:
         return done
