@@ -215,12 +215,12 @@ __device__ __forceinline__ int cols_swz(int row) {
 
 // 32 rows of results of a wave, BLOCKS * 32 columns: put in order in LDS of the wave's own, then written in runs of 16 bytes a lane.
 // rows: that LDS; dst: column 0 of the first of `high` rows that are `ld` elements apart and have `width` columns; y: the wave's first
-// column; value(j, r): columns 32 j + 8 r + 4 half .. + 3 of row l32.
+// column; value(j, r): columns 32 j + 8 r + 4 half .. + 3 of row l32.  lines: the wave's columns are whole lines that nothing reads soon: nt.
 template <class E, int BLOCKS>
 struct RowsOut {
   static constexpr int ES = (int)sizeof(E), PITCH = BLOCKS * 32 * ES + 16, PER = 16 / ES, RUNS = BLOCKS * 32 / PER;  // elements per run, runs per row
   template <class F>
-  static __device__ __forceinline__ void put(char *rows, char *dst, long ld, int high, int width, int y, F value) {
+  static __device__ __forceinline__ void put(char *rows, char *dst, long ld, int high, int width, int y, F value, bool lines = false) {
     const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
     typedef E v4e __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -240,7 +240,9 @@ struct RowsOut {
       const v4u v = *reinterpret_cast<const v4u *>(rows + row * PITCH + c * ES);
       if (row >= high || at >= width) continue;
       const u32 off = ((u32)row * (u32)ld + (u32)at) * (u32)ES;
-      if (ld % PER == 0 && at + PER <= width) {
+      if (lines) {
+        store_result<kResultPolicy>(out, off, v);
+      } else if (ld % PER == 0 && at + PER <= width) {
         store_result<kRowPolicy>(out, off, v);
       } else if (at + PER <= width) {  // rows begin on any element: the same 16 bytes, unaligned
         typedef u32 v4un __attribute__((ext_vector_type(4), aligned(2)));
@@ -372,9 +374,12 @@ __device__ __forceinline__ void gated_results(const GatedParams &p, char *rows, 
     const long row = row0 + x0 + i * 32;
     auto part = [&](int j, int r) __attribute__((always_inline)) { return v4f{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]}; };
     if constexpr (GATE == GATE_KEEP) {
+      // Read in the backward pass: they would only push operands and h out of the memory-side cache (16384 x 1024 -> 1024 over 32: 103 us, 99.8
+      // like this; 8192 rows over 16: 48.3, 45.3)
+      const bool lines = CB == 2 && p.n % 64 == 0;
       char *pre = p.pre + row * 2 * p.n * 2;
-      RowsOut<Half, CB>::put(rows, pre, 2l * p.n, left, p.n, y, part);
-      RowsOut<Half, CB>::put(rows, pre + 2l * p.n, 2l * p.n, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) { return part(j + CB, r); });
+      RowsOut<Half, CB>::put(rows, pre, 2l * p.n, left, p.n, y, part, lines);
+      RowsOut<Half, CB>::put(rows, pre + 2l * p.n, 2l * p.n, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) { return part(j + CB, r); }, lines);
     }
     RowsOut<Out, CB>::put(rows, p.out + row * p.n * (long)sizeof(Out), p.n, left, p.n, y, [&](int j, int r) __attribute__((always_inline)) {
       const v4f g = part(j, r), u = part(j + CB, r);
