@@ -23,6 +23,7 @@ struct GroupedParams {
   int groups, rows;        // groups, rows of the row operands
   int n, k;                // weight (groups, n, k)
   int x_dtype;             // MXFP4 products: UNIT_MXFP4, or UNIT_F16 / UNIT_BF16 for x still in floats
+  int past_caches = 0;     // weight gradients of 16 bits in whole lines: nt
 };
 
 __device__ __forceinline__ int group_size(const GroupedParams &p, int g) {

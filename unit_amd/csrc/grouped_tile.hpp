@@ -752,7 +752,7 @@ __device__ __forceinline__ void compute_tile(const GateParams<GATE> &p, char *ld
       const v4u v = *reinterpret_cast<const v4u *>(rows + row * PITCH + c * ES_OUT);
       if (x >= high || y >= ys) continue;
       const u32 at = ((u32)x * (u32)ys + (u32)y) * (u32)ES_OUT;
-      if (DIR == GRAD_WEIGHT && ES_OUT == 4 && lines) {
+      if (DIR == GRAD_WEIGHT && (ES_OUT == 4 ? lines : p.past_caches && ys % 64 == 0)) {
         store_result<kResultPolicy>(out, at, v);
       } else if (whole) {
         store_result<kRowPolicy>(out, at, v);
