@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from unit_amd import experts as X
+from unit_amd.grouped import Mxfp4Tensor, Mxfp8Tensor
 
 
 def _groups(sizes, rows):
@@ -123,3 +124,21 @@ def test_arguments_are_refused_by_name():
             call()
     with pytest.raises(TypeError, match="x: expected dtype"):
         X.gated_linear(x.double(), w.double())
+
+
+def test_what_is_no_tensor_is_refused():
+    x, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(32, 64, dtype=torch.bfloat16)
+    codes = torch.zeros(20000, dtype=torch.uint8)
+    x4, w4, x8 = Mxfp4Tensor(codes, (4, 64)), Mxfp4Tensor(codes, (32, 64)), Mxfp8Tensor(codes, (4, 64))
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad):
+            for bad in (x4, x8, [1.0]):
+                with pytest.raises(TypeError, match="x: expected a torch.Tensor"):
+                    X.gated_linear(bad, w)
+                with pytest.raises(TypeError, match="x: expected a torch.Tensor"):
+                    X.expert_linear(bad, w[None], torch.tensor([4]))
+            for bad in (w4, None):
+                with pytest.raises(TypeError, match="weight: expected a torch.Tensor"):
+                    X.gated_linear(x, bad)
+                with pytest.raises(TypeError, match="weight: expected a torch.Tensor"):
+                    X.expert_linear(x, bad, torch.tensor([4]))

@@ -25,6 +25,12 @@ def _name(x):
         raise TypeError(f"x: expected dtype {' or '.join(str(d) for d in _NAME)}, got {x.dtype}") from None
 
 
+def _tensors(x, weight):
+    for name, t in (("x", x), ("weight", weight)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+
+
 def _aligned(grad):
     grad = grad.contiguous()
     if grad.data_ptr() % 16:  # a part of a larger gradient (torch.cat's, say): the kernels read 16 bytes at a time
@@ -68,6 +74,7 @@ def expert_linear(x, weight, group_sizes, keep=None):
     keep "mxfp8": x is kept for it in 8 bits."""
     if keep not in (None, "mxfp8"):
         raise ValueError(f"keep: expected None or 'mxfp8', got {keep!r}")
+    _tensors(x, weight)
     return _ExpertLinear.apply(x, weight, group_sizes, keep)
 
 
@@ -98,6 +105,7 @@ def gated_linear(x, weight, group_sizes=None, activation="silu", keep="pre"):
     if keep not in ("pre", "mxfp8", "rows"):
         raise ValueError(f"keep: expected 'pre', 'mxfp8' or 'rows', got {keep!r}")
     _activation(activation)
+    _tensors(x, weight)
     if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad):
         return gated_dense(x, weight, group_sizes, activation, _name(x))
     return _GatedLinear.apply(x, weight, group_sizes, activation, keep)
