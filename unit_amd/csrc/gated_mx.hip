@@ -28,7 +28,7 @@ int run(const char *what, const GatedParams &p, hipStream_t s) {
 
 // as grouped_mx_takes_floats: one launch for everything, where the chip holds its workgroups at once
 bool gated_mx_takes_floats(const GroupedParams &p) {
-  return (p.x_dtype == UNIT_F16 || p.x_dtype == UNIT_BF16) && p.k % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && grouped_split_pays(p);
+  return (p.x_dtype == UNIT_F16 || p.x_dtype == UNIT_BF16) && p.k % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && grouped_split_pays(p, 2);
 }
 
 int run_gated_mx(const char *what, const GatedParams &p, int out_dtype, hipStream_t s) {

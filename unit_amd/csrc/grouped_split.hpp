@@ -136,10 +136,13 @@ __global__ __launch_bounds__(KW * 64, 2) void grouped_split(GateParams<GATE> p, 
   }
 }
 
-// Which products take it: as many workgroups as the chip holds at once.  More rows or columns are better off quantised once.
-inline bool grouped_split_pays(const GroupedParams &p) {
+// Which products take it: as many workgroups as the chip holds at once.  More rows or columns are better off quantised once.  Of a unit's two
+// planes of scales, four bytes a row of all groups' weights, the second is reached by a 32-bit offset within a descriptor of 2^31 - 1 bytes:
+// where a plane and sixteen rows would pass it (2^29 rows, 64 GiB of codes) the tiles take over, whose offsets are of 64 bits.  halves: 2 of a
+// gated product
+inline bool grouped_split_pays(const GroupedParams &p, int halves = 1) {
   const long parts = p.sizes ? (p.groups + 1 < p.rows ? p.groups + 1 : p.rows) : 1;
-  return p.rows <= 16 && parts * ceil_div(p.n, 16) <= 512;
+  return p.rows <= 16 && parts * ceil_div(p.n, 16) <= 512 && (long)p.groups * halves * p.n < (1l << 29) - 16;
 }
 
 template <class X, class Out, int GATE = GATE_NONE>
