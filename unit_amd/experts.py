@@ -9,6 +9,7 @@ import sys
 import time
 
 import torch
+from torch.autograd import forward_ad
 
 from .gated import _activation, _gated_grad, gated_dense, gated_dense_grad, gated_dense_mxfp4
 from .grouped import Mxfp4Tensor, Mxfp8Tensor, _grouped_grad, grouped_dense, grouped_dense_grad, grouped_dense_mxfp4, quantize_mxfp4, quantize_mxfp8
@@ -29,6 +30,16 @@ def _tensors(x, weight):
     for name, t in (("x", x), ("weight", weight)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+
+
+def _derived(x, weight):
+    """whether a derivative may be asked for: in the backward pass, or in forward mode, whose tangents an autograd function refuses and a
+    bare product would drop"""
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return True
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside of any level nothing has a tangent: asking each operand takes a microsecond
+        return False
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in (x, weight))
 
 
 def _aligned(grad):
@@ -99,14 +110,14 @@ class _GatedLinear(torch.autograd.Function):
 
 
 def gated_linear(x, weight, group_sizes=None, activation="silu", keep="pre"):
-    """gated_dense in x's type, differentiable in x and weight, once.  keep: what it holds until then beside the weight, bytes per row of
+    """gated_dense in x's type, differentiable in x and weight, once, by the backward pass alone (forward mode is refused).  keep: what it holds until then beside the weight, bytes per row of
     16-bit operands: "pre" x and the pre-activations (2 K + 4 N), "mxfp8" both in 8 bits (K + 2 N and a thirty-second), "rows" x alone
     (2 K): the pre-activations are computed again."""
     if keep not in ("pre", "mxfp8", "rows"):
         raise ValueError(f"keep: expected 'pre', 'mxfp8' or 'rows', got {keep!r}")
     _activation(activation)
     _tensors(x, weight)
-    if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad):
+    if not _derived(x, weight):
         return gated_dense(x, weight, group_sizes, activation, _name(x))
     return _GatedLinear.apply(x, weight, group_sizes, activation, keep)
 
