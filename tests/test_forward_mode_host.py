@@ -62,3 +62,19 @@ def test_a_level_without_tangents_keeps_nothing():
     x, w = operands()
     with forward_ad.dual_level():
         assert X.gated_linear(x, w).grad_fn is None
+
+
+@pytest.mark.parametrize("gate", [None, "silu"])
+def test_layer_of_mxfp4_weights_refuses_tangents_of_its_rows(monkeypatch, gate):
+    product = lambda x, w, *rest: torch.full((x.shape[0], 6 if w.shape[1] == 12 else w.shape[1]), 0.5, dtype=x.dtype)
+    monkeypatch.setattr(X, "grouped_dense_mxfp4", product)
+    monkeypatch.setattr(X, "gated_dense_mxfp4", product)
+    weight = lambda *shape: X.Mxfp4Tensor(torch.empty(0, dtype=torch.uint8), shape)
+    layer = X.ExpertLayer(weight(3, 12 if gate else 6, 16), weight(3, 16, 6), 2, gate)
+    x, logits = torch.randn(5, 16), torch.randn(5, 3)
+    with forward_ad.dual_level():
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="x: carries a forward-mode tangent"):
+                layer(forward_ad.make_dual(x, torch.ones_like(x)), logits)
+        y = layer(x, forward_ad.make_dual(logits, torch.ones_like(logits)))  # the router's derivative is whole
+        assert forward_ad.unpack_dual(y).tangent is not None

@@ -174,8 +174,11 @@ class ExpertLayer:
             raise ValueError(f"x: expected two axes, got shape {tuple(x.shape)}")
         if tuple(logits.shape) != (x.shape[0], self.up.shape[0]):
             raise ValueError(f"logits: expected ({x.shape[0]}, {self.up.shape[0]}), got {tuple(logits.shape)}")
-        if isinstance(self.up, Mxfp4Tensor) and x.requires_grad and torch.is_grad_enabled():
-            raise ValueError("x: requires a gradient, which a layer with MXFP4 weights has none of; detach it or use torch.no_grad()")
+        if isinstance(self.up, Mxfp4Tensor):
+            if x.requires_grad and torch.is_grad_enabled():
+                raise ValueError("x: requires a gradient, which a layer with MXFP4 weights has none of; detach it or use torch.no_grad()")
+            if _derived(x, x):
+                raise ValueError("x: carries a forward-mode tangent, which a layer with MXFP4 weights has no derivative for")
         order, token, sizes, share = route(logits, self.top_k)
         if isinstance(self.up, Mxfp4Tensor):
             product = lambda a, w: grouped_dense_mxfp4(a, w, sizes, name)  # noqa: E731
