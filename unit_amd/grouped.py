@@ -334,6 +334,8 @@ def grouped_dense(data, weight, group_sizes, out_dtype="float32"):
     if out is not None:
         return out
     dt = _out_dtype(out_dtype)
+    if isinstance(data, Mxfp8Tensor):
+        raise TypeError("data: expected a torch.Tensor, got Mxfp8Tensor (which grouped_dense_grad takes)")
     data, weight, sizes, e, n, k = _grouped(data, weight, group_sizes)
     out = torch.empty((data.shape[0], n), dtype=dt, device=data.device)
     check(_lib.load().unit_grouped_dense(data.data_ptr(), weight.data_ptr(), sizes.data_ptr(), sizes.element_size(), out.data_ptr(),
