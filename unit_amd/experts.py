@@ -22,14 +22,14 @@ _NAME = {torch.float32: "float32", torch.float16: "float16", torch.bfloat16: "bf
 def _name(x):
     try:
         return _NAME[x.dtype]
-    except KeyError:
+    except (KeyError, AttributeError):
+        _tensor(x, "x")
         raise TypeError(f"x: expected dtype {' or '.join(str(d) for d in _NAME)}, got {x.dtype}") from None
 
 
-def _tensors(x, weight):
-    for name, t in (("x", x), ("weight", weight)):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+def _tensor(t, name, kinds=torch.Tensor, expected="a torch.Tensor"):
+    if not isinstance(t, kinds):
+        raise TypeError(f"{name}: expected {expected}, got {type(t).__name__}")
 
 
 def _derived(x, weight):
@@ -85,7 +85,8 @@ def expert_linear(x, weight, group_sizes, keep=None):
     keep "mxfp8": x is kept for it in 8 bits."""
     if keep not in (None, "mxfp8"):
         raise ValueError(f"keep: expected None or 'mxfp8', got {keep!r}")
-    _tensors(x, weight)
+    _tensor(x, "x")
+    _tensor(weight, "weight")
     return _ExpertLinear.apply(x, weight, group_sizes, keep)
 
 
@@ -116,7 +117,8 @@ def gated_linear(x, weight, group_sizes=None, activation="silu", keep="pre"):
     if keep not in ("pre", "mxfp8", "rows"):
         raise ValueError(f"keep: expected 'pre', 'mxfp8' or 'rows', got {keep!r}")
     _activation(activation)
-    _tensors(x, weight)
+    _tensor(x, "x")
+    _tensor(weight, "weight")
     if not _derived(x, weight):
         return gated_dense(x, weight, group_sizes, activation, _name(x))
     return _GatedLinear.apply(x, weight, group_sizes, activation, keep)
@@ -148,6 +150,8 @@ class ExpertLayer:
             raise ValueError(f"keep: expected 'pre', 'mxfp8' or 'rows', got {keep!r}")
         if gate is None and keep != "pre":
             raise ValueError(f"keep: {keep!r} is of a layer with a gate")
+        for name, t in (("up", up), ("down", down)):
+            _tensor(t, name, (torch.Tensor, Mxfp4Tensor), "a torch.Tensor or an Mxfp4Tensor")
         times, width = (1, "hidden") if gate is None else (2, "2 * hidden")
         if not len(up.shape) == len(down.shape) == 3 or up.shape[0] != down.shape[0] or up.shape[1] != times * down.shape[2] or up.shape[2] != down.shape[1]:
             raise ValueError(f"up {tuple(up.shape)}, down {tuple(down.shape)}: expected (E, {width}, model) and (E, model, hidden)")
@@ -159,6 +163,8 @@ class ExpertLayer:
 
     def quantized(self):
         """The same layer with MXFP4 weights."""
+        if isinstance(self.up, Mxfp4Tensor):
+            raise TypeError("quantized: the layer's weights are in MXFP4 already")
         return ExpertLayer(quantize_mxfp4(self.up.detach()), quantize_mxfp4(self.down.detach()), self.top_k, self.gate, self.keep)
 
     def _hidden(self, x, sizes, product):
@@ -172,6 +178,7 @@ class ExpertLayer:
         name = _name(x)
         if x.dim() != 2:
             raise ValueError(f"x: expected two axes, got shape {tuple(x.shape)}")
+        _tensor(logits, "logits")
         if tuple(logits.shape) != (x.shape[0], self.up.shape[0]):
             raise ValueError(f"logits: expected ({x.shape[0]}, {self.up.shape[0]}), got {tuple(logits.shape)}")
         if isinstance(self.up, Mxfp4Tensor):
