@@ -87,6 +87,8 @@ def expert_linear(x, weight, group_sizes, keep=None):
         raise ValueError(f"keep: expected None or 'mxfp8', got {keep!r}")
     _tensor(x, "x")
     _tensor(weight, "weight")
+    if not _derived(x, weight):
+        return grouped_dense(x, weight, group_sizes, _name(x))
     return _ExpertLinear.apply(x, weight, group_sizes, keep)
 
 
