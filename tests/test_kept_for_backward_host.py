@@ -76,3 +76,42 @@ def test_evaluating_a_layer_quantises_nothing(ran):
     with torch.no_grad():
         layer(torch.randn(5, 16), torch.zeros(5, 1))
     assert ran == ["grouped"]
+
+
+def held(y):
+    """elements that the function holds beside the weight and the sizes"""
+    return [None if t is None else t.numel() for t in y.grad_fn.saved_tensors]
+
+
+@pytest.mark.parametrize("keep", ["pre", "mxfp8", "rows"])
+@pytest.mark.parametrize("trained", ["x", "w", "both"])
+def test_gated_linear_holds_rows_that_are_read_again(ran, keep, trained):
+    x, w = operands()
+    x.requires_grad_(trained != "w"), w.requires_grad_(trained != "x")
+    y = X.gated_linear(x, w, None, "silu", keep)
+    rows = 7 * 16 if trained != "x" or keep == "rows" else None
+    assert held(y) == [rows, 12 * 16, None, None if keep == "rows" else 7 * 12]
+    assert ran.count("quantize") == (1 if keep == "mxfp8" and rows else 0)
+    y.square().sum().backward()
+    a, b = (t.detach().clone().requires_grad_() for t in (x, w))
+    p = (a @ b.T).unflatten(-1, (2, -1))
+    (torch.nn.functional.silu(p[:, 0]) * p[:, 1]).square().sum().backward()
+    assert (x.grad is None) == (trained == "w") and (w.grad is None) == (trained == "x")
+    for ours, want in ((x.grad, a.grad), (w.grad, b.grad)):  # float32 sums of some tens of products, in another order
+        assert ours is None or torch.allclose(ours, want, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("keep", [None, "mxfp8"])
+@pytest.mark.parametrize("trained", ["x", "w", "both"])
+def test_expert_linear_holds_rows_that_are_read_again(ran, keep, trained):
+    x, w = operands(1)
+    x.requires_grad_(trained != "w"), w.requires_grad_(trained != "x")
+    y = X.expert_linear(x, w, torch.tensor([7]), keep)
+    assert held(y)[:2] == [None if trained == "x" else 7 * 16, 12 * 16]
+    assert ran.count("quantize") == (1 if keep == "mxfp8" and trained != "x" else 0)
+    y.square().sum().backward()
+    a, b = (t.detach().clone().requires_grad_() for t in (x, w))
+    (a @ b[0].T).square().sum().backward()
+    assert (x.grad is None) == (trained == "w") and (w.grad is None) == (trained == "x")
+    for ours, want in ((x.grad, a.grad), (w.grad, b.grad)):
+        assert ours is None or torch.allclose(ours, want, rtol=1e-4, atol=1e-4)

@@ -64,11 +64,23 @@ def _kept(ctx):
     return [t if shape is None else Mxfp8Tensor(t, shape) for t, shape in zip(ctx.saved_tensors, ctx.shapes)]
 
 
+def _rows_kept(ctx, x, keep):
+    """the rows as the backward pass reads them: for the weight's gradient, or to compute pre-activations again; None where it does neither"""
+    if not ctx.needs_input_grad[1] and keep != "rows":
+        return None
+    return quantize_mxfp8(x) if keep == "mxfp8" else x
+
+
+def _unread(weight, grad):
+    """in the place of rows that were not kept: of their shape, an element's memory"""
+    return weight.new_empty(()).expand(grad.shape[0], weight.shape[-1])
+
+
 class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, group_sizes, keep):
         ctx.name = _name(x)
-        _keep(ctx, quantize_mxfp8(x) if keep == "mxfp8" else x, weight, group_sizes)
+        _keep(ctx, _rows_kept(ctx, x, keep), weight, group_sizes)
         return grouped_dense(x, weight, group_sizes, _name(x))
 
     @staticmethod
@@ -76,13 +88,14 @@ class _ExpertLinear(torch.autograd.Function):
         _once("expert_linear")
         x, weight, group_sizes = _kept(ctx)
         wanted = ctx.needs_input_grad[:2]  # a frozen operand's gradient is not computed
+        x = _unread(weight, grad) if x is None else x
         args = x, weight, _aligned(grad), group_sizes, ctx.name, _NAME[weight.dtype]
         return *(grouped_dense_grad(*args) if all(wanted) else _grouped_grad(*args, wanted)), None, None
 
 
 def expert_linear(x, weight, group_sizes, keep=None):
     """grouped_dense in x's type, differentiable in x and weight, once: a backward pass with create_graph=True is refused.
-    keep "mxfp8": x is kept for it in 8 bits."""
+    x is held for it where the weight asks for a gradient; keep "mxfp8": in 8 bits."""
     if keep not in (None, "mxfp8"):
         raise ValueError(f"keep: expected None or 'mxfp8', got {keep!r}")
     _tensor(x, "x")
@@ -100,7 +113,7 @@ class _GatedLinear(torch.autograd.Function):
             h, pre = gated_dense(x, weight, group_sizes, activation, _name(x)), None
         else:
             h, pre = gated_dense(x, weight, group_sizes, activation, _name(x), keep=keep)
-        _keep(ctx, quantize_mxfp8(x) if keep == "mxfp8" else x, weight, group_sizes, pre)
+        _keep(ctx, _rows_kept(ctx, x, keep), weight, group_sizes, pre)
         return h
 
     @staticmethod
@@ -108,6 +121,7 @@ class _GatedLinear(torch.autograd.Function):
         _once("gated_linear")
         x, weight, group_sizes, pre = _kept(ctx)
         wanted = ctx.needs_input_grad[:2]
+        x = _unread(weight, grad) if x is None else x
         args = x, weight, _aligned(grad), group_sizes, ctx.activation, pre, ctx.name, _NAME[weight.dtype]
         return *(gated_dense_grad(*args) if all(wanted) else _gated_grad(*args, wanted)), None, None, None
 
@@ -115,7 +129,7 @@ class _GatedLinear(torch.autograd.Function):
 def gated_linear(x, weight, group_sizes=None, activation="silu", keep="pre"):
     """gated_dense in x's type, differentiable in x and weight, once, by the backward pass alone (forward mode is refused).  keep: what it holds until then beside the weight, bytes per row of
     16-bit operands: "pre" x and the pre-activations (2 K + 4 N), "mxfp8" both in 8 bits (K + 2 N and a thirty-second), "rows" x alone
-    (2 K): the pre-activations are computed again."""
+    (2 K): the pre-activations are computed again.  With a frozen weight x is held for "rows" alone."""
     if keep not in ("pre", "mxfp8", "rows"):
         raise ValueError(f"keep: expected 'pre', 'mxfp8' or 'rows', got {keep!r}")
     _activation(activation)

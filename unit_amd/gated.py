@@ -28,9 +28,9 @@ def _activation(name):
         raise ValueError(f"activation: expected 'silu' or 'gelu_tanh', got {name!r}") from None
 
 
-def _gated(data, weight, group_sizes):
-    """data, weight, the groups as the library takes them, (rows, groups, N, K)"""
-    if not isinstance(data, Mxfp8Tensor):
+def _gated(data, weight, group_sizes, read=True):
+    """data, weight, the groups as the library takes them, (rows, groups, N, K); read: the rows' elements are, not their shape alone"""
+    if not isinstance(data, Mxfp8Tensor) and read:
         data = _floats(data, "data", _HALVES, 2)
     weight = _floats(weight, "weight", _HALVES, 2 if group_sizes is None else 3)
     if not isinstance(data, Mxfp8Tensor) and weight.dtype != data.dtype:
@@ -148,7 +148,8 @@ def gated_dense_grad(data, weight, grad, group_sizes=None, activation="silu", pr
 def _gated_grad(data, weight, grad, group_sizes, activation, pre, out_dtype, weight_out_dtype, wanted=(True, True)):
     """(ddata, dweight), None in the place of one that is not wanted"""
     act, dt, wdt = _activation(activation), _out_dtype(out_dtype), _out_dtype(weight_out_dtype, "weight_out_dtype")
-    data, weight, sizes, (rows, e, n, k) = _gated(data, weight, group_sizes)
+    read = wanted[1] or pre is None  # dx from kept pre-activations takes nothing from the rows
+    data, weight, sizes, (rows, e, n, k) = _gated(data, weight, group_sizes, read)
     grad = _dev(grad, "grad", weight.dtype, 2)
     _same_device(grad, "grad", weight)
     if tuple(grad.shape) != (rows, n):
@@ -160,7 +161,7 @@ def _gated_grad(data, weight, grad, group_sizes, activation, pre, out_dtype, wei
             raise ValueError(f"pre: expected ({rows}, 2, {n}), got {tuple(pre.shape)}")
         _same_device(pre, "pre", weight)
     L, code = _lib.load(), _CODE[weight.dtype]
-    x = (*data._pointers()[:2], _MXFP8) if isinstance(data, Mxfp8Tensor) else (data.data_ptr(), None, code)
+    x = (None, None, code) if not read else (*data._pointers()[:2], _MXFP8) if isinstance(data, Mxfp8Tensor) else (data.data_ptr(), None, code)
     kept = (None, None, 0) if pre is None else (*pre._pointers()[:2], _MXFP8) if isinstance(pre, Mxfp8Tensor) else (pre.data_ptr(), None, code)
     need = ctypes.c_size_t()
     check(L.unit_gated_dense_grad_ws_bytes(x[2], code, rows, e, n, k, ctypes.byref(need)))

@@ -308,8 +308,9 @@ _NAME = {v: k for k, v in _OUT.items()}
 _HALVES = (torch.float16, torch.bfloat16)
 
 
-def _grouped(data, weight, group_sizes):
-    if isinstance(data, Mxfp8Tensor):
+def _grouped(data, weight, group_sizes, read=True):
+    """read: the rows' elements are, not their shape alone"""
+    if isinstance(data, Mxfp8Tensor) or not read:
         weight = _floats(weight, "weight", _HALVES, 3)
     else:
         data = _floats(data, "data", _HALVES, 2)
@@ -356,7 +357,7 @@ def grouped_dense_grad(data, weight, grad, group_sizes, out_dtype="float32", wei
 def _grouped_grad(data, weight, grad, group_sizes, out_dtype, weight_out_dtype, wanted=(True, True)):
     """(ddata, dweight), None in the place of one that is not wanted: it costs neither time nor memory"""
     dt, wdt = _out_dtype(out_dtype), _out_dtype(weight_out_dtype, "weight_out_dtype")
-    data, weight, sizes, e, n, k = _grouped(data, weight, group_sizes)
+    data, weight, sizes, e, n, k = _grouped(data, weight, group_sizes, wanted[1])
     grad = _dev(grad, "grad", weight.dtype, 2)
     _same_device(grad, "grad", data)
     rows = data.shape[0]
