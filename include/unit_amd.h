@@ -403,10 +403,13 @@ int unit_gated_dense_mxfp4(const void *x, const void *xscales, int32_t x_dtype, 
  * no group and for groups without rows.  x (rows, K) in dtype or in MXFP8 (x_dtype UNIT_MXFP8), not read where there is pre and no
  * dw; pre what unit_gated_dense kept, or NULL: gate x and up x are then computed from x again.  The gate's gradients, dh u act'(g) and
  * dh act(g), are computed in fp32 and rounded to dtype, the type of w, dh and of the products that follow; those sum in fp32 and
- * round once to dx_dtype and dw_dtype (UNIT_F32 or dtype).  ws: unit_gated_dense_grad_ws_bytes, 16-byte aligned, of any
- * contents, the call's alone until it has run on the stream. */
+ * round once to dx_dtype and dw_dtype (UNIT_F32 or dtype).  ws: unit_gated_dense_grad_ws_bytes, or where one of dx and dw is NULL
+ * unit_gated_dense_grad_one_ws_bytes (x_dtype: dtype where x is not read), 16-byte aligned, of any contents, the call's alone until
+ * it has run on the stream. */
 int unit_gated_dense_grad_ws_bytes(int32_t x_dtype, int32_t dtype, int32_t rows, int32_t groups, int32_t N, int32_t K,
                                    size_t *bytes);
+int unit_gated_dense_grad_one_ws_bytes(int32_t x_dtype, int32_t dtype, int32_t rows, int32_t groups, int32_t N, int32_t K,
+                                       size_t *bytes);
 int unit_gated_dense_grad(const void *x, const void *x_scales, int32_t x_dtype, const void *w, const void *dh, const void *pre,
                           const void *pre_scales, int32_t pre_dtype, const void *sizes, int32_t size_bytes, void *dx,
                           int32_t dx_dtype, void *dw, int32_t dw_dtype, int32_t dtype, int32_t activation, int32_t rows,

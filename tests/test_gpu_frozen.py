@@ -78,3 +78,32 @@ def test_evaluation_takes_no_checkpoint(dev):
     assert torch.equal(got, want) and got.grad_fn is None
     with torch.no_grad():
         assert torch.equal(expert_linear(x.clone().requires_grad_(), w, sizes, keep="mxfp8"), want)
+
+
+def peak_of(call):
+    """bytes that `call` has allocated at a time, its results among them"""
+    call()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = call()
+    return torch.cuda.max_memory_allocated() - before, out
+
+
+@pytest.mark.parametrize("keep", ["pre", "mxfp8", "rows"])
+def test_a_single_gradient_takes_its_own_workspace(dev, keep):
+    """The gate's gradients; for dw, or where pre-activations are computed again, the rows restored from MXFP8.  No sums of dw's splits."""
+    from unit_amd.gated import _gated_grad
+    rows, n, k = 10000, 256, 256  # whose dw alone is shared out to many workgroups beside dx
+    x, w = operands(rows, 0, 2 * n, k, dev)
+    seed = torch.randn((rows, n), generator=torch.Generator().manual_seed(5)).bfloat16().to(dev)
+    pre = None if keep == "rows" else U.gated_dense(x, w, None, "silu", "bfloat16", keep=keep)[1]
+    data = U.quantize_mxfp8(x) if keep != "pre" else x
+    blocks = lambda b: -(-b // 512) * 512  # of the allocator
+    want = U.gated_dense_grad(data, w, seed, None, "silu", pre, "bfloat16", "bfloat16")
+    restored = -(-rows * k * 2 // 256) * 256 if keep != "pre" else 0
+    for wanted, result, x16 in (((True, False), rows * k * 2, restored if pre is None else 0), ((False, True), 2 * n * k * 2, restored)):
+        peak, both = peak_of(lambda: _gated_grad(data, w, seed, None, "silu", pre, "bfloat16", "bfloat16", wanted))
+        assert peak == blocks(rows * n * 4 + x16) + blocks(result), (wanted, peak)
+        i = wanted.index(True)
+        assert both[1 - i] is None and float((both[i].double() - want[i].double()).norm() / want[i].double().norm()) <= 2 * 2.0 ** -8

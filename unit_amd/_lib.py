@@ -64,6 +64,7 @@ SYMBOLS = (
     "unit_gated_dense",
     "unit_gated_dense_mxfp4",
     "unit_gated_dense_grad_ws_bytes",
+    "unit_gated_dense_grad_one_ws_bytes",
     "unit_gated_dense_grad",
     "unit_mxfp8_bytes",
     "unit_quantize_mxfp8",
@@ -161,7 +162,8 @@ def load():
     L.unit_grouped_dense_mxfp4.argtypes = [vp, vp, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, vp, size, vp]
     L.unit_gated_dense.argtypes = [vp, vp, vp, i32, vp, i32, i32, i32, vp, vp, i32, i32, i32, i32, i32, vp]
     L.unit_gated_dense_mxfp4.argtypes = [vp, vp, i32, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, size, vp]
-    L.unit_gated_dense_grad_ws_bytes.argtypes = [i32, i32, i32, i32, i32, i32, sizep]
+    for name in ("unit_gated_dense_grad_ws_bytes", "unit_gated_dense_grad_one_ws_bytes"):
+        getattr(L, name).argtypes = [i32, i32, i32, i32, i32, i32, sizep]
     L.unit_gated_dense_grad.argtypes = [vp, vp, i32, vp, vp, vp, vp, i32, vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, size, vp]
     L.unit_mxfp8_bytes.argtypes = [i64, i32, sizep, sizep]
     L.unit_quantize_mxfp8.argtypes = [vp, i32, i64, i32, vp, vp, vp]

@@ -224,14 +224,14 @@ extern "C" int unit_gated_dense_mxfp4(const void *x, const void *xscales, int32_
 
 namespace {
 
-// The parts of the workspace of a gradient: dpre, the rows restored from MXFP8, float32 sums of dw's splits
+// The parts of the workspace of a gradient: dpre, the rows restored from MXFP8, float32 sums of dw's splits (of one group's dw beside dx)
 struct GradParts {
   size_t dpre, x, sums;
-  GradParts(int x_dtype, int rows, int groups, int N, int K) {
+  GradParts(bool restored, bool shared_out, int rows, int N, int K) {
     const auto lines = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
-    const int splits = groups == 1 && rows ? gated_pair_plan(rows, 1, true, 2 * N, K).splits : 1;
+    const int splits = shared_out && rows ? gated_pair_plan(rows, 1, true, 2 * N, K).splits : 1;
     dpre = lines((size_t)rows * N * 4);
-    x = x_dtype == UNIT_MXFP8 ? lines((size_t)rows * K * 2) : 0;
+    x = restored ? lines((size_t)rows * K * 2) : 0;
     sums = splits > 1 ? (size_t)splits * N * K * 8 : 0;
   }
   size_t bytes() const { return dpre + x + sums; }
@@ -247,12 +247,23 @@ int check_grad_shape(const char *what, int x_dtype, int dtype, int rows, int gro
 
 }  // namespace
 
-extern "C" int unit_gated_dense_grad_ws_bytes(int32_t x_dtype, int32_t dtype, int32_t rows, int32_t groups, int32_t N, int32_t K, size_t *bytes) {
-  const char *what = "unit_gated_dense_grad_ws_bytes";
+namespace {
+
+int workspace(const char *what, bool both, int x_dtype, int dtype, int rows, int groups, int N, int K, size_t *bytes) {
   if (int rc = check_grad_shape(what, x_dtype, dtype, rows, groups, N, K)) return rc;
   if (!bytes) return fail(UNIT_E_ARG, "%s: null pointer", what);
-  *bytes = GradParts(x_dtype, rows, groups, N, K).bytes();
+  *bytes = GradParts(x_dtype == UNIT_MXFP8, both && groups == 1, rows, N, K).bytes();
   return UNIT_OK;
+}
+
+}  // namespace
+
+extern "C" int unit_gated_dense_grad_ws_bytes(int32_t x_dtype, int32_t dtype, int32_t rows, int32_t groups, int32_t N, int32_t K, size_t *bytes) {
+  return workspace("unit_gated_dense_grad_ws_bytes", true, x_dtype, dtype, rows, groups, N, K, bytes);
+}
+
+extern "C" int unit_gated_dense_grad_one_ws_bytes(int32_t x_dtype, int32_t dtype, int32_t rows, int32_t groups, int32_t N, int32_t K, size_t *bytes) {
+  return workspace("unit_gated_dense_grad_one_ws_bytes", false, x_dtype, dtype, rows, groups, N, K, bytes);
 }
 
 extern "C" int unit_gated_dense_grad(const void *x, const void *x_scales, int32_t x_dtype, const void *w, const void *dh, const void *pre, const void *pre_scales,
@@ -267,7 +278,7 @@ extern "C" int unit_gated_dense_grad(const void *x, const void *x_scales, int32_
   if (dw && dw_dtype != UNIT_F32 && dw_dtype != dtype) return fail(UNIT_E_ARG, "%s: out_dtype of dw must be UNIT_F32 or dtype, got %d", what, dw_dtype);
   if (pre && pre_dtype != dtype && pre_dtype != UNIT_MXFP8) return fail(UNIT_E_ARG, "%s: pre_dtype must be dtype or UNIT_MXFP8, got %d", what, pre_dtype);
   const bool needs_x = dw || !pre, x8 = x_dtype == UNIT_MXFP8;
-  const GradParts parts(x_dtype, rows, groups, N, K);
+  const GradParts parts(x8 && needs_x, dx && dw && !sizes, rows, N, K);
   if (int rc = check_ptrs(what, rows, {w, dh, ws})) return rc;
   if (int rc = check_ptrs(what, rows && needs_x, {x})) return rc;
   if (int rc = check_aligned(what, {pre, dx, dw})) return rc;

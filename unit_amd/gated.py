@@ -164,7 +164,8 @@ def _gated_grad(data, weight, grad, group_sizes, activation, pre, out_dtype, wei
     x = (None, None, code) if not read else (*data._pointers()[:2], _MXFP8) if isinstance(data, Mxfp8Tensor) else (data.data_ptr(), None, code)
     kept = (None, None, 0) if pre is None else (*pre._pointers()[:2], _MXFP8) if isinstance(pre, Mxfp8Tensor) else (pre.data_ptr(), None, code)
     need = ctypes.c_size_t()
-    check(L.unit_gated_dense_grad_ws_bytes(x[2], code, rows, e, n, k, ctypes.byref(need)))
+    workspace = L.unit_gated_dense_grad_ws_bytes if all(wanted) else L.unit_gated_dense_grad_one_ws_bytes
+    check(workspace(x[2], code, rows, e, n, k, ctypes.byref(need)))
     with _on(weight):
         ws = torch.empty((need.value,), dtype=torch.uint8, device=weight.device)
         ddata = torch.empty((rows, k), dtype=dt, device=weight.device) if wanted[0] else None
