@@ -314,8 +314,14 @@ extern "C" int unit_gated_dense_grad(const void *x, const void *x_scales, int32_
     const auto product = [&](const void *y, void *out) {
       return GroupedParams{dpre, static_cast<const char *>(y), nullptr, nullptr, static_cast<char *>(out), sizes, size_bytes, groups, rows, 2 * N, K};
     };
+    // dh, dpre, the rows and dx, w and dw; what was kept
+    const size_t weights = (size_t)groups * N * K * 4, half = (size_t)rows * N * 2;
+    const size_t kept = !pre ? 0 : pre_dtype == UNIT_MXFP8 ? mx8_code_bytes(2l * rows, N) : 2 * half;
+    const size_t moved = kept + 3 * half + (size_t)rows * K * (dx_dtype == UNIT_F32 ? 6 : 4) + 2 * weights;
+    GroupedParams pw = product(x, split ? sums : dw);
+    pw.past_caches = dw_past_caches(weights, moved, pre != nullptr);
     const auto run = dtype == UNIT_F16 ? run_gated_pair_f16 : run_gated_pair_bf16;
-    if (int rc = run(what, product(w, dx), dx_dtype, product(x, split ? sums : dw), split ? (int)UNIT_F32 : dw_dtype, plan, s)) return rc;
+    if (int rc = run(what, product(w, dx), dx_dtype, pw, split ? (int)UNIT_F32 : dw_dtype, plan, s)) return rc;
     return split ? add_splits(what, sums, dw, dw_dtype, 2l * N * K, plan.splits, s) : UNIT_OK;
   }
   if (dx)

@@ -79,6 +79,21 @@ struct PairPlan {
 // both: 2 N; one_group: no sizes.  A function of these values alone: the workspace's size goes by it.
 PairPlan gated_pair_plan(int rows, int groups, bool one_group, int both, int k);
 
+// Whether dw of 16 bits goes past the caches: it would push out of the memory-side cache (256 MiB) what the call has yet to read, w above all,
+// but what fits there is read back from it by the update that follows.  dw of 40 MiB, and either the pre-activations were computed from
+// the rows first (w is read twice) or the call moves 280 MiB in all (moved: every operand, intermediate and result once).  Measured with an update
+// of w by dw behind each call, us, through the caches and past them, * the one taken (rows x K -> N over groups; dw, moved):
+//   pre kept   1000 x 512 -> 1024 over 64 (128 MiB, 268): *122.4, 125.7     700 x 960 -> 1024 over 32 (120, 249): *114.6, 117.7
+//              6000 x 640 -> 1024 over 32 (80, 233): *119.4, 120.9          8192 x 384 -> 2048 over 16 (48, 268): *144.7, 146.4
+//              4096 x 768 -> 2048 over 16 (96, 284): 170.7, *168.5          8192 x 512 -> 2048 over 16 (64, 304): 168.9, *167.9
+//              3000 x 576 -> 512 over 128 (144, 309): 152.5, *145.2         4000 x 1024 -> 1024 over 64 (256, 567): 283, *273
+//   in MXFP8   4096 x 832 -> 1024 over 32 (104, 263): *129.5, 129.6         4096 x 960 -> 1024 over 32 (120, 299): 139.3, *138.1
+//   from rows  8192 x 256 -> 2048 over 16 (32 MiB): *123.5, 124.7           8192 x 384 -> 2048 over 16 (48): 169.3, *166.1
+//              4096 x 768 -> 2048 over 16 (96): 205, *181                   4096 x 1024 -> 1024 over 32 (128): 181, *175
+// Of 69 such pairs the choice is the slower one in six, by 2.2 % at most.  Timed without the update, calls from rows that move 265 to 320 MiB are up
+// to 7 % slower past the caches, the others as above.
+inline bool dw_past_caches(size_t dw_bytes, size_t moved, bool kept) { return dw_bytes >= (size_t)40 << 20 && (!kept || moved >= (size_t)280 << 20); }
+
 // px: dpre, w, dx; pw: dpre, x, dw (splits > 1: float32 sums of each split, one behind the other)
 int run_gated_pair_f16(const char *what, const GroupedParams &px, int dx_dtype, const GroupedParams &pw, int dw_dtype, const PairPlan &plan, hipStream_t s);
 int run_gated_pair_bf16(const char *what, const GroupedParams &px, int dx_dtype, const GroupedParams &pw, int dw_dtype, const PairPlan &plan, hipStream_t s);

@@ -56,9 +56,6 @@ int run_gated_pair(const char *what, const char *tag, const GroupedParams &px, G
   g.dw_nts = ceil_div(pw.k, TW::BY), g.dw_xts = ceil_div(pw.n, TW::BX);
   // at most: every group, and the rows of none, ends inside a tile; a multiple of the XCDs, so that both products are dealt to them alike
   if (plan.splits > 1) pw.groups = plan.splits;  // each with sums of its own
-  // dw of 2^27 bytes and more goes past the caches, which it would take from dpre and x.  us: 64 x 2048 x 1024 bf16 (268 MB) 132, 117 like this;
-  // 16 x 4096 x 1024 (134 MB) 182.5, 178.5; 16 x 2048 x 1024 (67 MB) 150.3, 153.5
-  pw.past_caches = (size_t)pw.groups * pw.n * pw.k * sizeof(OutW) >= (size_t)1 << 27;
   g.dw_parts = pw.groups;
   const long parts = px.sizes ? (px.groups + 1 < px.rows ? px.groups + 1 : px.rows) : 1;
   const long dx = ((px.rows + parts * (TX::BX - 1)) / TX::BX * g.dx_nts + 7 + 7) / 8 * 8, dw = (long)g.dw_parts * g.dw_nts * g.dw_xts;
