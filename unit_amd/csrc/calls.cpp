@@ -401,6 +401,9 @@ bool out_type(PyObject *o, at::ScalarType *t) {
   return false;
 }
 
+// work goes to the current device's stream: operands that live on another device are the Python operator's
+bool here(const at::Tensor &t) { return t.device().index() == c10::hip::current_device(); }
+
 // floats the library can be handed as they are, or null
 const at::Tensor *floats(PyObject *o, int *code) {
   if (!THPVariable_CheckExact(o)) return nullptr;
@@ -452,7 +455,7 @@ int without_gil(F &&call) {
 PyObject *quantize(PyObject *const *a, Py_ssize_t n) {
   int code;
   const at::Tensor *x = n == 1 ? floats(a[0], &code) : nullptr;
-  if (!x || x->dim() < 2 || x->dim() > 3 || !small(*x)) Py_RETURN_NONE;
+  if (!x || x->dim() < 2 || x->dim() > 3 || !small(*x) || !here(*x)) Py_RETURN_NONE;
   const int32_t k = (int32_t)x->size(-1);
   int64_t rows = 1;
   for (int i = 0; i + 1 < x->dim(); ++i) rows *= x->size(i);
@@ -476,7 +479,7 @@ PyObject *quantize(PyObject *const *a, Py_ssize_t n) {
 PyObject *dequantize(PyObject *const *a, Py_ssize_t n) {
   Mx q;
   at::ScalarType type;
-  if (n != 2 || !mx_operand(a[0], &q) || !out_type(a[1], &type)) Py_RETURN_NONE;
+  if (n != 2 || !mx_operand(a[0], &q) || !here(q.buf) || !out_type(a[1], &type)) Py_RETURN_NONE;
   at::Tensor out = result(q.buf, at::IntArrayRef(q.size, q.dims), type);
   void *s = stream(), *dst = out.data_ptr();
   char *src = q.data();
@@ -494,7 +497,7 @@ const at::Tensor *group_sizes(PyObject *o, int64_t groups, const at::Tensor &lik
 PyObject *product_mx(PyObject *const *a, Py_ssize_t n) {
   Mx w, q;
   at::ScalarType type;
-  if (n != 4 || !mx_operand(a[1], &w) || !out_type(a[3], &type)) Py_RETURN_NONE;
+  if (n != 4 || !mx_operand(a[1], &w) || !here(w.buf) || !out_type(a[3], &type)) Py_RETURN_NONE;
   const bool grouped = a[2] != Py_None;
   if (w.dims != (grouped ? 3 : 2)) Py_RETURN_NONE;
   const int32_t k = (int32_t)w.size[w.dims - 1], cols = (int32_t)w.size[w.dims - 2], groups = grouped ? (int32_t)w.size[0] : 1;
@@ -543,7 +546,7 @@ bool experts(PyObject *x, PyObject *w, PyObject *sizes, Experts *e) {
   e->x = floats(x, &e->code);
   if (!e->x || e->code == UNIT_F32 || e->x->dim() != 2 || !small(*e->x)) return false;
   e->w = operand(w, e->x->scalar_type(), 3);
-  if (!e->w || !small(*e->w) || e->w->size(2) != e->x->size(1) || e->w->device() != e->x->device()) return false;
+  if (!e->w || !small(*e->w) || e->w->size(2) != e->x->size(1) || e->w->device() != e->x->device() || !here(*e->x)) return false;
   e->rows = (int32_t)e->x->size(0), e->groups = (int32_t)e->w->size(0), e->cols = (int32_t)e->w->size(1), e->k = (int32_t)e->w->size(2);
   e->sizes = group_sizes(sizes, e->groups, *e->x);
   if (!e->sizes) return false;
@@ -584,9 +587,6 @@ PyObject *grouped_grad(PyObject *const *a, Py_ssize_t n) {
 }
 
 // ------------------------------------------------------------------------------- gated products and MXFP8
-// work goes to the current device's stream: operands that live on another device are the Python operator's
-bool here(const at::Tensor &t) { return t.device().index() == c10::hip::current_device(); }
-
 // an empty Mxfp8Tensor; its codes and scales
 PyObject *mx8_empty(const at::Tensor &like, at::IntArrayRef shape, char **codes, char **scales) {
   int64_t rows = 1;

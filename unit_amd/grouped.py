@@ -54,6 +54,13 @@ def _same_device(t, name, data):
         raise ValueError(f"{name}: lives on {t.device}, the data on {data.device}")
 
 
+def _on(t):
+    """the device that t lives on as the current one, so that its current stream is what the work runs on"""
+    if _device is not None and t.device.index == _device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
 class _GroupedCalls(_Calls):
     """The common case of this module's operators as native functions, like ops._Calls."""
 
@@ -117,9 +124,10 @@ def quantize_mxfp4(x):
     x = _floats(x, "x", tuple(_CODE))
     if x.dim() not in (2, 3):
         raise ValueError(f"x: expected two axes or three, got shape {tuple(x.shape)}")
-    q = _mxfp4_empty(x.shape, x.device)
-    codes, scales, rows, k = q._pointers()
-    check(_lib.load().unit_quantize_mxfp4(x.data_ptr(), _CODE[x.dtype], rows, k, codes, scales, _stream()))
+    with _on(x):
+        q = _mxfp4_empty(x.shape, x.device)
+        codes, scales, rows, k = q._pointers()
+        check(_lib.load().unit_quantize_mxfp4(x.data_ptr(), _CODE[x.dtype], rows, k, codes, scales, _stream()))
     return q
 
 
@@ -135,8 +143,10 @@ def dequantize_mxfp4(q, out_dtype="float32"):
     if out is not None:
         return out
     codes, scales, rows, k = _mxfp4(q, "q")._pointers()
-    out = torch.empty(q.shape, dtype=_out_dtype(out_dtype), device=q.device)
-    check(_lib.load().unit_dequantize_mxfp4(codes, scales, rows, k, out.data_ptr(), _CODE[out.dtype], _stream()))
+    dt = _out_dtype(out_dtype)
+    with _on(q.buf):
+        out = torch.empty(q.shape, dtype=dt, device=q.device)
+        check(_lib.load().unit_dequantize_mxfp4(codes, scales, rows, k, out.data_ptr(), _CODE[dt], _stream()))
     return out
 
 
@@ -153,9 +163,10 @@ def prepare_mxfp4_weight(codes, scales, k=None):
     k = 32 * b if k is None else int(k)
     if not 32 * (b - 1) < k <= 32 * b:
         raise ValueError(f"k: {k} elements do not fill {b} blocks of 32")
-    q = _mxfp4_empty((*codes.shape[:-1], k), codes.device)
-    to, sto, rows, _ = q._pointers()
-    check(_lib.load().unit_prepare_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, k, to, sto, _stream()))
+    with _on(codes):
+        q = _mxfp4_empty((*codes.shape[:-1], k), codes.device)
+        to, sto, rows, _ = q._pointers()
+        check(_lib.load().unit_prepare_mxfp4(codes.data_ptr(), scales.data_ptr(), rows, k, to, sto, _stream()))
     return q
 
 
@@ -170,28 +181,28 @@ def _mxfp4_product(data, weight, group_sizes, out_dtype, ndim):
     if len(data.shape) != 2 or data.shape[1] != k:
         raise ValueError(f"data: expected (rows, {k}), got {tuple(data.shape)}")
     _same_device(weight, "weight", data)
-    rows, ws = data.shape[0], None
-    if quantised:
-        x, xs = data._pointers()[:2]
-        operand = (x, xs, _MXFP4)
-    else:
-        need = ctypes.c_size_t()
-        check(_lib.load().unit_mxfp4_workspace_bytes(rows, k, ctypes.byref(need)))
-        ws = torch.empty((need.value,), dtype=torch.uint8, device=data.device)
-        operand = (data.data_ptr(), None, _CODE[data.dtype])
+    sizes = None
     if ndim == 3:
         sizes = _sizes(group_sizes, data)
         if sizes.shape[0] != weight.shape[0]:
             raise ValueError(f"group_sizes: expected {weight.shape[0]} entries, got {sizes.shape[0]}")
-    codes, scales = weight._pointers()[:2]
-    out = torch.empty((rows, n), dtype=dt, device=data.device)
-    tail = (None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _stream())
-    L = _lib.load()
-    if ndim == 2:
-        check(L.unit_dense_mxfp4(*operand, codes, scales, out.data_ptr(), _CODE[dt], rows, n, k, *tail))
-    else:
-        check(L.unit_grouped_dense_mxfp4(*operand, codes, scales, sizes.data_ptr(), sizes.element_size(), out.data_ptr(), _CODE[dt],
-                                         rows, weight.shape[0], n, k, *tail))
+    rows, ws, L = data.shape[0], None, _lib.load()
+    with _on(weight.buf):
+        if quantised:
+            operand = (*data._pointers()[:2], _MXFP4)
+        else:
+            need = ctypes.c_size_t()
+            check(L.unit_mxfp4_workspace_bytes(rows, k, ctypes.byref(need)))
+            ws = torch.empty((need.value,), dtype=torch.uint8, device=data.device)
+            operand = (data.data_ptr(), None, _CODE[data.dtype])
+        codes, scales = weight._pointers()[:2]
+        out = torch.empty((rows, n), dtype=dt, device=data.device)
+        tail = (None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _stream())
+        if ndim == 2:
+            check(L.unit_dense_mxfp4(*operand, codes, scales, out.data_ptr(), _CODE[dt], rows, n, k, *tail))
+        else:
+            check(L.unit_grouped_dense_mxfp4(*operand, codes, scales, sizes.data_ptr(), sizes.element_size(), out.data_ptr(), _CODE[dt],
+                                             rows, weight.shape[0], n, k, *tail))
     return out
 
 
@@ -211,13 +222,6 @@ def grouped_dense_mxfp4(data, weight, group_sizes, out_dtype="float32"):
 
 
 # ------------------------------------------------------------------------------- MXFP8
-def _on(t):
-    """the device that t lives on as the current one, so that its current stream is what the work runs on"""
-    if _device is not None and t.device.index == _device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
-
-
 def _mxfp8_bytes(rows, k):
     codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
     check(_lib.load().unit_mxfp8_bytes(rows, k, ctypes.byref(codes), ctypes.byref(scales)))
@@ -338,9 +342,10 @@ def grouped_dense(data, weight, group_sizes, out_dtype="float32"):
     if isinstance(data, Mxfp8Tensor):
         raise TypeError("data: expected a torch.Tensor, got Mxfp8Tensor (which grouped_dense_grad takes)")
     data, weight, sizes, e, n, k = _grouped(data, weight, group_sizes)
-    out = torch.empty((data.shape[0], n), dtype=dt, device=data.device)
-    check(_lib.load().unit_grouped_dense(data.data_ptr(), weight.data_ptr(), sizes.data_ptr(), sizes.element_size(), out.data_ptr(),
-                                         _CODE[data.dtype], _CODE[dt], data.shape[0], e, n, k, _stream()))
+    with _on(data):
+        out = torch.empty((data.shape[0], n), dtype=dt, device=data.device)
+        check(_lib.load().unit_grouped_dense(data.data_ptr(), weight.data_ptr(), sizes.data_ptr(), sizes.element_size(), out.data_ptr(),
+                                             _CODE[data.dtype], _CODE[dt], data.shape[0], e, n, k, _stream()))
     return out
 
 
@@ -363,16 +368,18 @@ def _grouped_grad(data, weight, grad, group_sizes, out_dtype, weight_out_dtype, 
     rows = data.shape[0]
     if tuple(grad.shape) != (rows, n):
         raise ValueError(f"grad: expected ({rows}, {n}), got {tuple(grad.shape)}")
-    L, tail = _lib.load(), (rows, e, n, k, _stream())
+    L = _lib.load()
     ddata = dweight = None
-    if wanted[0]:
-        ddata = torch.empty((rows, k), dtype=dt, device=weight.device)
-        check(L.unit_grouped_dense_grad_data(grad.data_ptr(), weight.data_ptr(), sizes.data_ptr(), sizes.element_size(), ddata.data_ptr(),
-                                             _CODE[weight.dtype], _CODE[dt], *tail))
-    if wanted[1]:
-        if isinstance(data, Mxfp8Tensor):
-            data = dequantize_mxfp8(data, _NAME[weight.dtype])
-        dweight = torch.empty((e, n, k), dtype=wdt, device=weight.device)
-        check(L.unit_grouped_dense_grad_weight(data.data_ptr(), grad.data_ptr(), sizes.data_ptr(), sizes.element_size(), dweight.data_ptr(),
-                                               _CODE[weight.dtype], _CODE[wdt], *tail))
+    with _on(weight):
+        tail = (rows, e, n, k, _stream())
+        if wanted[0]:
+            ddata = torch.empty((rows, k), dtype=dt, device=weight.device)
+            check(L.unit_grouped_dense_grad_data(grad.data_ptr(), weight.data_ptr(), sizes.data_ptr(), sizes.element_size(), ddata.data_ptr(),
+                                                 _CODE[weight.dtype], _CODE[dt], *tail))
+        if wanted[1]:
+            if isinstance(data, Mxfp8Tensor):
+                data = dequantize_mxfp8(data, _NAME[weight.dtype])
+            dweight = torch.empty((e, n, k), dtype=wdt, device=weight.device)
+            check(L.unit_grouped_dense_grad_weight(data.data_ptr(), grad.data_ptr(), sizes.data_ptr(), sizes.element_size(), dweight.data_ptr(),
+                                                   _CODE[weight.dtype], _CODE[wdt], *tail))
     return ddata, dweight
