@@ -45,7 +45,7 @@ int add_splits(const char *what, const void *parts, void *out, int out_dtype, lo
 }
 
 // dpre from dh and the pre-activations, eight columns a lane: 16 bytes of each of three operands in, of each of two results out (six,
-// eight and two in MXFP8), which is what it is bound by: 8192 x 2048, bf16, 168 MB in 28.7 us (5.8 TB/s).  Workgroups past the first `gates`
+// eight and two in MXFP8), which is what it is bound by: 8192 x 2048, bf16, 168 MB in 26.8 us (6.3 TB/s).  Workgroups past the first `gates`
 // restore rows from MXFP8 for the product that follows: a launch less (777 x 776 beside 777 x 1032: 8.0 us in two, 5.3 in one).
 template <class Half, bool MX8, int ROUNDS>
 __global__ __launch_bounds__(256) void gate_grad_kernel(const char *pre, const unsigned char *scales, const Half *dh, Half *dpre, int pieces, int N, Activation act,

@@ -1,6 +1,7 @@
 // Both products of a gated product's gradients in one launch: dx[r] = w^T dpre[r] and dw = sum dpre[r] x[r]^T, which have dpre in common and
 // nothing to wait for in each other.  Workgroups of the longer reduction come first, those of the other fill the CUs that the last round
-// of the first leaves idle.  us with the gate's gradients in front, bf16, rows x K -> N over groups (two launches; one):
+// of the first leaves idle.  us with the gate's gradients in front, bf16, rows x K -> N over groups (two launches; one; single runs side by
+// side: another card is off by up to a tenth, both alike):
 //   8192 x 1024 -> 2048 over 16: 212, 181    8192 x 1024 -> 1024 over 16: 114, 97    4000 x 768 -> 768 over 32: 83, 57
 //   1000 x 520 -> 776 over 12: 28.9, 23.3    300 x 1024 -> 1024: 20.2, 14.1          2000 x 1024 -> 1024: 41, 26
 //

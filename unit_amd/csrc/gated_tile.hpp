@@ -6,7 +6,7 @@
 namespace unit {
 
 // Which tile (rows x columns of h, each of which is a row of the gate's and of the up projection's weight).  us, bf16 unless said otherwise,
-// measured on both sides of each line (* the one taken):
+// measured on both sides of each line (* the one taken; single runs side by side: another card is off by up to a tenth, both sides alike):
 //   NARROW  64 x 32, two sets of waves that share the k-steps: one round of it.  Few tiles wait for their stages, each CU for its own: smaller
 //           ones are more of them.
 //             20 x 2048 -> 4096:           NARROW *9.5, SMALL 12.9    100 x 2048 -> 4096 (256 tiles): NARROW *10.2, SMALL 13.3

@@ -14,7 +14,8 @@ inline size_t mx8_scale_bytes(long rows, int K) { return (size_t)rows * mx8_bloc
 
 // The block's scale, biased by 127: the smallest power of two (2^-127 at least) for which the block's largest magnitude is at most
 // 448 = 1.75 * 2^8.  Nothing saturates: the formats' own rule, the exponent less 8 throughout, would cut magnitudes of 449 to 511
-// down to 448, up to an eighth off, where a rounding is off by a sixteenth at most.  amax_bits: that magnitude as a float's bits.
+// down to 448, up to an eighth off, where a rounding is off by a sixteenth at most (of an element of 2^-6 scales or more; below, in the
+// subnormal range, by 2^-10 scales, all of a smaller element).  amax_bits: that magnitude as a float's bits.
 __device__ __forceinline__ u32 mx8_scale(u32 amax_bits) {
   const u32 e = amax_bits >> 23, above = (amax_bits & 0x7fffffu) > 0x600000u;
   return e == 255 ? 255u : e + above < 8 ? 0u : e + above - 8;
