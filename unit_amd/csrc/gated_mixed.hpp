@@ -32,12 +32,9 @@ int run_gated_mixed(const char *what, const char *tag, const GatedParams &p, int
   constexpr int lds = 2 * TF::STAGE > NB * TB::STAGE ? 2 * TF::STAGE : NB * TB::STAGE;
   static_assert(lds <= kMaxLds && TF::NT == TB::NT && TF::BX == (int)kFront, "rings fit the LDS, workgroups are of one size");
   auto kern = gated_mixed<Op, TF, TB, NB, Out, GATE>;
-  static thread_local bool allowed = false;
-  if (!allowed && lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds);
-    if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: hipFuncSetAttribute: %s", what, hipGetErrorString(e));
-    allowed = true;
-  }
+  static thread_local unsigned long long allowed = 0;
+  if (lds > 65536)
+    if (int rc = allow_lds(what, reinterpret_cast<const void *>(kern), &allowed)) return rc;
   MixedGrid g;
   g.front_nts = ceil_div(p.n, TF::BY / 2), g.back_nts = ceil_div(p.n, TB::BY / 2);
   // at most: every group, and the rows of none, ends one row past the remainder that small tiles take; every one has such a remainder

@@ -46,12 +46,9 @@ int run_gated_pair(const char *what, const char *tag, const GroupedParams &px, G
   constexpr int lds = NX * TX::STAGE > NW * TW::STAGE ? NX * TX::STAGE : NW * TW::STAGE;
   static_assert(lds <= kMaxLds && TX::NT == TW::NT, "rings fit the LDS, workgroups are of one size");
   auto kern = gated_pair<Op, TX, NX, TW, NW, OutX, OutW>;
-  static thread_local bool allowed = false;
-  if (!allowed && lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds);
-    if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: hipFuncSetAttribute: %s", what, hipGetErrorString(e));
-    allowed = true;
-  }
+  static thread_local unsigned long long allowed = 0;
+  if (lds > 65536)
+    if (int rc = allow_lds(what, reinterpret_cast<const void *>(kern), &allowed)) return rc;
   PairGrid g;
   g.dx_nts = ceil_div(px.k, TX::BY);
   g.dw_nts = ceil_div(pw.k, TW::BY), g.dw_xts = ceil_div(pw.n, TW::BX);

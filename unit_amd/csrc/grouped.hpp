@@ -26,6 +26,20 @@ struct GroupedParams {
   int past_caches = 0;     // weight gradients of 16 bits in whole lines: nt
 };
 
+// More than 64 KiB of dynamic LDS for a kernel: granted to it on the current device, so asked for once a device (and thread).  allowed: of the
+// kernel, a bit per device that has granted it; devices past the 64th are asked every time.
+inline int allow_lds(const char *what, const void *kern, unsigned long long *allowed) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return fail(UNIT_E_DEVICE, "%s: hipGetDevice: %s", what, hipGetErrorString(e));
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (*allowed & bit) return UNIT_OK;
+  e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds);
+  if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: hipFuncSetAttribute: %s", what, hipGetErrorString(e));
+  *allowed |= bit;
+  return UNIT_OK;
+}
+
 __device__ __forceinline__ int group_size(const GroupedParams &p, int g) {
   if (!p.sizes) return p.rows;
   long s = p.size_bytes == 8 ? static_cast<const long *>(p.sizes)[g] : (long)static_cast<const int *>(p.sizes)[g];

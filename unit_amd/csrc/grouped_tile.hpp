@@ -797,12 +797,9 @@ int run_grouped_tile(const char *what, const char *tag, const GateParams<GATE> &
   constexpr int lds = NSTAGE * (T::STAGE + (Op::kMx ? ((T::BX + T::BY) * 8 + 1023) / 1024 * 1024 : 0));
   static_assert(lds <= kMaxLds, "ring does not fit the LDS");
   auto kern = grouped_tile<Op, DIR, T, NSTAGE, Out, GATE>;
-  static thread_local bool allowed = false;
-  if (!allowed && lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds);
-    if (e != hipSuccess) return fail(UNIT_E_LAUNCH, "%s: hipFuncSetAttribute: %s", what, hipGetErrorString(e));
-    allowed = true;
-  }
+  static thread_local unsigned long long allowed = 0;
+  if (lds > 65536)
+    if (int rc = allow_lds(what, reinterpret_cast<const void *>(kern), &allowed)) return rc;
   const int ys = DIR == FORWARD ? p.n : p.k, nts = ceil_div(ys, GATE ? T::BY / 2 : T::BY), xts = ceil_div(p.n, T::BX);
   long wgs;
   if (DIR == GRAD_WEIGHT) {
