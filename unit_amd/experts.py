@@ -127,9 +127,10 @@ class _GatedLinear(torch.autograd.Function):
 
 
 def gated_linear(x, weight, group_sizes=None, activation="silu", keep="pre"):
-    """gated_dense in x's type, differentiable in x and weight, once, by the backward pass alone (forward mode is refused).  keep: what it holds until then beside the weight, bytes per row of
-    16-bit operands: "pre" x and the pre-activations (2 K + 4 N), "mxfp8" both in 8 bits (K + 2 N and a thirty-second), "rows" x alone
-    (2 K): the pre-activations are computed again.  With a frozen weight x is held for "rows" alone."""
+    """gated_dense in x's type, differentiable in x and weight, once, by the backward pass alone (forward mode is refused).  keep: what it
+    holds until then beside the weight, bytes per row of 16-bit operands: "pre" x and the pre-activations (2 K + 4 N), "mxfp8" both in
+    8 bits (K + 2 N and a thirty-second), "rows" x alone (2 K): the pre-activations are computed again.  With a frozen weight x is held
+    for "rows" alone."""
     if keep not in ("pre", "mxfp8", "rows"):
         raise ValueError(f"keep: expected 'pre', 'mxfp8' or 'rows', got {keep!r}")
     _activation(activation)
